@@ -329,6 +329,156 @@ RQ_API int rq_llama_reset_tokens(rq_llama* m);
  * (src/streaming_quantized.rs:131-141,603-609): roll the KV length back. */
 RQ_API int rq_llama_truncate(rq_llama* m, int64_t new_len);
 
+/* ------------------------------------------------- paged serving operators */
+
+/* No counterpart in the reference, whose cache is one contiguous f32 buffer
+ * per layer and sequence (QuantStreamCache, src/streaming_quantized.rs:93-152).
+ * All pointers of this section are device memory on the context's device
+ * unless a comment says host; every call is asynchronous on `stream`, reads
+ * nothing back, allocates nothing and can be captured in a CUDA graph.  Sizes
+ * that a kernel reads from device memory (lengths, offsets, slots, table
+ * entries) are checked on the device: an index outside its range is skipped,
+ * as each comment says, never followed. */
+
+/* Element types of q, k, v, probabilities and outputs. */
+enum rq_dtype { RQ_F32 = 0, RQ_F16 = 1, RQ_BF16 = 2 };
+
+/* A paged key/value cache of one layer, held in 4 bits: n_pages pages of
+ * page_size positions (a multiple of 16, at most 4096; n_pages * page_size <
+ * 2^31) of n_kv_heads heads, head_dim 32, 64, 96 or 128.  Blocks of 32
+ * elements of a head's row: d = f16(m / -8) with m the element of largest
+ * magnitude (the first of equals; d saturates at 65504), code = the nearest
+ * multiple of d in 0..15 (ties up), value (code - 8) * d: 4.5 bits an
+ * element.  A NaN makes its block NaN.  Position `off` of page `p` is slot p *
+ * page_size + off.  Positions never written read as zeros. */
+typedef struct rq_kv4 rq_kv4;
+RQ_API int rq_kv4_create(rq_ctx* ctx, int64_t n_pages, int page_size, int n_kv_heads, int head_dim, rq_kv4** out);
+RQ_API int rq_kv4_free(rq_kv4* c);
+/* Any of the out-pointers may be NULL. */
+RQ_API int rq_kv4_info(const rq_kv4* c, int64_t* n_pages, int* page_size, int* n_kv_heads, int* head_dim,
+                       size_t* device_bytes);
+/* Quantizes the keys and values of n tokens into slots[n]; a slot outside
+ * the cache (-1: padding) is skipped.  k and v are [n][n_kv_heads][head_dim]
+ * with the given strides of token and head in elements (host array of two),
+ * elements contiguous.  The slots of one call must differ. */
+RQ_API int rq_kv4_append(rq_kv4* c, int dtype, const void* k, const int64_t k_stride[2], const void* v,
+                         const int64_t v_stride[2], const int32_t* slots, int64_t n, void* stream);
+/* k, v [n][n_kv_heads][head_dim] = the values held in slots[n] (zeros for a
+ * slot outside the cache). */
+RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, void* k, void* v, void* stream);
+
+/* Attention of the newest tokens of `batch` sequences over the cache.
+ * Sequence b holds kv_lens[b] positions, its newest tokens (already appended)
+ * among them; position j lives in page block_table[b * table_stride + j /
+ * page_size].  Its n queries are the rows cu_q[b] .. cu_q[b + 1] - 1 of q
+ * (n <= max_q; cu_q NULL: row b, n = 1), query i at position kv_lens[b] - n +
+ * i; it sees the positions j <= its own and, with window > 0, j > its own -
+ * window.  out row = softmax_j(scale * q . k_j) v over the seen positions, in
+ * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  A query
+ * that sees nothing gets zeros.  Positions behind table_width * page_size or
+ * on a page outside the cache are not seen.  Rows of q and out that belong to
+ * no sequence (or lie at or behind n_tokens) are left as they were.  out may
+ * be q.  max_len (> 0): an upper bound of kv_lens that only guides how the
+ * work is split (0: table_width * page_size).  `workspace` holds at least
+ * rq_kv4_attention_workspace bytes, used by this call alone until it is done
+ * (two captured graphs that may run at once need one each). */
+typedef struct rq_kv4_query {
+    int dtype;
+    const void* q;        /* [n_tokens][n_heads][head_dim] */
+    int64_t q_stride[2];  /* token, head; elements */
+    void* out;
+    int64_t out_stride[2];
+    int64_t n_tokens, n_heads, batch, max_q;
+    const int32_t* cu_q;        /* [batch + 1] or NULL */
+    const int32_t* kv_lens;     /* [batch] */
+    const int32_t* block_table; /* [batch][table_width] */
+    int64_t table_stride, table_width, max_len, window;
+    float scale;
+    void* workspace;
+    size_t workspace_bytes;
+} rq_kv4_query;
+RQ_API int rq_kv4_attention_workspace(const rq_kv4* c, const rq_kv4_query* a, size_t* bytes);
+RQ_API int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream);
+
+/* Per head of q and k: y = x / sqrt(mean(x^2) + eps) * weight (a NULL weight:
+ * y = x), then the first rot_dim elements rotated by the angles of the
+ * token's position (interleaved 0: element i with i + rot_dim / 2; 1: element
+ * 2i with 2i + 1).  cos, sin: f32 [max_pos][rot_dim / 2].  Computed in f32,
+ * rounded once.  A token whose position lies outside 0..max_pos-1 (-1:
+ * padding) leaves its output rows as they were.  q_out may be q and k_out may
+ * be k; otherwise outputs and inputs must not overlap.  n_heads or n_kv_heads
+ * may be 0.  head_dim even, at most 256. */
+typedef struct rq_qk_rope {
+    int dtype;
+    int64_t n_tokens, n_heads, n_kv_heads, head_dim, rot_dim;
+    int interleaved;
+    const void* q;
+    int64_t q_stride[2]; /* token, head; elements */
+    void* q_out;
+    int64_t q_out_stride[2];
+    const void* k;
+    int64_t k_stride[2];
+    void* k_out;
+    int64_t k_out_stride[2];
+    const float* q_weight; /* [head_dim] or NULL */
+    const float* k_weight;
+    float eps;
+    const float* cos;
+    const float* sin;
+    int64_t max_pos;
+    const int32_t* positions; /* [n_tokens] */
+} rq_qk_rope;
+RQ_API int rq_qk_norm_rope(rq_ctx* ctx, const rq_qk_rope* a, void* stream);
+/* The same in one launch with the append: the normalised, rotated k (k_out is
+ * not used) and v go to `slots` of the cache as rq_kv4_append would put them.
+ * A token whose position lies outside the tables is not appended either. */
+RQ_API int rq_qk_norm_rope_append(rq_kv4* c, const rq_qk_rope* a, const void* v, const int64_t v_stride[2],
+                                  const int32_t* slots, void* stream);
+
+/* Page bookkeeping of `batch` sequences, on the device.  The free pages are a
+ * ring of n_pages entries with state {head, free, short}: ring[(head + i) %
+ * n_pages], i < free.  extend: sequence b holds ctx_lens[b] positions in its
+ * first ceil(ctx_lens[b] / page_size) table entries and gets new_lens[b]
+ * more; the pages that these need are taken from the ring in the order of the
+ * sequences and written into the table.  Outputs: kv_lens[b] = ctx_lens[b] +
+ * new_lens[b] (may be ctx_lens), cu_new[batch + 1] the offsets of the new
+ * tokens, and for each of n_tokens rows (n_tokens >= the sum of new_lens; the
+ * rest is padding) its position and slot, -1 and -1 for padding.  Where the
+ * ring holds too few pages, `short` counts the missing ones and their table
+ * entries and slots are -1; a token behind the table's width gets slot -1.
+ * state_out may be state_in.  Negative lengths count as 0. */
+RQ_API int rq_pages_extend(rq_ctx* ctx, int64_t batch, int page_size, const int32_t* ctx_lens, const int32_t* new_lens,
+                           int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* ring,
+                           int64_t n_pages, const int32_t* state_in, int32_t* state_out, int32_t* kv_lens,
+                           int32_t* cu_new, int32_t* positions, int32_t* slots, int64_t n_tokens, void* stream);
+/* Gives back the pages of sequence b behind its first keep_lens[b] positions
+ * (of held_lens[b]): their table entries become -1 and the pages join the end
+ * of the ring, in the order of the sequences.  state {head, free, short}
+ * updated in place. */
+RQ_API int rq_pages_release(rq_ctx* ctx, int64_t batch, int page_size, const int32_t* held_lens,
+                            const int32_t* keep_lens, int32_t* table, int64_t table_stride, int64_t table_width,
+                            int32_t* ring, int64_t n_pages, int32_t* state, void* stream);
+
+/* Verification of drafted tokens (the sampled counterpart of the greedy
+ * accept of examples/spec_decode_70b.rs:262-283).  For sequence b with n =
+ * n_drafts[b] drafts (NULL: max_drafts): p row i (i = 0..n) are the target's
+ * probabilities after i accepted drafts, q row i (i < n) those the i-th draft
+ * was drawn from (q NULL: the draft was certain).  Draft i is accepted while
+ * u[b][i] * q_i(draft) < p_i(draft).  Then one token is drawn by r[b] in
+ * [0, 1): after a rejection at row i from max(p_i - q_i, 0) (from p_i where
+ * that has no mass), otherwise from p_n: the first j whose running sum of
+ * weights exceeds r * their total.  Sums and products in 64 bits.  NaN and
+ * negative probabilities count as 0, infinite ones as the largest finite
+ * value, an r outside [0, 1) as the nearest inside; a row without mass draws
+ * -1; a draft outside the vocabulary is rejected.  tokens[b] [max_drafts + 1] = the
+ * accepted drafts, the drawn token, then -1; accepted[b] their number.
+ * p [batch][max_drafts + 1][vocab] and q [batch][max_drafts][vocab] with
+ * strides of sequence and row in elements; drafts, u [batch][max_drafts]. */
+RQ_API int rq_spec_verify(rq_ctx* ctx, int dtype, const void* p, const int64_t p_stride[2], const void* q,
+                          const int64_t q_stride[2], const int32_t* drafts, const int32_t* n_drafts, const float* u,
+                          const float* r, int64_t batch, int64_t max_drafts, int64_t vocab, int32_t* tokens,
+                          int32_t* accepted, void* stream);
+
 /* ------------------------------------------------------------------- GGUF */
 
 /* A GGUF file read into host memory once (one sequential read, as

@@ -20,6 +20,14 @@ BLOCK_BYTES = {Q4_0: 18, Q8_0: 34, Q2_K: 84, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6
 BLOCK_ELEMS = {Q4_0: 32, Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 
 
+RQ_F32, RQ_F16, RQ_BF16 = 0, 1, 2
+try:  # torch element types of the paged serving operators
+    import torch
+    DTYPES = {torch.float32: RQ_F32, torch.float16: RQ_F16, torch.bfloat16: RQ_BF16}
+except Exception:  # pragma: no cover
+    DTYPES = {}
+
+
 class RqError(RuntimeError):
     """A non-zero status from librq; the message is rq_last_error()
     (the counterpart of the reference's ``Error::Msg``)."""
@@ -101,6 +109,40 @@ SIGNATURES.update({
     "rq_gguf_read_f32": (I, [P, ctypes.c_char_p, P, I64]),
     "rq_weight_upload_gguf": (I, [P, P, ctypes.c_char_p, I64, I64, I64, I64, PP]),
     "rq_llama_load_gguf_dir": (I, [P, ctypes.c_char_p]),
+})
+
+class Kv4Query(ctypes.Structure):
+    """rq_kv4_query of include/rq.h."""
+    _fields_ = [("dtype", I), ("q", P), ("q_stride", I64 * 2), ("out", P), ("out_stride", I64 * 2), ("n_tokens", I64),
+                ("n_heads", I64), ("batch", I64), ("max_q", I64), ("cu_q", P), ("kv_lens", P), ("block_table", P),
+                ("table_stride", I64), ("table_width", I64), ("max_len", I64), ("window", I64),
+                ("scale", ctypes.c_float), ("workspace", P), ("workspace_bytes", SZ)]
+
+
+class QkRope(ctypes.Structure):
+    """rq_qk_rope of include/rq.h."""
+    _fields_ = [("dtype", I), ("n_tokens", I64), ("n_heads", I64), ("n_kv_heads", I64), ("head_dim", I64),
+                ("rot_dim", I64), ("interleaved", I), ("q", P), ("q_stride", I64 * 2), ("q_out", P),
+                ("q_out_stride", I64 * 2), ("k", P), ("k_stride", I64 * 2), ("k_out", P), ("k_out_stride", I64 * 2),
+                ("q_weight", P), ("k_weight", P), ("eps", ctypes.c_float), ("cos", P), ("sin", P), ("max_pos", I64),
+                ("positions", P)]
+
+
+_STRIDES = ctypes.POINTER(I64)
+SIGNATURES.update({
+    "rq_kv4_create": (I, [P, I64, I, I, I, PP]),
+    "rq_kv4_free": (I, [P]),
+    "rq_kv4_info": (I, [P, ctypes.POINTER(I64), ctypes.POINTER(I), ctypes.POINTER(I), ctypes.POINTER(I),
+                        ctypes.POINTER(SZ)]),
+    "rq_kv4_append": (I, [P, I, P, _STRIDES, P, _STRIDES, P, I64, P]),
+    "rq_kv4_read": (I, [P, P, I64, I, P, P, P]),
+    "rq_kv4_attention_workspace": (I, [P, ctypes.POINTER(Kv4Query), ctypes.POINTER(SZ)]),
+    "rq_kv4_attention": (I, [P, ctypes.POINTER(Kv4Query), P]),
+    "rq_qk_norm_rope": (I, [P, ctypes.POINTER(QkRope), P]),
+    "rq_qk_norm_rope_append": (I, [P, ctypes.POINTER(QkRope), P, _STRIDES, P, P]),
+    "rq_pages_extend": (I, [P, I64, I, P, P, P, I64, I64, P, I64, P, P, P, P, P, P, I64, P]),
+    "rq_pages_release": (I, [P, I64, I, P, P, P, I64, I64, P, I64, P, P]),
+    "rq_spec_verify": (I, [P, I, P, _STRIDES, P, _STRIDES, P, P, P, P, I64, I64, I64, P, P, P]),
 })
 
 _lib = None

@@ -1,0 +1,636 @@
+// rq_kv4.cu -- the 4-bit paged key/value cache: create, append, read; and the
+// pass that normalises queries and keys per head and rotates them by their
+// positions, with or without the append in the same launch.  No counterpart
+// in the reference, whose cache is contiguous f32 (QuantStreamCache,
+// src/streaming_quantized.rs:93-152) and whose rotation is a pass of its own
+// (QAttn::forward, :201-240).
+
+#include <algorithm>
+#include <new>
+
+#include "rq_kv4.cuh"
+
+namespace rq {
+
+int check_device_ptr(const rq_ctx* ctx, const void* p, const char* fn, const char* name) {
+    if (!p) return set_error(RQ_ERR_INVALID, "%s: %s is NULL", fn, name);
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(RQ_ERR_INVALID, "%s: %s must be device memory", fn, name);
+    }
+    if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != ctx->device))
+        return set_error(RQ_ERR_INVALID, "%s: %s must be device memory on device %d", fn, name, ctx->device);
+    return RQ_OK;
+}
+
+int launch_pdl(const void* fn, unsigned grid, unsigned block, size_t smem, cudaStream_t st, void** args, const char* what,
+               unsigned cluster) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cuda_error(cudaLaunchKernelExC(&cfg, fn, args), what);
+}
+
+namespace {
+
+size_t dtype_size(int dtype) { return dtype == RQ_F32 ? 4 : dtype == RQ_F16 || dtype == RQ_BF16 ? 2 : 0; }
+
+bool wide_ok(const void* p, int64_t s0, int64_t s1, size_t size) {
+    return (((uintptr_t)p | (uintptr_t)(s0 * (int64_t)size) | (uintptr_t)(s1 * (int64_t)size)) & 15) == 0;
+}
+
+// ------------------------------------------------------------------ append
+//
+// One thread per 8 elements, the aligned four lanes holding a block of 32.
+// Bound by memory: 16 (or 32) bytes in, 4.5 out, per thread.
+struct AppendP {
+    const void* x[2];          // k, v
+    int64_t tok[2], head[2];   // strides in elements
+    bool wide[2];
+    const int32_t* slots;
+    int64_t n, n_slots;
+    uint8_t* data;
+    int page_size, n_kv, nb;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendP p) {
+    pdl_wait();
+    const int per = 4 * p.nb;
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t row = i / per;
+    if (row >= p.n * 2 * p.n_kv) return;
+    const int e = (int)(i - row * per);
+    const int64_t n = row / (2 * p.n_kv);
+    const int r = (int)(row - n * 2 * p.n_kv);
+    const bool is_v = r >= p.n_kv;
+    const int head = is_v ? r - p.n_kv : r;
+    const int32_t slot = p.slots[n];
+    float x[8];
+    load8(static_cast<const T*>(p.x[is_v]) + n * p.tok[is_v] + head * p.head[is_v] + 8 * e, p.wide[is_v], x);
+    uint8_t* rec = kv4_record(p.data, p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, head);
+    kv4_store(rec, p.nb, slot & 15, e >> 2, is_v, x);
+}
+
+// k and v rows of the given slots, dequantized; zeros for a slot outside the
+// cache.  The append's thread mapping.
+struct ReadP {
+    const uint8_t* data;
+    const int32_t* slots;
+    int64_t n, n_slots;
+    int page_size, n_kv, nb;
+    void* x[2];  // [n][n_kv][head_dim]
+    bool wide;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ ReadP p) {
+    pdl_wait();
+    const int per = 4 * p.nb;
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t row = i / per;
+    if (row >= p.n * 2 * p.n_kv) return;
+    const int e = (int)(i - row * per);
+    const int64_t n = row / (2 * p.n_kv);
+    const int r = (int)(row - n * 2 * p.n_kv);
+    const bool is_v = r >= p.n_kv;
+    const int head = is_v ? r - p.n_kv : r;
+    const int32_t slot = p.slots[n];
+    const uint8_t* rec =
+        kv4_record(const_cast<uint8_t*>(p.data), p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, head);
+    float x[8];
+    kv4_load(rec, p.nb, slot & 15, e >> 2, is_v, x);
+    store8(static_cast<T*>(p.x[is_v]) + (n * p.n_kv + head) * (32 * p.nb) + 8 * e, p.wide, x);
+}
+
+// --------------------------------------------------- norm and rotation
+//
+// y = x / sqrt(mean(x^2) + eps) * w per head (w NULL: y = x), then the first
+// rot elements rotated in pairs by the angles of the token's position.  A row
+// is cut into units of E elements (16 bytes, or one element where alignment
+// or sizes forbid that); a lane holds the unit with the first halves of its
+// pairs and the one with the second, so the rotation needs no exchange and a
+// row may be its own output.  Bound by memory; the lanes of a group keep
+// their cosines, sines and weights in registers over `hpg` heads of a token.
+struct RopeP {
+    const void* x[2];  // q, k
+    void* y[2];
+    int64_t xt[2], xh[2], yt[2], yh[2];  // strides in elements: token, head
+    const float* w[2];
+    const float* cos;
+    const float* sin;
+    const int32_t* pos;
+    int64_t n, max_pos;
+    int heads[2];
+    int hd, rot, inter, lpr, hpg;
+    float eps;
+};
+
+template <typename T, int E>
+__device__ __forceinline__ void load_unit(const T* __restrict__ p, float (&x)[E]) {
+    if constexpr (E == 1) {
+        x[0] = to_f32(p[0]);
+    } else {
+        T tmp[E];
+        *reinterpret_cast<uint4*>(tmp) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = to_f32(tmp[i]);
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_unit(T* p, const float (&x)[E]) {
+    if constexpr (E == 1) {
+        p[0] = from_f32<T>(x[0]);
+    } else {
+        T tmp[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) tmp[i] = from_f32<T>(x[i]);
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(tmp);
+    }
+}
+
+template <typename T, int E, int S>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeP p) {
+    pdl_wait();
+    const int lpr = p.lpr, lane = threadIdx.x & 31, sl = lane & (lpr - 1);
+    const unsigned group = (lpr == 32 ? 0xffffffffu : ((1u << lpr) - 1u)) << (lane & ~(lpr - 1));
+    const int64_t gi = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
+    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
+    const int64_t n = gi / (gq + gk);
+    if (n >= p.n) return;
+    int sub = (int)(gi - n * (gq + gk));
+    const int which = sub >= gq;
+    if (which) sub -= gq;
+    const int64_t pos = p.pos[n];
+    if (pos < 0 || pos >= p.max_pos) return;  // the row stays as it was
+    const int P = p.rot / (2 * E), rest = (p.hd - p.rot) / E;
+    int u0[S], u1[S];
+    float c0[S][E], s0[S][E], w0[S][E], w1[S][E];
+    const float* w = p.w[which];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const int i = sl + s * lpr;
+        const int r = 2 * (i - P);
+        u0[s] = i < P ? i : r < rest ? 2 * P + r : -1;
+        u1[s] = i < P ? i + P : r + 1 < rest ? 2 * P + r + 1 : -1;
+        // halves: the pair (e of u0, e of u1) turns by angle i E + e;
+        // interleaved: neighbours inside a unit, E / 2 angles a unit (E = 1
+        // is paired by index below)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            c0[s][e] = 1.0f;
+            s0[s][e] = 0.0f;
+            if (i < P) {
+                int64_t a;
+                if (!p.inter || E == 1) a = (int64_t)i * E + e;
+                else a = e < E / 2 ? (int64_t)u0[s] * (E / 2) + e : (int64_t)u1[s] * (E / 2) + (e - E / 2);
+                c0[s][e] = p.cos[pos * (p.rot / 2) + a];
+                s0[s][e] = p.sin[pos * (p.rot / 2) + a];
+            }
+        }
+        if (p.inter && E == 1 && i < P) {  // single elements: the pair is (2 i, 2 i + 1)
+            u0[s] = 2 * i;
+            u1[s] = 2 * i + 1;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            w0[s][e] = w && u0[s] >= 0 ? w[u0[s] * E + e] : 1.0f;
+            w1[s][e] = w && u1[s] >= 0 ? w[u1[s] * E + e] : 1.0f;
+        }
+    }
+    const int h0 = sub * p.hpg, h1 = min(h0 + p.hpg, p.heads[which]);
+    const T* xr = static_cast<const T*>(p.x[which]) + n * p.xt[which];
+    T* yr = static_cast<T*>(p.y[which]) + n * p.yt[which];
+    for (int h = h0; h < h1; h++) {
+        const T* x = xr + h * p.xh[which];
+        T* y = yr + h * p.yh[which];
+        float a[S][E], b[S][E];
+        float ss = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) a[s][e] = b[s][e] = 0.0f;
+            if (u0[s] >= 0) load_unit<T, E>(x + u0[s] * E, a[s]);
+            if (u1[s] >= 0) load_unit<T, E>(x + u1[s] * E, b[s]);
+        }
+        if (w) {
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int e = 0; e < E; e++) ss = fmaf(a[s][e], a[s][e], fmaf(b[s][e], b[s][e], ss));
+            for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+            const float r = 1.0f / sqrtf(ss / (float)p.hd + p.eps);
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    a[s][e] = a[s][e] * r * w0[s][e];
+                    b[s][e] = b[s][e] * r * w1[s][e];
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            if (sl + s * lpr < P) {
+                if (E == 1 || !p.inter) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const float f = a[s][e], g = b[s][e];
+                        a[s][e] = f * c0[s][e] - g * s0[s][e];
+                        b[s][e] = f * s0[s][e] + g * c0[s][e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e + 1 < E; e += 2) {
+                        float f = a[s][e], g = a[s][e + 1];
+                        a[s][e] = f * c0[s][e / 2] - g * s0[s][e / 2];
+                        a[s][e + 1] = f * s0[s][e / 2] + g * c0[s][e / 2];
+                        f = b[s][e];
+                        g = b[s][e + 1];
+                        b[s][e] = f * c0[s][E / 2 + e / 2] - g * s0[s][E / 2 + e / 2];
+                        b[s][e + 1] = f * s0[s][E / 2 + e / 2] + g * c0[s][E / 2 + e / 2];
+                    }
+                }
+            }
+            if (u0[s] >= 0) store_unit<T, E>(y + u0[s] * E, a[s]);
+            if (u1[s] >= 0) store_unit<T, E>(y + u1[s] * E, b[s]);
+        }
+    }
+}
+
+// The same with the append: 16 lanes a row of q, k or v (head_dim <= 128),
+// 8 consecutive elements a lane as the blocks of the cache want them; the
+// rotation's partner comes through shared memory.
+struct RopeAppendP {
+    RopeP r;  // y[1] unused
+    bool wide_q, wide_qo;
+    AppendP a;  // x[0] = k, x[1] = v
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(const __grid_constant__ RopeAppendP p) {
+    pdl_wait();
+    __shared__ float rows[16][132];
+    const int lane = threadIdx.x & 31, sl = lane & 15, gidx = threadIdx.x >> 4;
+    const int H = p.r.heads[0], kv = p.a.n_kv, per = H + 2 * kv, nb = p.a.nb, hd = 32 * nb;
+    const int64_t gi = (int64_t)blockIdx.x * 16 + gidx;
+    const int64_t n = gi / per;
+    bool live = n < p.a.n;
+    const int r = live ? (int)(gi - n * per) : 0;
+    const int kind = r < H ? 0 : r < H + kv ? 1 : 2;  // q, k, v
+    const int64_t pos = live ? p.r.pos[n] : -1;
+    live = live && pos >= 0 && pos < p.r.max_pos;
+    const bool mine = live && sl < 4 * nb;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    if (mine) {
+        if (kind == 0) load8(static_cast<const T*>(p.r.x[0]) + n * p.r.xt[0] + r * p.r.xh[0] + 8 * sl, p.wide_q, x);
+        else
+            load8(static_cast<const T*>(p.a.x[kind - 1]) + n * p.a.tok[kind - 1] +
+                      (r - H - (kind - 1) * kv) * p.a.head[kind - 1] + 8 * sl,
+                  p.a.wide[kind - 1], x);
+    }
+    if (kind < 2) {
+        const float* w = p.r.w[kind];
+        if (w) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffu << (lane & 16), ss, o);
+            const float s = 1.0f / sqrtf(ss / (float)hd + p.r.eps);
+            if (mine)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = x[i] * s * w[8 * sl + i];
+        }
+    }
+    float* row = rows[gidx];
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < 8; i++) row[8 * sl + i] = x[i];
+    __syncwarp();
+    if (mine && kind < 2) {
+        const int rot = p.r.rot, half = rot / 2;
+        const float* cs = p.r.cos + pos * half;
+        const float* sn = p.r.sin + pos * half;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = 8 * sl + i;
+            if (d < rot) {
+                int a, f, g;  // angle, first and second of the pair
+                if (p.r.inter) {
+                    a = d >> 1;
+                    f = d & ~1;
+                    g = f + 1;
+                } else {
+                    a = d < half ? d : d - half;
+                    f = a;
+                    g = a + half;
+                }
+                const float c = cs[a], s = sn[a];
+                x[i] = d == f ? row[f] * c - row[g] * s : row[f] * s + row[g] * c;
+            }
+        }
+    }
+    if (kind == 0) {
+        if (mine) store8(static_cast<T*>(p.r.y[0]) + n * p.r.yt[0] + r * p.r.yh[0] + 8 * sl, p.wide_qo, x);
+    } else {
+        const int head = r - H - (kind - 1) * kv;
+        uint8_t* rec = nullptr;
+        int tok = 0;
+        if (mine) {
+            const int32_t slot = p.a.slots[n];
+            rec = kv4_record(p.a.data, p.a.n_slots, p.a.page_size, kv, 576 * nb, slot, head);
+            tok = slot & 15;
+        }
+        kv4_store(rec, nb, tok, sl >> 2, kind == 2, x);
+    }
+}
+
+int check_cache(const rq_kv4* c, const char* fn) {
+    return c ? RQ_OK : set_error(RQ_ERR_INVALID, "%s: NULL cache", fn);
+}
+
+int check_rope(const rq_ctx* ctx, const rq_qk_rope* a, bool append, const char* fn) {
+    if (!ctx || !a) return set_error(RQ_ERR_INVALID, "%s: NULL argument", fn);
+    if (!dtype_size(a->dtype)) return set_error(RQ_ERR_UNSUPPORTED, "%s: dtype %d (f32 = 0, f16 = 1, bf16 = 2)", fn, a->dtype);
+    if (a->n_tokens < 0 || a->n_heads < 0 || a->n_kv_heads < 0 || a->n_heads > 65536 || a->n_kv_heads > 65536 ||
+        a->n_tokens > INT32_MAX)
+        return set_error(RQ_ERR_INVALID, "%s: %lld tokens, %lld / %lld heads", fn, (long long)a->n_tokens,
+                         (long long)a->n_heads, (long long)a->n_kv_heads);
+    if (a->head_dim < 2 || a->head_dim > 256 || a->head_dim % 2 || a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 2)
+        return set_error(RQ_ERR_INVALID, "%s: head_dim %lld (even, 2..256), rot_dim %lld (even, 0..head_dim)", fn,
+                         (long long)a->head_dim, (long long)a->rot_dim);
+    if (a->rot_dim && a->max_pos < 1) return set_error(RQ_ERR_INVALID, "%s: max_pos %lld", fn, (long long)a->max_pos);
+    int rc = RQ_OK;
+    if (a->n_tokens) {
+        if (!rc) rc = check_device_ptr(ctx, a->positions, fn, "positions");
+        if (!rc && a->n_heads) rc = check_device_ptr(ctx, a->q, fn, "q");
+        if (!rc && a->n_heads) rc = check_device_ptr(ctx, a->q_out, fn, "q_out");
+        if (!rc && a->n_kv_heads) rc = check_device_ptr(ctx, a->k, fn, "k");
+        if (!rc && a->n_kv_heads && !append) rc = check_device_ptr(ctx, a->k_out, fn, "k_out");
+        if (!rc && a->rot_dim) rc = check_device_ptr(ctx, a->cos, fn, "cos");
+        if (!rc && a->rot_dim) rc = check_device_ptr(ctx, a->sin, fn, "sin");
+        if (!rc && a->q_weight) rc = check_device_ptr(ctx, a->q_weight, fn, "q_weight");
+        if (!rc && a->k_weight) rc = check_device_ptr(ctx, a->k_weight, fn, "k_weight");
+    }
+    return rc;
+}
+
+RopeP rope_params(const rq_qk_rope* a) {
+    RopeP p{};
+    p.x[0] = a->q;
+    p.x[1] = a->k;
+    p.y[0] = a->q_out;
+    p.y[1] = a->k_out;
+    p.xt[0] = a->q_stride[0];
+    p.xh[0] = a->q_stride[1];
+    p.xt[1] = a->k_stride[0];
+    p.xh[1] = a->k_stride[1];
+    p.yt[0] = a->q_out_stride[0];
+    p.yh[0] = a->q_out_stride[1];
+    p.yt[1] = a->k_out_stride[0];
+    p.yh[1] = a->k_out_stride[1];
+    p.w[0] = a->q_weight;
+    p.w[1] = a->k_weight;
+    p.cos = a->cos;
+    p.sin = a->sin;
+    p.pos = a->positions;
+    p.n = a->n_tokens;
+    p.max_pos = a->rot_dim ? a->max_pos : INT32_MAX;
+    p.heads[0] = (int)a->n_heads;
+    p.heads[1] = (int)a->n_kv_heads;
+    p.hd = (int)a->head_dim;
+    p.rot = (int)a->rot_dim;
+    p.inter = a->interleaved != 0;
+    p.eps = a->eps;
+    return p;
+}
+
+int check_grid(int64_t blocks, const char* fn) {
+    return blocks > INT32_MAX ? set_error(RQ_ERR_INVALID, "%s: too many rows for one call", fn) : RQ_OK;
+}
+
+AppendP append_params(const rq_kv4* c, const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh,
+                      const int32_t* slots, int64_t n, size_t size) {
+    AppendP p{};
+    p.x[0] = k;
+    p.x[1] = v;
+    p.tok[0] = kt;
+    p.head[0] = kh;
+    p.tok[1] = vt;
+    p.head[1] = vh;
+    p.wide[0] = wide_ok(k, kt, kh, size);
+    p.wide[1] = wide_ok(v, vt, vh, size);
+    p.slots = slots;
+    p.n = n;
+    p.n_slots = c->n_pages * c->page_size;
+    p.data = c->data;
+    p.page_size = c->page_size;
+    p.n_kv = c->n_kv;
+    p.nb = c->head_dim / 32;
+    return p;
+}
+
+}  // namespace
+}  // namespace rq
+
+using namespace rq;
+
+extern "C" {
+
+int rq_kv4_create(rq_ctx* ctx, int64_t n_pages, int page_size, int n_kv_heads, int head_dim, rq_kv4** out) {
+    if (!ctx || !out) return set_error(RQ_ERR_INVALID, "rq_kv4_create: NULL argument");
+    *out = nullptr;
+    if (n_pages < 1 || page_size < kKv4Tile || page_size > 4096 || page_size % kKv4Tile || n_kv_heads < 1 || n_kv_heads > 65536)
+        return set_error(RQ_ERR_INVALID,
+                         "rq_kv4_create: %lld pages of %d positions (a multiple of 16 up to 4096), %d kv heads",
+                         (long long)n_pages, page_size, n_kv_heads);
+    if (head_dim != 32 && head_dim != 64 && head_dim != 96 && head_dim != 128)
+        return set_error(RQ_ERR_UNSUPPORTED, "rq_kv4_create: head_dim %d (32, 64, 96 or 128)", head_dim);
+    if (n_pages > INT32_MAX / page_size)
+        return set_error(RQ_ERR_INVALID, "rq_kv4_create: %lld pages of %d positions pass 2^31 slots", (long long)n_pages,
+                         page_size);
+    DevGuard g(ctx->device);
+    rq_kv4* c = new (std::nothrow) rq_kv4();
+    if (!c) return set_error(RQ_ERR_OOM, "host allocation failed");
+    c->ctx = ctx;
+    c->n_pages = n_pages;
+    c->page_size = page_size;
+    c->n_kv = n_kv_heads;
+    c->head_dim = head_dim;
+    c->bytes = (size_t)n_pages * n_kv_heads * (page_size / kKv4Tile) * 576 * (head_dim / 32);
+    int rc = cuda_error(cudaMalloc((void**)&c->data, c->bytes), "cudaMalloc(kv4)");
+    if (!rc) {
+        // zero scales: positions never written read as zeros
+        rc = cuda_error(cudaMemset(c->data, 0, c->bytes), "kv4 clear");
+        if (!rc) rc = cuda_error(cudaDeviceSynchronize(), "kv4 clear");
+        if (rc) cudaFree(c->data);
+    }
+    if (rc) {
+        delete c;
+        return rc;
+    }
+    *out = c;
+    return RQ_OK;
+}
+
+int rq_kv4_free(rq_kv4* c) {
+    if (!c) return RQ_OK;
+    DevGuard g(c->ctx->device);
+    cudaFree(c->data);
+    delete c;
+    return RQ_OK;
+}
+
+int rq_kv4_info(const rq_kv4* c, int64_t* n_pages, int* page_size, int* n_kv_heads, int* head_dim, size_t* device_bytes) {
+    int rc = check_cache(c, "rq_kv4_info");
+    if (rc) return rc;
+    if (n_pages) *n_pages = c->n_pages;
+    if (page_size) *page_size = c->page_size;
+    if (n_kv_heads) *n_kv_heads = c->n_kv;
+    if (head_dim) *head_dim = c->head_dim;
+    if (device_bytes) *device_bytes = c->bytes;
+    return RQ_OK;
+}
+
+int rq_kv4_append(rq_kv4* c, int dtype, const void* k, const int64_t k_stride[2], const void* v, const int64_t v_stride[2],
+                  const int32_t* slots, int64_t n, void* stream) {
+    int rc = check_cache(c, "rq_kv4_append");
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!size) return set_error(RQ_ERR_UNSUPPORTED, "rq_kv4_append: dtype %d (f32 = 0, f16 = 1, bf16 = 2)", dtype);
+    if (n < 0 || n > INT32_MAX || !k_stride || !v_stride)
+        return set_error(RQ_ERR_INVALID, "rq_kv4_append: n = %lld, strides %s", (long long)n, k_stride && v_stride ? "given" : "NULL");
+    if (n == 0) return RQ_OK;
+    DevGuard g(c->ctx->device);
+    rc = check_device_ptr(c->ctx, k, "rq_kv4_append", "k");
+    if (!rc) rc = check_device_ptr(c->ctx, v, "rq_kv4_append", "v");
+    if (!rc) rc = check_device_ptr(c->ctx, slots, "rq_kv4_append", "slots");
+    if (rc) return rc;
+    AppendP p = append_params(c, k, k_stride[0], k_stride[1], v, v_stride[0], v_stride[1], slots, n, size);
+    const int64_t blocks = (n * 2 * c->n_kv * 4 * p.nb + 255) / 256;
+    rc = check_grid(blocks, "rq_kv4_append");
+    if (rc) return rc;
+    const void* fn = dtype == RQ_F32 ? (const void*)kv4_append_kernel<float>
+                     : dtype == RQ_F16 ? (const void*)kv4_append_kernel<__half>
+                                       : (const void*)kv4_append_kernel<__nv_bfloat16>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "kv4 append kernel");
+}
+
+int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, void* k, void* v, void* stream) {
+    int rc = check_cache(c, "rq_kv4_read");
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!size) return set_error(RQ_ERR_UNSUPPORTED, "rq_kv4_read: dtype %d (f32 = 0, f16 = 1, bf16 = 2)", dtype);
+    if (n < 0 || n > INT32_MAX) return set_error(RQ_ERR_INVALID, "rq_kv4_read: n = %lld", (long long)n);
+    if (n == 0) return RQ_OK;
+    DevGuard g(c->ctx->device);
+    rc = check_device_ptr(c->ctx, slots, "rq_kv4_read", "slots");
+    if (!rc) rc = check_device_ptr(c->ctx, k, "rq_kv4_read", "k");
+    if (!rc) rc = check_device_ptr(c->ctx, v, "rq_kv4_read", "v");
+    if (rc) return rc;
+    ReadP p{};
+    p.data = c->data;
+    p.slots = slots;
+    p.n = n;
+    p.n_slots = c->n_pages * c->page_size;
+    p.page_size = c->page_size;
+    p.n_kv = c->n_kv;
+    p.nb = c->head_dim / 32;
+    p.x[0] = k;
+    p.x[1] = v;
+    p.wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+    const int64_t blocks = (n * 2 * c->n_kv * 4 * p.nb + 255) / 256;
+    rc = check_grid(blocks, "rq_kv4_read");
+    if (rc) return rc;
+    const void* fn = dtype == RQ_F32 ? (const void*)kv4_read_kernel<float>
+                     : dtype == RQ_F16 ? (const void*)kv4_read_kernel<__half>
+                                       : (const void*)kv4_read_kernel<__nv_bfloat16>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "kv4 read kernel");
+}
+
+int rq_qk_norm_rope(rq_ctx* ctx, const rq_qk_rope* a, void* stream) {
+    static const char* fn_name = "rq_qk_norm_rope";
+    if (!ctx) return set_error(RQ_ERR_INVALID, "%s: NULL argument", fn_name);
+    DevGuard g(ctx->device);
+    int rc = check_rope(ctx, a, false, fn_name);
+    if (rc) return rc;
+    if (!a->n_tokens || !(a->n_heads + a->n_kv_heads)) return RQ_OK;
+    RopeP p = rope_params(a);
+    const size_t size = dtype_size(a->dtype);
+    const int wide = (int)(16 / size);
+    bool vec = p.hd % wide == 0 && p.rot % (2 * wide) == 0;
+    for (int i = 0; i < 2; i++)
+        if (p.heads[i]) vec = vec && wide_ok(p.x[i], p.xt[i], p.xh[i], size) && wide_ok(p.y[i], p.yt[i], p.yh[i], size);
+    const int E = vec ? wide : 1;
+    const int slots = p.rot / (2 * E) + ((p.hd - p.rot) / E + 1) / 2;
+    p.lpr = 1;
+    while (p.lpr < slots && p.lpr < 32) p.lpr *= 2;
+    const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
+    // heads a group goes over: one while the rows do not fill the device's
+    // threads, else four (the tables' loads shared)
+    p.hpg = rows * p.lpr <= (int64_t)ctx->sm_count * 2048 ? 1 : 4;
+    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
+    const int64_t blocks = (p.n * (gq + gk) * p.lpr + 255) / 256;
+    rc = check_grid(blocks, fn_name);
+    if (rc) return rc;
+    const void* fn;
+    if (a->dtype == RQ_F32)
+        fn = vec ? (const void*)qk_norm_rope_kernel<float, 4, 1> : (const void*)qk_norm_rope_kernel<float, 1, 4>;
+    else if (a->dtype == RQ_F16)
+        fn = vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1> : (const void*)qk_norm_rope_kernel<__half, 1, 4>;
+    else
+        fn = vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1>
+                 : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "q/k norm and rotation kernel");
+}
+
+int rq_qk_norm_rope_append(rq_kv4* c, const rq_qk_rope* a, const void* v, const int64_t v_stride[2], const int32_t* slots,
+                           void* stream) {
+    static const char* fn_name = "rq_qk_norm_rope_append";
+    int rc = check_cache(c, fn_name);
+    if (rc) return rc;
+    DevGuard g(c->ctx->device);
+    rc = check_rope(c->ctx, a, true, fn_name);
+    if (rc) return rc;
+    if (a->head_dim != c->head_dim || a->n_kv_heads != c->n_kv)
+        return set_error(RQ_ERR_INVALID, "%s: %lld kv heads of %lld, the cache holds %d of %d", fn_name,
+                         (long long)a->n_kv_heads, (long long)a->head_dim, c->n_kv, c->head_dim);
+    if (!v_stride) return set_error(RQ_ERR_INVALID, "%s: v_stride is NULL", fn_name);
+    if (!a->n_tokens) return RQ_OK;
+    rc = check_device_ptr(c->ctx, v, fn_name, "v");
+    if (!rc) rc = check_device_ptr(c->ctx, slots, fn_name, "slots");
+    if (rc) return rc;
+    const size_t size = dtype_size(a->dtype);
+    RopeAppendP p{};
+    p.r = rope_params(a);
+    p.wide_q = wide_ok(p.r.x[0], p.r.xt[0], p.r.xh[0], size);
+    p.wide_qo = wide_ok(p.r.y[0], p.r.yt[0], p.r.yh[0], size);
+    p.a = append_params(c, a->k, a->k_stride[0], a->k_stride[1], v, v_stride[0], v_stride[1], slots, a->n_tokens, size);
+    const int64_t blocks = (a->n_tokens * (a->n_heads + 2 * a->n_kv_heads) + 15) / 16;
+    rc = check_grid(blocks, fn_name);
+    if (rc) return rc;
+    const void* fn = a->dtype == RQ_F32 ? (const void*)qk_norm_rope_append_kernel<float>
+                     : a->dtype == RQ_F16 ? (const void*)qk_norm_rope_append_kernel<__half>
+                                          : (const void*)qk_norm_rope_append_kernel<__nv_bfloat16>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "q/k norm, rotation and append kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,255 @@
+// rq_kv4.cuh -- the paged key/value cache held in 4 bits: layout, rounding and
+// the helpers that its kernels (append, read, attention) share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "rq_internal.cuh"
+
+// A block is 32 consecutive elements of one head's row: an f16 scale d and 32
+// codes, value = (code - 8) * d.  The cache is [page][kv head][tile], a tile
+// being 16 consecutive positions of one head, so a tile is one contiguous
+// record of 576 * NB bytes (NB = head_dim / 32) that one bulk copy brings in:
+//   K codes 256 NB | V codes 256 NB | K scales 32 NB | V scales 32 NB
+// Codes lie in the order in which the lanes of a warp feed them to
+// mma.m16n8k16 (lane = 4 g + t), so attention reads them with 16-byte
+// conflict-free loads and turns them into f16 operands without a shuffle:
+//   K  lane (g, t), word 2 b + n: the 8 elements 32 b + 8 t .. + 7 of token
+//      4 (g / 2) + (g % 2) + 2 n (column g of score tile n); element 2 i + h
+//      in nibble i + 4 h, so a 16-bit lane mask yields two neighbours.
+//   V  lane (g, t), word 2 b + p: tokens 4 t + 2 p (low half) and 4 t + 2 p + 1
+//      (high half); nibble k of a half is element 32 b + 8 k + g.
+//   scales: [token / 4][b][token % 4] f16.
+// A token's K words and V halves are its own: an append writes no byte that
+// holds another token's codes.
+struct rq_kv4 {
+    rq_ctx* ctx;
+    uint8_t* data;
+    int64_t n_pages;
+    int page_size, n_kv, head_dim;
+    size_t bytes;
+};
+
+namespace rq {
+
+constexpr int kKv4Tile = 16;  // positions of a tile
+
+template <int NB>
+struct Kv4Rec {
+    static constexpr int kCodes = 256 * NB;  // bytes of one code region
+    static constexpr int kV = kCodes, kKs = 2 * kCodes, kVs = kKs + 32 * NB;
+    static constexpr int kBytes = 576 * NB;
+};
+
+// Byte of word w (0 .. 2 NB - 1) of `lane` inside a code region: planes of
+// four words a lane (16 bytes), then one of two where 2 NB is not a multiple
+// of four.
+__host__ __device__ __forceinline__ int kv4_word(int nb, int lane, int w) {
+    const int full = nb >> 1;  // planes of four words
+    return (w >> 2) < full ? (w >> 2) * 512 + lane * 16 + (w & 3) * 4 : full * 512 + lane * 8 + (w & 3) * 4;
+}
+__host__ __device__ __forceinline__ int kv4_scale(int nb, int tok, int b) {
+    return 2 * ((tok >> 2) * 4 * nb + b * 4 + (tok & 3));
+}
+// K: token and the group t of 8 elements inside block b -> lane and word
+__host__ __device__ __forceinline__ int kv4_k_at(int nb, int tok, int b, int t) {
+    const int g = 2 * (tok >> 2) + (tok & 1);
+    return kv4_word(nb, g * 4 + t, 2 * b + ((tok >> 1) & 1));
+}
+// V: the 16-bit item of token tok, block b, column g
+__host__ __device__ __forceinline__ int kv4_v_at(int nb, int tok, int b, int g) {
+    return kv4_word(nb, g * 4 + (tok >> 2), 2 * b + ((tok >> 1) & 1)) + 2 * (tok & 1);
+}
+
+// The record of (slot, head); NULL for a slot outside the cache.
+__device__ __forceinline__ uint8_t* kv4_record(uint8_t* data, int64_t n_slots, int page_size, int n_kv, int rec_bytes,
+                                               int32_t slot, int head) {
+    if (slot < 0 || slot >= n_slots) return nullptr;
+    const int page = slot / page_size, off = slot % page_size;
+    return data + (((int64_t)page * n_kv + head) * (page_size / kKv4Tile) + off / kKv4Tile) * rec_bytes;
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// 8 consecutive elements as f32; `wide`: p is 16-byte aligned
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, bool wide, float (&x)[8]) {
+    if (wide) {
+        T tmp[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            reinterpret_cast<uint4*>(tmp)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(tmp[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ p, bool wide, const float (&x)[8]) {
+    if (wide) {
+        T tmp[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) tmp[i] = from_f32<T>(x[i]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(tmp)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = from_f32<T>(x[i]);
+    }
+}
+
+// The four lanes of an aligned group hold a block, 8 elements each.  Returns
+// the block's scale (f16 value in f32) and this lane's 8 codes as nibbles in
+// element order.  d = f16(m / -8), m the element of the largest magnitude
+// (the lowest index of equals); m / 8 is exact, so d is one rounding.  A code
+// is the nearest multiple of d (ties to the higher code): (c - 8.5) * d has at
+// most 16 bits, exact in f32, so the comparisons below decide exactly where
+// an f32 quotient would be off near a border.  A NaN makes the scale NaN (the
+// block reads back as NaN); infinities saturate the scale at 65504.
+__device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], float& d_out) {
+    float m = x[0];
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        nan |= x[i] != x[i];
+        if (fabsf(x[i]) > fabsf(m)) m = x[i];
+    }
+    const unsigned lane = threadIdx.x & 31;
+    const unsigned group = 0xFu << (lane & 28);
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+        const float other = __shfl_xor_sync(group, m, o);
+        const bool lower = (lane & o) != 0;  // the other lane holds lower indexes
+        if (lower ? fabsf(other) >= fabsf(m) : fabsf(other) > fabsf(m)) m = other;
+    }
+    nan = (__ballot_sync(group, nan) & group) != 0;
+    const float d = __half2float(__float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f)));
+    uint32_t w = 0;
+    if (nan) {
+        d_out = __int_as_float(0x7fffffff);
+        return 0x88888888u;
+    }
+    d_out = d;
+    if (d == 0.0f) return 0x88888888u;
+    const float inv = 1.0f / d;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float t = fminf(fmaxf(floorf(x[i] * inv + 8.5f), 0.0f), 15.0f);
+        const float lo = (t - 8.5f) * d, hi = (t - 7.5f) * d;
+        if (t > 0.0f && (d > 0.0f ? x[i] < lo : x[i] > lo)) t -= 1.0f;
+        else if (t < 15.0f && (d > 0.0f ? x[i] >= hi : x[i] <= hi)) t += 1.0f;
+        w |= (uint32_t)t << (4 * i);
+    }
+    return w;
+}
+
+// element-order nibbles -> K word (element 2 i + h to nibble i + 4 h) and back
+__device__ __forceinline__ uint32_t kv4_k_word(uint32_t w) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) r |= ((w >> (4 * i)) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    return r;
+}
+__device__ __forceinline__ uint32_t kv4_k_unword(uint32_t r) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) w |= ((r >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) << (4 * i);
+    return w;
+}
+
+// Writes one lane's share of a token's block: x holds elements 32 b + 8 t ..
+// + 7 (t = lane % 4; the aligned four lanes hold the block).  rec NULL: the
+// lane takes part in the group's exchange and writes nothing.
+__device__ __forceinline__ void kv4_store(uint8_t* rec, int nb, int tok, int b, bool is_v, const float (&x)[8]) {
+    float d;
+    const uint32_t w = kv4_quantize(x, d);
+    const unsigned lane = threadIdx.x & 31, t = lane & 3;
+    const unsigned group = 0xFu << (lane & 28);
+    uint8_t* codes = rec + (is_v ? 256 * nb : 0);
+    if (!is_v) {
+        if (rec) *reinterpret_cast<uint32_t*>(codes + kv4_k_at(nb, tok, b, (int)t)) = kv4_k_word(w);
+    } else {
+        // element 8 k + g of lane k goes to nibble k of item g: lane t writes
+        // items 2 t and 2 t + 1
+        uint32_t a = 0, c = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t o = __shfl_sync(group, w, (int)((lane & 28) + k));
+            a |= ((o >> (8 * t)) & 15u) << (4 * k);
+            c |= ((o >> (8 * t + 4)) & 15u) << (4 * k);
+        }
+        if (rec) {
+            *reinterpret_cast<uint16_t*>(codes + kv4_v_at(nb, tok, b, (int)(2 * t))) = (uint16_t)a;
+            *reinterpret_cast<uint16_t*>(codes + kv4_v_at(nb, tok, b, (int)(2 * t + 1))) = (uint16_t)c;
+        }
+    }
+    if (rec && t == 0)
+        *reinterpret_cast<__half*>(rec + 512 * nb + (is_v ? 32 * nb : 0) + kv4_scale(nb, tok, b)) = __float2half_rn(d);
+}
+
+// The inverse: this lane's 8 values of a token's block.
+__device__ __forceinline__ void kv4_load(const uint8_t* rec, int nb, int tok, int b, bool is_v, float (&x)[8]) {
+    const unsigned lane = threadIdx.x & 31, t = lane & 3;
+    const unsigned group = 0xFu << (lane & 28);
+    uint32_t w = 0;
+    float d = 0.0f;
+    if (rec) d = __half2float(*reinterpret_cast<const __half*>(rec + 512 * nb + (is_v ? 32 * nb : 0) + kv4_scale(nb, tok, b)));
+    if (!is_v) {
+        if (rec) w = kv4_k_unword(*reinterpret_cast<const uint32_t*>(rec + kv4_k_at(nb, tok, b, (int)t)));
+    } else {
+        uint32_t items = 0;
+        if (rec)
+            items = *reinterpret_cast<const uint16_t*>(rec + 256 * nb + kv4_v_at(nb, tok, b, (int)(2 * t))) |
+                    ((uint32_t)*reinterpret_cast<const uint16_t*>(rec + 256 * nb + kv4_v_at(nb, tok, b, (int)(2 * t + 1))) << 16);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {  // items 2 k, 2 k + 1 of lane k: its nibble t is this lane's elements 2 k, 2 k + 1
+            const uint32_t o = __shfl_sync(group, items, (int)((lane & 28) + k));
+            w |= ((o >> (4 * t)) & 15u) << (8 * k);
+            w |= ((o >> (16 + 4 * t)) & 15u) << (8 * k + 4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = ((float)((w >> (4 * i)) & 15u) - 8.0f) * d;
+}
+
+// shared host helpers of the paged operators (rq_kv4.cu)
+struct DevGuard {  // the context's device for the duration of a call
+    int prev = -1;
+    explicit DevGuard(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~DevGuard() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+};
+// RQ_OK when p is device memory on ctx's device, else an error that names it
+int check_device_ptr(const rq_ctx* ctx, const void* p, const char* fn, const char* name);
+// a launch that may begin while the previous kernel of the stream drains
+// (the kernel waits with griddepcontrol.wait before it touches memory);
+// cluster > 1: thread-block clusters of that many CTAs along x
+int launch_pdl(const void* fn, unsigned grid, unsigned block, size_t smem, cudaStream_t st, void** args, const char* what,
+               unsigned cluster = 1);
+
+__device__ __forceinline__ void pdl_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+}
+
+}  // namespace rq

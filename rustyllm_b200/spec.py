@@ -11,6 +11,45 @@ from __future__ import annotations
 from collections import deque
 
 
+def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
+    """(tokens [batch, n + 1], accepted [batch]) int32: the drafted tokens
+    drafts [batch, n] checked against the target's probabilities p [batch, n +
+    1, vocab] and those they were drawn from, q [batch, n, vocab] (None: each
+    was certain), with the uniform numbers u [batch, n] and r [batch]
+    (float32); rq_spec_verify of include/rq.h.  n_drafts [batch] (int32)
+    limits a row's drafts.  A row of tokens is the accepted drafts, one drawn
+    token and -1s; with n = 0 the call samples from p."""
+    import ctypes
+
+    import torch
+
+    from . import _lib
+    from .kv4 import dtype_of, int32, need, stream_of
+    from .linear import Context
+    need(isinstance(p, torch.Tensor) and p.is_cuda and p.dim() == 3 and p.stride(2) == 1,
+         "p: a CUDA tensor [batch, n + 1, vocab] with contiguous rows is wanted")
+    b, n, vocab = p.shape[0], p.shape[1] - 1, p.shape[2]
+    dev = p.device
+    need(q is None or (q.shape == (b, n, vocab) and q.dtype == p.dtype and q.device == dev
+                       and (q.stride(2) == 1 or q.numel() == 0)),
+         f"q: [{b}, {n}, {vocab}] {p.dtype} with contiguous rows on {dev} is wanted")
+    int32(drafts, "drafts", dev, (b, n))
+    for name, x, shape in (("u", u, (b, n)), ("r", r, (b,))):
+        need(x.dtype is torch.float32 and tuple(x.shape) == shape and x.device == dev and x.is_contiguous(),
+             f"{name}: a contiguous float32 {list(shape)} on {dev} is wanted")
+    if n_drafts is not None:
+        int32(n_drafts, "n_drafts", dev, (b,))
+    tokens = torch.empty((b, n + 1), dtype=torch.int32, device=dev)
+    accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    pair = ctypes.c_int64 * 2
+    _lib.check(_lib.lib().rq_spec_verify(
+        Context.get(dev.index).handle, dtype_of(p, "p"), p.data_ptr(), pair(p.stride(0), p.stride(1)),
+        None if q is None else q.data_ptr(), None if q is None else pair(q.stride(0), q.stride(1)), drafts.data_ptr(),
+        None if n_drafts is None else n_drafts.data_ptr(), u.data_ptr(), r.data_ptr(), b, n, vocab, tokens.data_ptr(),
+        accepted.data_ptr(), stream_of(dev)))
+    return tokens, accepted
+
+
 class SpecDecoder:
     def __init__(self, target, draft, k: int = 4, adaptive: bool = False, window: int = 4):
         self.target, self.draft = target, draft
