@@ -286,6 +286,21 @@ RQ_API int rq_llama_free(rq_llama* m);
  * copied).  Replaces QBlock::load (src/streaming_quantized.rs:290-303). */
 RQ_API int rq_llama_set_layer(rq_llama* m, int64_t layer, const rq_weight* const* w7,
                               const float* rms1, const float* rms2);
+/* Norms of q and k per head before the rotation (eps = rms_eps), for models
+ * that have them: f32 [head_dim] each, host or device, copied.  The one-launch
+ * step (rq_llama_set_fused) is not used then.  No reference counterpart. */
+RQ_API int rq_llama_set_qk_norm(rq_llama* m, int64_t layer, const float* q_weight, const float* k_weight);
+/* Holds the model's cache in 4 bits and in pages of page_size positions (see
+ * rq_kv4_create: head_dim 32, 64, 96 or 128) in place of the f32 cache, which
+ * is freed: 4.5 / 32 of its memory.  Starts empty, so call it before the first
+ * forward; pages come from one ring as the position grows and go back when it
+ * is moved (rq_llama_truncate, a forward's index_pos).  The one-launch step is
+ * not used then.  No reference counterpart. */
+RQ_API int rq_llama_use_kv4(rq_llama* m, int page_size);
+/* The keys (rotated) and values that the 4-bit cache of a layer holds at
+ * positions pos .. pos + n - 1: f32 [n][n_kv_heads][head_dim] (this rank's
+ * heads), host or device.  Synchronous. */
+RQ_API int rq_llama_read_kv4(rq_llama* m, int64_t layer, int64_t pos, int64_t n, float* k, float* v);
 /* F16 [vocab][hidden] token embedding (model.embed_tokens.weight). */
 RQ_API int rq_llama_set_embedding(rq_llama* m, const uint16_t* embed_f16);
 /* Final RmsNorm weight (f32 [hidden]) and F16 lm_head rows of this rank

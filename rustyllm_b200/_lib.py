@@ -79,6 +79,9 @@ SIGNATURES.update({
     "rq_llama_set_layer": (I, [P, I64, PP, P, P]),
     "rq_llama_set_embedding": (I, [P, P]),
     "rq_llama_set_head": (I, [P, P, P]),
+    "rq_llama_set_qk_norm": (I, [P, I64, P, P]),
+    "rq_llama_use_kv4": (I, [P, I]),
+    "rq_llama_read_kv4": (I, [P, I64, I64, I64, P, P]),
     "rq_llama_forward": (I, [P, P, I64, I64, P, P, P]),
     "rq_llama_decode_step": (I, [P, P]),
     "rq_llama_forward_all": (I, [P, P, I64, I64, P, P, P]),

@@ -445,6 +445,56 @@ AppendP append_params(const rq_kv4* c, const void* k, int64_t kt, int64_t kh, co
 }
 
 }  // namespace
+
+int qk_norm_rope(const rq_ctx* ctx, const rq_qk_rope* a, cudaStream_t st) {
+    RopeP p = rope_params(a);
+    const size_t size = dtype_size(a->dtype);
+    const int wide = (int)(16 / size);
+    bool vec = p.hd % wide == 0 && p.rot % (2 * wide) == 0;
+    for (int i = 0; i < 2; i++)
+        if (p.heads[i]) vec = vec && wide_ok(p.x[i], p.xt[i], p.xh[i], size) && wide_ok(p.y[i], p.yt[i], p.yh[i], size);
+    const int E = vec ? wide : 1;
+    const int slots = p.rot / (2 * E) + ((p.hd - p.rot) / E + 1) / 2;
+    p.lpr = 1;
+    while (p.lpr < slots && p.lpr < 32) p.lpr *= 2;
+    const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
+    // heads a group goes over: one while the rows do not fill the device's
+    // threads, else four (the tables' loads shared)
+    p.hpg = rows * p.lpr <= (int64_t)ctx->sm_count * 2048 ? 1 : 4;
+    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
+    const int64_t blocks = (p.n * (gq + gk) * p.lpr + 255) / 256;
+    const int rc = check_grid(blocks, "rq_qk_norm_rope");
+    if (rc) return rc;
+    const void* fn;
+    if (a->dtype == RQ_F32)
+        fn = vec ? (const void*)qk_norm_rope_kernel<float, 4, 1> : (const void*)qk_norm_rope_kernel<float, 1, 4>;
+    else if (a->dtype == RQ_F16)
+        fn = vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1> : (const void*)qk_norm_rope_kernel<__half, 1, 4>;
+    else
+        fn = vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1>
+                 : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, st, args, "q/k norm and rotation kernel");
+}
+
+int qk_norm_rope_append(const rq_kv4* c, const rq_qk_rope* a, const void* v, const int64_t v_stride[2], const int32_t* slots,
+                        cudaStream_t st) {
+    const size_t size = dtype_size(a->dtype);
+    RopeAppendP p{};
+    p.r = rope_params(a);
+    p.wide_q = wide_ok(p.r.x[0], p.r.xt[0], p.r.xh[0], size);
+    p.wide_qo = wide_ok(p.r.y[0], p.r.yt[0], p.r.yh[0], size);
+    p.a = append_params(c, a->k, a->k_stride[0], a->k_stride[1], v, v_stride[0], v_stride[1], slots, a->n_tokens, size);
+    const int64_t blocks = (a->n_tokens * (a->n_heads + 2 * a->n_kv_heads) + 15) / 16;
+    const int rc = check_grid(blocks, "rq_qk_norm_rope_append");
+    if (rc) return rc;
+    const void* fn = a->dtype == RQ_F32 ? (const void*)qk_norm_rope_append_kernel<float>
+                     : a->dtype == RQ_F16 ? (const void*)qk_norm_rope_append_kernel<__half>
+                                          : (const void*)qk_norm_rope_append_kernel<__nv_bfloat16>;
+    void* args[] = {&p};
+    return launch_pdl(fn, (unsigned)blocks, 256, 0, st, args, "q/k norm, rotation and append kernel");
+}
+
 }  // namespace rq
 
 using namespace rq;
@@ -571,34 +621,7 @@ int rq_qk_norm_rope(rq_ctx* ctx, const rq_qk_rope* a, void* stream) {
     int rc = check_rope(ctx, a, false, fn_name);
     if (rc) return rc;
     if (!a->n_tokens || !(a->n_heads + a->n_kv_heads)) return RQ_OK;
-    RopeP p = rope_params(a);
-    const size_t size = dtype_size(a->dtype);
-    const int wide = (int)(16 / size);
-    bool vec = p.hd % wide == 0 && p.rot % (2 * wide) == 0;
-    for (int i = 0; i < 2; i++)
-        if (p.heads[i]) vec = vec && wide_ok(p.x[i], p.xt[i], p.xh[i], size) && wide_ok(p.y[i], p.yt[i], p.yh[i], size);
-    const int E = vec ? wide : 1;
-    const int slots = p.rot / (2 * E) + ((p.hd - p.rot) / E + 1) / 2;
-    p.lpr = 1;
-    while (p.lpr < slots && p.lpr < 32) p.lpr *= 2;
-    const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
-    // heads a group goes over: one while the rows do not fill the device's
-    // threads, else four (the tables' loads shared)
-    p.hpg = rows * p.lpr <= (int64_t)ctx->sm_count * 2048 ? 1 : 4;
-    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
-    const int64_t blocks = (p.n * (gq + gk) * p.lpr + 255) / 256;
-    rc = check_grid(blocks, fn_name);
-    if (rc) return rc;
-    const void* fn;
-    if (a->dtype == RQ_F32)
-        fn = vec ? (const void*)qk_norm_rope_kernel<float, 4, 1> : (const void*)qk_norm_rope_kernel<float, 1, 4>;
-    else if (a->dtype == RQ_F16)
-        fn = vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1> : (const void*)qk_norm_rope_kernel<__half, 1, 4>;
-    else
-        fn = vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1>
-                 : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4>;
-    void* args[] = {&p};
-    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "q/k norm and rotation kernel");
+    return qk_norm_rope(ctx, a, (cudaStream_t)stream);
 }
 
 int rq_qk_norm_rope_append(rq_kv4* c, const rq_qk_rope* a, const void* v, const int64_t v_stride[2], const int32_t* slots,
@@ -617,20 +640,7 @@ int rq_qk_norm_rope_append(rq_kv4* c, const rq_qk_rope* a, const void* v, const 
     rc = check_device_ptr(c->ctx, v, fn_name, "v");
     if (!rc) rc = check_device_ptr(c->ctx, slots, fn_name, "slots");
     if (rc) return rc;
-    const size_t size = dtype_size(a->dtype);
-    RopeAppendP p{};
-    p.r = rope_params(a);
-    p.wide_q = wide_ok(p.r.x[0], p.r.xt[0], p.r.xh[0], size);
-    p.wide_qo = wide_ok(p.r.y[0], p.r.yt[0], p.r.yh[0], size);
-    p.a = append_params(c, a->k, a->k_stride[0], a->k_stride[1], v, v_stride[0], v_stride[1], slots, a->n_tokens, size);
-    const int64_t blocks = (a->n_tokens * (a->n_heads + 2 * a->n_kv_heads) + 15) / 16;
-    rc = check_grid(blocks, fn_name);
-    if (rc) return rc;
-    const void* fn = a->dtype == RQ_F32 ? (const void*)qk_norm_rope_append_kernel<float>
-                     : a->dtype == RQ_F16 ? (const void*)qk_norm_rope_append_kernel<__half>
-                                          : (const void*)qk_norm_rope_append_kernel<__nv_bfloat16>;
-    void* args[] = {&p};
-    return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "q/k norm, rotation and append kernel");
+    return qk_norm_rope_append(c, a, v, v_stride, slots, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -247,6 +247,20 @@ int check_device_ptr(const rq_ctx* ctx, const void* p, const char* fn, const cha
 int launch_pdl(const void* fn, unsigned grid, unsigned block, size_t smem, cudaStream_t st, void** args, const char* what,
                unsigned cluster = 1);
 
+// The operators for callers inside the library that know their pointers
+// (rq_llama.cu): no checks of memory kinds, the device already current, a
+// bounded wait that gives up reported in *err.
+int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t st);
+int qk_norm_rope(const rq_ctx* ctx, const rq_qk_rope* a, cudaStream_t st);
+int qk_norm_rope_append(const rq_kv4* c, const rq_qk_rope* a, const void* v, const int64_t v_stride[2], const int32_t* slots,
+                        cudaStream_t st);
+int pages_extend(int64_t batch, int page_size, const int32_t* ctx_lens, const int32_t* new_lens, int32_t* table,
+                 int64_t table_stride, int64_t table_width, const int32_t* ring, int64_t n_pages, const int32_t* state_in,
+                 int32_t* state_out, int32_t* kv_lens, int32_t* cu_new, int32_t* positions, int32_t* slots, int64_t n_tokens,
+                 cudaStream_t st);
+int pages_release(int64_t batch, int page_size, const int32_t* held_lens, const int32_t* keep_lens, int32_t* table,
+                  int64_t table_stride, int64_t table_width, int32_t* ring, int64_t n_pages, int32_t* state, cudaStream_t st);
+
 __device__ __forceinline__ void pdl_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");

@@ -593,41 +593,14 @@ size_t plan_bytes(const rq_kv4* c, const rq_kv4_query* a, const Plan& pl) {
 }
 
 }  // namespace
-}  // namespace rq
 
-using namespace rq;
-
-extern "C" {
-
-int rq_kv4_attention_workspace(const rq_kv4* c, const rq_kv4_query* a, size_t* bytes) {
-    if (!bytes) return set_error(RQ_ERR_INVALID, "rq_kv4_attention_workspace: NULL argument");
-    int rc = check_query(c, a, "rq_kv4_attention_workspace");
-    if (rc) return rc;
-    *bytes = plan_bytes(c, a, make_plan(c, a));
-    return RQ_OK;
-}
-
-int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream) {
-    static const char* fn_name = "rq_kv4_attention";
-    int rc = check_query(c, a, fn_name);
-    if (rc) return rc;
-    if (!a->batch || !a->n_tokens) return RQ_OK;
-    DevGuard g(c->ctx->device);
-    const rq_ctx* ctx = c->ctx;
-    rc = check_device_ptr(ctx, a->q, fn_name, "q");
-    if (!rc) rc = check_device_ptr(ctx, a->out, fn_name, "out");
-    if (!rc) rc = check_device_ptr(ctx, a->kv_lens, fn_name, "kv_lens");
-    if (!rc && a->cu_q) rc = check_device_ptr(ctx, a->cu_q, fn_name, "cu_q");
-    if (!rc && a->table_width) rc = check_device_ptr(ctx, a->block_table, fn_name, "block_table");
-    if (rc) return rc;
+int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t st) {
     const Plan pl = make_plan(c, a);
     const size_t need = plan_bytes(c, a, pl);
     if (need) {
         if (a->workspace_bytes < need)
             return set_error(RQ_ERR_INVALID, "rq_kv4_attention: workspace of %zu bytes, need %zu", a->workspace_bytes, need);
-        rc = check_device_ptr(ctx, a->workspace, fn_name, "workspace");
-        if (rc) return rc;
-        if ((uintptr_t)a->workspace & 15) return set_error(RQ_ERR_INVALID, "rq_kv4_attention: workspace is not 16-byte aligned");
+        if (!a->workspace || (uintptr_t)a->workspace & 15) return set_error(RQ_ERR_INVALID, "rq_kv4_attention: workspace is NULL or not 16-byte aligned");
     }
     if (pl.units * pl.splits > INT32_MAX || pl.units * pl.R > INT32_MAX)
         return set_error(RQ_ERR_INVALID, "rq_kv4_attention: too many rows for one call");
@@ -663,16 +636,47 @@ int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream) {
         const int64_t rows = a->n_tokens * a->n_heads * pl.splits;
         p.ml = reinterpret_cast<float2*>(p.part + rows * c->head_dim);
     }
-    p.err = ctx->derr;
+    p.err = err;
     const int nb = c->head_dim / 32;
     const size_t smem = (size_t)kWarps * std::max(kStages * 576 * nb, pl.R * 32 * nb * 4);
     const void* fn = pick(a->dtype, nb, false, pl.mode);
     void* args[] = {&p};
-    rc = launch_pdl(fn, (unsigned)(pl.units * pl.splits), kWarps * 32, smem, (cudaStream_t)stream, args,
+    const int rc = launch_pdl(fn, (unsigned)(pl.units * pl.splits), kWarps * 32, smem, st, args,
                     "kv4 attention kernel");
     if (rc || pl.splits == 1) return rc;
     const void* jf = pick(a->dtype, nb, true, pl.mode);
-    return launch_pdl(jf, (unsigned)(pl.units * pl.R), 32 * nb, 0, (cudaStream_t)stream, args, "kv4 join kernel");
+    return launch_pdl(jf, (unsigned)(pl.units * pl.R), 32 * nb, 0, st, args, "kv4 join kernel");
+}
+
+
+}  // namespace rq
+
+using namespace rq;
+
+extern "C" {
+
+int rq_kv4_attention_workspace(const rq_kv4* c, const rq_kv4_query* a, size_t* bytes) {
+    if (!bytes) return set_error(RQ_ERR_INVALID, "rq_kv4_attention_workspace: NULL argument");
+    int rc = check_query(c, a, "rq_kv4_attention_workspace");
+    if (rc) return rc;
+    *bytes = plan_bytes(c, a, make_plan(c, a));
+    return RQ_OK;
+}
+
+int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream) {
+    static const char* fn_name = "rq_kv4_attention";
+    int rc = check_query(c, a, fn_name);
+    if (rc) return rc;
+    if (!a->batch || !a->n_tokens) return RQ_OK;
+    DevGuard g(c->ctx->device);
+    const rq_ctx* ctx = c->ctx;
+    rc = check_device_ptr(ctx, a->q, fn_name, "q");
+    if (!rc) rc = check_device_ptr(ctx, a->out, fn_name, "out");
+    if (!rc) rc = check_device_ptr(ctx, a->kv_lens, fn_name, "kv_lens");
+    if (!rc && a->cu_q) rc = check_device_ptr(ctx, a->cu_q, fn_name, "cu_q");
+    if (!rc && a->table_width) rc = check_device_ptr(ctx, a->block_table, fn_name, "block_table");
+    if (!rc && a->workspace) rc = check_device_ptr(ctx, a->workspace, fn_name, "workspace");
+    return rc ? rc : kv4_attention(c, a, ctx->derr, (cudaStream_t)stream);
 }
 
 }  // extern "C"

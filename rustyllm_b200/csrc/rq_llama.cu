@@ -29,6 +29,7 @@
 
 #include "rq_attn.cuh"
 #include "rq_decode.cuh"
+#include "rq_kv4.cuh"
 #include "rq_p2p.cuh"
 #include "rq_mv_common.cuh"
 
@@ -41,6 +42,9 @@ struct rq_llama {
         float* rms2;
         float* kc;  // [n_kv][max_seq][head_dim]
         float* vc;
+        float* qn = nullptr;  // q / k norm weights [head_dim] (rq_llama_set_qk_norm)
+        float* kn = nullptr;
+        rq_kv4* kv4 = nullptr;  // the layer's cache in 4 bits (rq_llama_use_kv4; kc, vc are then NULL)
     };
     std::vector<Layer> layers;
     __half* embed;    // [vocab][hidden]
@@ -87,6 +91,18 @@ struct rq_llama {
     unsigned* bar;                      // grid-barrier arrivals
     int* derr;                          // error word of the step
     bool fused = false;                 // rq_llama_set_fused
+    // 4-bit paged cache (rq_llama_use_kv4): one table for all layers, its
+    // pages taken and given back as the position moves
+    int kv4_page = 0;             // page size; 0: f32 cache
+    int64_t kv4_width = 0;        // pages of max_seq positions
+    int32_t* kv4_table = nullptr; // [width]
+    int32_t* kv4_ring = nullptr;  // [width]
+    int32_t* kv4_state = nullptr; // {head, free, short}
+    int32_t* kv4_rows = nullptr;  // [Tmax] positions, [Tmax] slots of a forward's tokens
+    int32_t* kv4_seek = nullptr;  // {keep, gap, kv_len, 0, cu[2]}
+    void* kv4_ws = nullptr;       // attention workspace
+    size_t kv4_ws_bytes = 0;
+    int32_t* iota = nullptr;      // [Tmax + 1] 0, 1, ..: lengths and positions as device values
     std::vector<void*> allocs;
     std::vector<rq_weight*> owned;  // weights uploaded by rq_llama_load_gguf_dir
 };
@@ -466,6 +482,94 @@ bool l2_prefetch_enabled() {
     return on == 1;
 }
 
+// The q / k norms of a layer and the rotation as rq_qk_rope: T rows of m->q
+// and m->k, in place.
+rq_qk_rope qk_args(const rq_llama* m, const rq_llama::Layer& L, int64_t T) {
+    const rq_llama_config& c = m->cfg;
+    rq_qk_rope a{};
+    a.dtype = RQ_F32;
+    a.n_tokens = T;
+    a.n_heads = m->nh_l;
+    a.n_kv_heads = m->nkv_l;
+    a.head_dim = c.head_dim;
+    a.rot_dim = c.head_dim;
+    a.q = a.q_out = m->q;
+    a.k = a.k_out = m->k;
+    a.q_stride[0] = a.q_out_stride[0] = m->nh_l * c.head_dim;
+    a.k_stride[0] = a.k_out_stride[0] = m->nkv_l * c.head_dim;
+    a.q_stride[1] = a.q_out_stride[1] = a.k_stride[1] = a.k_out_stride[1] = c.head_dim;
+    a.q_weight = L.qn;
+    a.k_weight = L.kn;
+    a.eps = c.rms_eps;
+    a.cos = m->rope_cos;
+    a.sin = m->rope_sin;
+    a.max_pos = c.max_seq;
+    a.positions = m->kv4_rows;
+    return a;
+}
+
+// RoPE, append and attention of T tokens over the 4-bit cache: m->att = the
+// heads' outputs.  m->kv4_rows / kv4_seek were filled by kv4_begin.
+int kv4_attend(rq_llama* m, const rq_llama::Layer& L, int64_t T, cudaStream_t st) {
+    const rq_llama_config& c = m->cfg;
+    const rq_qk_rope a = qk_args(m, L, T);
+    int rc = qk_norm_rope_append(L.kv4, &a, m->v, a.k_stride, m->kv4_rows + c.max_batch_tokens, st);
+    if (rc) return rc;
+    rq_kv4_query q{};
+    q.dtype = RQ_F32;
+    q.q = m->q;
+    q.q_stride[0] = q.out_stride[0] = m->nh_l * c.head_dim;
+    q.q_stride[1] = q.out_stride[1] = c.head_dim;
+    q.out = m->att;
+    q.n_tokens = T;
+    q.n_heads = m->nh_l;
+    q.batch = 1;
+    q.max_q = T;
+    q.cu_q = T == 1 ? nullptr : m->kv4_seek + 4;
+    q.kv_lens = m->kv4_seek + 2;
+    q.block_table = m->kv4_table;
+    q.table_stride = q.table_width = m->kv4_width;
+    q.max_len = c.max_seq;
+    q.scale = 1.0f / sqrtf((float)c.head_dim);
+    q.workspace = m->kv4_ws;
+    q.workspace_bytes = m->kv4_ws_bytes;
+    return kv4_attention(L.kv4, &q, m->derr, st);
+}
+
+// Pages, positions and slots of the T tokens at *m->pos.
+int kv4_begin(rq_llama* m, int64_t T, cudaStream_t st) {
+    return pages_extend(1, m->kv4_page, m->pos, m->iota + T, m->kv4_table, m->kv4_width, m->kv4_width, m->kv4_ring,
+                        m->kv4_width, m->kv4_state, m->kv4_state, m->kv4_seek + 2, m->kv4_seek + 4, m->kv4_rows,
+                        m->kv4_rows + m->cfg.max_batch_tokens, T, st);
+}
+
+// keep = min(*pos, to), gap = max(to - *pos, 0); *pos = to
+__global__ void kv4_seek_kernel(int32_t* pos, int32_t to, int32_t* seek, int32_t* old) {
+    pdl_enter();
+    const int p = *pos;
+    *old = p;
+    seek[0] = min(p, to);
+    seek[1] = max(to - p, 0);
+    *pos = to;
+}
+
+// Moves the position to `to`: the pages behind it go back to the ring, and
+// where it lies ahead the pages in between are taken (their positions hold
+// what was last written there, as in the f32 cache).
+int kv4_seek(rq_llama* m, int64_t to, cudaStream_t st) {
+    int32_t* pos = m->pos;
+    int32_t t = (int32_t)to;
+    int32_t* seek = m->kv4_seek;
+    int32_t* old = m->kv4_seek + 3;
+    void* args[] = {&pos, &t, &seek, &old};
+    int rc = launch_simple((const void*)kv4_seek_kernel, dim3(1), dim3(1), 0, st, args, "position kernel");
+    if (!rc) rc = pages_release(1, m->kv4_page, old, seek, m->kv4_table, m->kv4_width, m->kv4_width, m->kv4_ring,
+                                m->kv4_width, m->kv4_state, st);
+    if (!rc) rc = pages_extend(1, m->kv4_page, seek, seek + 1, m->kv4_table, m->kv4_width, m->kv4_width, m->kv4_ring,
+                               m->kv4_width, m->kv4_state, m->kv4_state, seek + 2, seek + 4, nullptr, nullptr, 0, st);
+    return rc;
+}
+
 void set_next(rq_llama* m, const rq_weight* const* ws, int n, uint32_t budget) {
     m->nx = PipeNext{};
     if (n > 0 && l2_prefetch_enabled()) m->nx = pipe_next(ws, n, budget);
@@ -694,6 +798,10 @@ int forward_device(rq_llama* m, int64_t T, bool want_logits, cudaStream_t st, bo
                            dim3(256), 0, st, args, "embed kernel");
         if (rc) return rc;
     }
+    if (m->kv4_page) {
+        rc = kv4_begin(m, T, st);
+        if (rc) return rc;
+    }
     for (int64_t l = 0; l < c.n_layers; l++) {
         rq_llama::Layer& L = m->layers[l];
         const bool tc = tensor_prefill(m, T, l);
@@ -723,7 +831,14 @@ int forward_device(rq_llama* m, int64_t T, bool want_logits, cudaStream_t st, bo
             }
             if (rc) return rc;
         }
-        if (T == 1 && c.head_dim % 32 == 0) {
+        if (L.qn && !L.kv4) {  // the norms alone; the kernels below rotate
+            rq_qk_rope a = qk_args(m, L, T);
+            a.rot_dim = 0;
+            a.positions = m->iota;
+            rc = qk_norm_rope(m->ctx, &a, st);
+            if (rc) return rc;
+        }
+        if (T == 1 && c.head_dim % 32 == 0 && !L.kv4) {
             const float* q = m->q;
             const float* k = m->k;
             const float* v = m->v;
@@ -741,25 +856,30 @@ int forward_device(rq_llama* m, int64_t T, bool want_logits, cudaStream_t st, bo
                                "attention kernel");
             if (rc) return rc;
         } else {
-            float* q = m->q;
-            const float* k = m->k;
-            const float* v = m->v;
-            float* kc = L.kc;
-            float* vc = L.vc;
-            const float* cs = m->rope_cos;
-            const float* sn = m->rope_sin;
-            const int32_t* pos = m->pos;
-            int nh = (int)m->nh_l, nkv = (int)m->nkv_l, hd = (int)c.head_dim, ms = (int)c.max_seq;
-            void* args[] = {&q, &k, &v, &kc, &vc, &cs, &sn, &pos, &nh, &nkv, &hd, &ms};
-            rc = launch_simple((const void*)rope_append_kernel, dim3((unsigned)(nh + nkv), (unsigned)T),
-                               dim3((unsigned)std::max(32, hd / 2)), 0, st, args, "rope kernel");
-            if (rc) return rc;
-            const float* qc = m->q;
-            float* att = m->att;
-            void* args2[] = {&qc, &kc, &vc, &pos, &nh, &nkv, &hd, &ms, &att};
-            rc = launch_simple((const void*)attention_kernel, dim3((unsigned)nh, (unsigned)T), dim3(128),
-                               (size_t)c.max_seq * sizeof(float), st, args2, "attention kernel");
-            if (rc) return rc;
+            if (L.kv4) {
+                rc = kv4_attend(m, L, T, st);
+                if (rc) return rc;
+            } else {
+                float* q = m->q;
+                const float* k = m->k;
+                const float* v = m->v;
+                float* kc = L.kc;
+                float* vc = L.vc;
+                const float* cs = m->rope_cos;
+                const float* sn = m->rope_sin;
+                const int32_t* pos = m->pos;
+                int nh = (int)m->nh_l, nkv = (int)m->nkv_l, hd = (int)c.head_dim, ms = (int)c.max_seq;
+                void* args[] = {&q, &k, &v, &kc, &vc, &cs, &sn, &pos, &nh, &nkv, &hd, &ms};
+                rc = launch_simple((const void*)rope_append_kernel, dim3((unsigned)(nh + nkv), (unsigned)T),
+                                   dim3((unsigned)std::max(32, hd / 2)), 0, st, args, "rope kernel");
+                if (rc) return rc;
+                const float* qc = m->q;
+                float* att = m->att;
+                void* args2[] = {&qc, &kc, &vc, &pos, &nh, &nkv, &hd, &ms, &att};
+                rc = launch_simple((const void*)attention_kernel, dim3((unsigned)nh, (unsigned)T), dim3(128),
+                                   (size_t)c.max_seq * sizeof(float), st, args2, "attention kernel");
+                if (rc) return rc;
+            }
             if (!tc && i8_ok(&L.w[3], 1, T)) {
                 // o on the int8 kernel: x (+)= att W^T, the residual in its epilogue
                 const XQ2 q2 = i8_stage(m, T, nq);
@@ -969,11 +1089,11 @@ struct Guard {
 // The one-launch decode step applies with one GPU, every layer set, one
 // weight type throughout and shapes the plan accepts.
 bool fused_plan(rq_llama* m, DecParams& p, size_t* smem) {
-    if (!m->fused || m->W != 1) return false;
+    if (!m->fused || m->W != 1 || m->kv4_page) return false;
     const rq_llama_config& c = m->cfg;
     int type = -1;
     for (int64_t l = 0; l < c.n_layers; l++) {
-        if (!m->layer_set[(size_t)l]) return false;
+        if (!m->layer_set[(size_t)l] || m->layers[(size_t)l].qn) return false;
         for (int i = 0; i < 7; i++) {
             const int t = m->layers[(size_t)l].w[i]->type;
             if (type < 0) type = t;
@@ -1108,6 +1228,12 @@ int rq_llama_create(rq_ctx* ctx, const rq_llama_config* cfg, rq_llama** out) {
     if (!rc) rc = dalloc(m, &m->dlayers, (size_t)c.n_layers);
     if (!rc) rc = dalloc(m, &m->bar, 1);
     if (!rc) rc = dalloc(m, &m->derr, 1);
+    if (!rc) rc = dalloc(m, &m->iota, (size_t)(T + 1));
+    if (!rc) {
+        std::vector<int32_t> iota((size_t)(T + 1));
+        for (int64_t i = 0; i <= T; i++) iota[(size_t)i] = (int32_t)i;
+        rc = cuda_error(cudaMemcpy(m->iota, iota.data(), iota.size() * 4, cudaMemcpyHostToDevice), "iota copy");
+    }
     if (!rc) {
         m->hlayers.assign((size_t)c.n_layers, rq::DecLayer{});
         m->layer_set.assign((size_t)c.n_layers, false);
@@ -1151,6 +1277,7 @@ int rq_llama_free(rq_llama* m) {
     if (!m) return RQ_OK;
     Guard g(m->ctx->device);
     for (void* p : m->allocs) cudaFree(p);
+    for (auto& L : m->layers) rq_kv4_free(L.kv4);
     for (rq_weight* w : m->owned) rq_weight_free(m->ctx, w);
     delete m;
     return RQ_OK;
@@ -1190,6 +1317,127 @@ int rq_llama_set_layer(rq_llama* m, int64_t layer, const rq_weight* const* w7, c
     D.vc = L.vc;
     m->layer_set[(size_t)layer] = true;
     return cuda_error(cudaMemcpy(m->dlayers + layer, &D, sizeof D, cudaMemcpyHostToDevice), "layer table copy");
+}
+
+int rq_llama_set_qk_norm(rq_llama* m, int64_t layer, const float* q_weight, const float* k_weight) {
+    if (!m || !q_weight || !k_weight) return set_error(RQ_ERR_INVALID, "rq_llama_set_qk_norm: NULL argument");
+    if (layer < 0 || layer >= m->cfg.n_layers)
+        return set_error(RQ_ERR_INVALID, "rq_llama_set_qk_norm: layer %lld", (long long)layer);
+    Guard g(m->ctx->device);
+    rq_llama::Layer& L = m->layers[(size_t)layer];
+    const size_t hd = (size_t)m->cfg.head_dim;
+    float* qn = L.qn;
+    float* kn = L.kn;
+    int rc = qn ? RQ_OK : dalloc(m, &qn, hd);
+    if (!rc && !kn) rc = dalloc(m, &kn, hd);
+    if (!rc) rc = copy_in(qn, q_weight, hd * 4);
+    if (!rc) rc = copy_in(kn, k_weight, hd * 4);
+    if (rc) return rc;
+    L.qn = qn;
+    L.kn = kn;
+    return RQ_OK;
+}
+
+int rq_llama_use_kv4(rq_llama* m, int page_size) {
+    if (!m) return set_error(RQ_ERR_INVALID, "rq_llama_use_kv4: NULL argument");
+    if (m->kv4_page) return set_error(RQ_ERR_INVALID, "rq_llama_use_kv4: the cache is in 4 bits already");
+    const rq_llama_config& c = m->cfg;
+    Guard g(m->ctx->device);
+    // everything is allocated before the f32 cache goes, so a failure leaves the model as it was
+    const int64_t T = c.max_batch_tokens, width = page_size > 0 ? (c.max_seq + page_size - 1) / page_size : 0;
+    const size_t first = m->allocs.size();
+    int rc = RQ_OK;
+    for (auto& L : m->layers)
+        if (!rc) rc = rq_kv4_create(m->ctx, width, page_size, (int)m->nkv_l, (int)c.head_dim, &L.kv4);
+    size_t ws = 0;
+    for (int64_t t = 1; t <= T && !rc; t++) {  // the largest workspace of any forward
+        rq_kv4_query q{};
+        q.n_tokens = q.max_q = t;
+        q.n_heads = m->nh_l;
+        q.batch = 1;
+        q.cu_q = t == 1 ? nullptr : m->iota;
+        q.table_width = width;
+        q.max_len = c.max_seq;
+        size_t n = 0;
+        rc = rq_kv4_attention_workspace(m->layers[0].kv4, &q, &n);
+        ws = std::max(ws, n);
+    }
+    int32_t *table = nullptr, *ring = nullptr, *state = nullptr, *rows = nullptr, *seek = nullptr;
+    uint8_t* wsp = nullptr;
+    if (!rc) rc = dalloc(m, &table, (size_t)width);
+    if (!rc) rc = dalloc(m, &ring, (size_t)width);
+    if (!rc) rc = dalloc(m, &state, 3);
+    if (!rc) rc = dalloc(m, &rows, (size_t)(2 * T));
+    if (!rc) rc = dalloc(m, &seek, 6);
+    if (!rc && ws) rc = dalloc(m, &wsp, ws);
+    if (!rc) {
+        std::vector<int32_t> host((size_t)width);
+        for (int64_t i = 0; i < width; i++) host[(size_t)i] = (int32_t)i;
+        const int32_t st0[3] = {0, (int32_t)width, 0};
+        rc = cuda_error(cudaMemcpy(ring, host.data(), host.size() * 4, cudaMemcpyHostToDevice), "ring copy");
+        if (!rc) rc = cuda_error(cudaMemcpy(state, st0, 12, cudaMemcpyHostToDevice), "ring state copy");
+        if (!rc) rc = cuda_error(cudaMemset(table, 0xFF, (size_t)width * 4), "table clear");
+        if (!rc) rc = cuda_error(cudaMemset(seek, 0, 24), "memset");
+        if (!rc) rc = cuda_error(cudaMemset(m->pos, 0, 4), "memset");
+        if (!rc) rc = cuda_error(cudaDeviceSynchronize(), "kv4 setup");
+    }
+    if (rc) {
+        for (size_t i = first; i < m->allocs.size(); i++) cudaFree(m->allocs[i]);
+        m->allocs.resize(first);
+        for (auto& L : m->layers) {
+            rq_kv4_free(L.kv4);
+            L.kv4 = nullptr;
+        }
+        return rc;
+    }
+    for (auto& L : m->layers) {
+        for (float* p : {L.kc, L.vc}) {
+            m->allocs.erase(std::find(m->allocs.begin(), m->allocs.end(), (void*)p));
+            cudaFree(p);
+        }
+        L.kc = L.vc = nullptr;
+    }
+    m->kv4_page = page_size;
+    m->kv4_width = width;
+    m->kv4_table = table;
+    m->kv4_ring = ring;
+    m->kv4_state = state;
+    m->kv4_rows = rows;
+    m->kv4_seek = seek;
+    m->kv4_ws = wsp;
+    m->kv4_ws_bytes = ws;
+    return RQ_OK;
+}
+
+int rq_llama_read_kv4(rq_llama* m, int64_t layer, int64_t pos, int64_t n, float* k, float* v) {
+    if (!m || !k || !v) return set_error(RQ_ERR_INVALID, "rq_llama_read_kv4: NULL argument");
+    if (!m->kv4_page) return set_error(RQ_ERR_INVALID, "rq_llama_read_kv4: the cache is f32 (rq_llama_use_kv4)");
+    const rq_llama_config& c = m->cfg;
+    if (layer < 0 || layer >= c.n_layers || pos < 0 || n < 0 || pos > c.max_seq - n)
+        return set_error(RQ_ERR_INVALID, "rq_llama_read_kv4: layer %lld, positions %lld..%lld", (long long)layer,
+                         (long long)pos, (long long)(pos + n));
+    if (!n) return RQ_OK;
+    Guard g(m->ctx->device);
+    std::vector<int32_t> table((size_t)m->kv4_width), slots((size_t)n);
+    int rc = cuda_error(cudaDeviceSynchronize(), "rq_llama_read_kv4");
+    if (!rc) rc = cuda_error(cudaMemcpy(table.data(), m->kv4_table, table.size() * 4, cudaMemcpyDeviceToHost), "table copy");
+    if (rc) return rc;
+    for (int64_t i = 0; i < n; i++) {
+        const int32_t page = table[(size_t)((pos + i) / m->kv4_page)];
+        slots[(size_t)i] = page < 0 ? -1 : page * m->kv4_page + (int32_t)((pos + i) % m->kv4_page);
+    }
+    const size_t one = (size_t)(n * m->nkv_l * c.head_dim);
+    int32_t* ds = nullptr;
+    float* d = nullptr;
+    rc = cuda_error(cudaMalloc((void**)&ds, slots.size() * 4), "cudaMalloc(read)");
+    if (!rc) rc = cuda_error(cudaMalloc((void**)&d, 2 * one * 4), "cudaMalloc(read)");
+    if (!rc) rc = cuda_error(cudaMemcpy(ds, slots.data(), slots.size() * 4, cudaMemcpyHostToDevice), "slot copy");
+    if (!rc) rc = rq_kv4_read(m->layers[(size_t)layer].kv4, ds, n, RQ_F32, d, d + one, nullptr);
+    if (!rc) rc = cuda_error(cudaMemcpy(k, d, one * 4, cudaMemcpyDefault), "k copy");
+    if (!rc) rc = cuda_error(cudaMemcpy(v, d + one, one * 4, cudaMemcpyDefault), "v copy");
+    cudaFree(ds);
+    cudaFree(d);
+    return rc;
 }
 
 int rq_llama_load_gguf_dir(rq_llama* m, const char* dir) {
@@ -1234,7 +1482,8 @@ int rq_llama_forward(rq_llama* m, const int32_t* tokens, int64_t T, int64_t inde
     cudaStream_t st = (cudaStream_t)stream;
     int32_t p = (int32_t)index_pos;
     int rc = cuda_error(cudaMemcpyAsync(m->tokens, tokens, (size_t)T * 4, cudaMemcpyHostToDevice, st), "token copy");
-    if (!rc) rc = cuda_error(cudaMemcpyAsync(m->pos, &p, 4, cudaMemcpyHostToDevice, st), "pos copy");
+    if (!rc && m->kv4_page) rc = kv4_seek(m, index_pos, st);
+    else if (!rc) rc = cuda_error(cudaMemcpyAsync(m->pos, &p, 4, cudaMemcpyHostToDevice, st), "pos copy");
     if (!rc) rc = forward_device(m, T, logits != nullptr, st);
     if (!rc && logits)
         rc = cuda_error(cudaMemcpyAsync(logits, m->logits, (size_t)c.vocab * 4, cudaMemcpyDefault, st), "logits copy");
@@ -1263,7 +1512,8 @@ int rq_llama_forward_all(rq_llama* m, const int32_t* tokens, int64_t T, int64_t 
     cudaStream_t st = (cudaStream_t)stream;
     int32_t p = (int32_t)index_pos;
     int rc = cuda_error(cudaMemcpyAsync(m->tokens, tokens, (size_t)T * 4, cudaMemcpyHostToDevice, st), "token copy");
-    if (!rc) rc = cuda_error(cudaMemcpyAsync(m->pos, &p, 4, cudaMemcpyHostToDevice, st), "pos copy");
+    if (!rc && m->kv4_page) rc = kv4_seek(m, index_pos, st);
+    else if (!rc) rc = cuda_error(cudaMemcpyAsync(m->pos, &p, 4, cudaMemcpyHostToDevice, st), "pos copy");
     if (!rc) rc = forward_device(m, T, logits != nullptr, st, true);
     if (!rc && logits)
         rc = cuda_error(cudaMemcpyAsync(logits, m->logits_all, (size_t)(T * c.vocab) * 4, cudaMemcpyDefault, st),
@@ -1324,6 +1574,10 @@ int rq_llama_truncate(rq_llama* m, int64_t new_len) {
         return set_error(RQ_ERR_INVALID, "rq_llama_truncate: %lld", (long long)new_len);
     Guard g(m->ctx->device);
     int32_t p = (int32_t)new_len;
+    if (m->kv4_page) {
+        const int rc = kv4_seek(m, new_len, nullptr);
+        return rc ? rc : cuda_error(cudaStreamSynchronize(nullptr), "truncate");
+    }
     // positions >= new_len are overwritten by later appends; only the
     // position moves (QuantStreamCache::truncate narrows the cache to new_len)
     return cuda_error(cudaMemcpy(m->pos, &p, 4, cudaMemcpyHostToDevice), "truncate");

@@ -211,6 +211,27 @@ int check_pages(const rq_ctx* ctx, int64_t batch, int page_size, int64_t table_s
 }
 
 }  // namespace
+
+int pages_extend(int64_t batch, int page_size, const int32_t* ctx_lens, const int32_t* new_lens, int32_t* table,
+                 int64_t table_stride, int64_t table_width, const int32_t* ring, int64_t n_pages, const int32_t* state_in,
+                 int32_t* state_out, int32_t* kv_lens, int32_t* cu_new, int32_t* positions, int32_t* slots, int64_t n_tokens,
+                 cudaStream_t st) {
+    PagesP p{(int)batch, page_size, ctx_lens, new_lens, table, table_stride, table_width, ring, n_pages, state_in,
+             state_out, kv_lens, cu_new, positions, slots, n_tokens, 1};
+    // one CTA writes 4096 rows in about the time a cluster takes to meet
+    while (p.ctas < 8 && (int64_t)p.ctas * 4096 < n_tokens) p.ctas *= 2;
+    void* args[] = {&p};
+    return launch_pdl((const void*)pages_extend_kernel, (unsigned)p.ctas, kThreads, 0, st, args, "page table kernel",
+                      (unsigned)p.ctas);
+}
+
+int pages_release(int64_t batch, int page_size, const int32_t* held_lens, const int32_t* keep_lens, int32_t* table,
+                  int64_t table_stride, int64_t table_width, int32_t* ring, int64_t n_pages, int32_t* state, cudaStream_t st) {
+    ReleaseP p{(int)batch, page_size, held_lens, keep_lens, table, table_stride, table_width, ring, n_pages, state};
+    void* args[] = {&p};
+    return launch_pdl((const void*)pages_release_kernel, 1, kThreads, 0, st, args, "page release kernel");
+}
+
 }  // namespace rq
 
 using namespace rq;
@@ -233,13 +254,8 @@ int rq_pages_extend(rq_ctx* ctx, int64_t batch, int page_size, const int32_t* ct
         {slots, "slots", n_tokens > 0}};
     for (auto& q : ptrs)
         if (q.used && (rc = check_device_ptr(ctx, q.p, fn, q.name))) return rc;
-    PagesP p{(int)batch, page_size, ctx_lens, new_lens, table, table_stride, table_width, ring, n_pages, state_in,
-             state_out, kv_lens, cu_new, positions, slots, n_tokens, 1};
-    // one CTA writes 4096 rows in about the time a cluster takes to meet
-    while (p.ctas < 8 && (int64_t)p.ctas * 4096 < n_tokens) p.ctas *= 2;
-    void* args[] = {&p};
-    return launch_pdl((const void*)pages_extend_kernel, (unsigned)p.ctas, kThreads, 0, (cudaStream_t)stream, args,
-                      "page table kernel", (unsigned)p.ctas);
+    return pages_extend(batch, page_size, ctx_lens, new_lens, table, table_stride, table_width, ring, n_pages, state_in,
+                        state_out, kv_lens, cu_new, positions, slots, n_tokens, (cudaStream_t)stream);
 }
 
 int rq_pages_release(rq_ctx* ctx, int64_t batch, int page_size, const int32_t* held_lens, const int32_t* keep_lens,
@@ -256,9 +272,8 @@ int rq_pages_release(rq_ctx* ctx, int64_t batch, int page_size, const int32_t* h
     if (!rc) rc = check_device_ptr(ctx, ring, fn, "ring");
     if (!rc) rc = check_device_ptr(ctx, state, fn, "state");
     if (rc) return rc;
-    ReleaseP p{(int)batch, page_size, held_lens, keep_lens, table, table_stride, table_width, ring, n_pages, state};
-    void* args[] = {&p};
-    return launch_pdl((const void*)pages_release_kernel, 1, kThreads, 0, (cudaStream_t)stream, args, "page release kernel");
+    return pages_release(batch, page_size, held_lens, keep_lens, table, table_stride, table_width, ring, n_pages, state,
+                         (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -13,7 +13,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from ._lib import LlamaConfig, check
+from ._lib import LlamaConfig, RqError, check
 from .linear import Context, QWeight
 
 try:
@@ -42,10 +42,12 @@ class StreamingLlamaQuantized:
         h = ctypes.c_void_p()
         check(_lib.lib().rq_llama_create(self.ctx.handle, ctypes.byref(c), ctypes.byref(h)))
         self.handle = h
+        self._kv_heads = cfg["n_kv_heads"]
         self._keep: list = []  # weights borrowed by the library
 
     def set_layer(self, layer: int, weights: list, rms1, rms2) -> None:
         assert len(weights) == 7
+        self._kv_heads = weights[1].out // self.cfg["head_dim"]  # this rank's
         arr = (ctypes.c_void_p * 7)(*[w.handle.value for w in weights])
         r1 = np.ascontiguousarray(rms1, dtype=np.float32)
         r2 = np.ascontiguousarray(rms2, dtype=np.float32)
@@ -66,6 +68,28 @@ class StreamingLlamaQuantized:
         """The QWeights (q, k, v, o, gate, up, down) set for a layer."""
         return self._keep[layer]
 
+    def set_qk_norm(self, layer: int, q_weight, k_weight) -> None:
+        """Norms of q and k per head ([head_dim] each) before the rotation."""
+        q = np.ascontiguousarray(q_weight, dtype=np.float32).reshape(-1)
+        k = np.ascontiguousarray(k_weight, dtype=np.float32).reshape(-1)
+        if q.size != self.cfg["head_dim"] or k.size != self.cfg["head_dim"]:
+            raise RqError(1, f"set_qk_norm: weights of {q.size} and {k.size}, expected {self.cfg['head_dim']}")
+        check(_lib.lib().rq_llama_set_qk_norm(self.handle, layer, q.ctypes.data, k.ctypes.data))
+
+    def use_kv4(self, page_size: int = 64) -> None:
+        """Holds the cache in 4 bits and in pages (rq_llama_use_kv4); call it
+        before the first forward."""
+        check(_lib.lib().rq_llama_use_kv4(self.handle, page_size))
+
+    def read_kv4(self, layer: int, pos: int, n: int):
+        """(k, v) f32 [n, n_kv_heads, head_dim] that the 4-bit cache holds
+        (one GPU, or this rank's heads)."""
+        heads = self._kv_heads
+        k = np.empty((n, heads, self.cfg["head_dim"]), dtype=np.float32)
+        v = np.empty_like(k)
+        check(_lib.lib().rq_llama_read_kv4(self.handle, layer, pos, n, k.ctypes.data, v.ctypes.data))
+        return k, v
+
     def set_embedding(self, embed_f16) -> None:
         e = np.ascontiguousarray(embed_f16).view(np.uint16)
         check(_lib.lib().rq_llama_set_embedding(self.handle, e.ctypes.data))
@@ -75,14 +99,28 @@ class StreamingLlamaQuantized:
         h = np.ascontiguousarray(lm_head_f16).view(np.uint16)
         check(_lib.lib().rq_llama_set_head(self.handle, n.ctypes.data, h.ctypes.data))
 
-    def forward(self, input_ids, index_pos: int, want_logits: bool = True):
-        """Logits (f32 [vocab], single rank only; None when not wanted) of the
-        last position and the greedy token."""
+    def _logits(self, shape: tuple, want: bool, out):
+        """(buffer, pointer) for logits of a shape: a new host array, the
+        caller's CUDA tensor, or none."""
+        if out is not None:
+            if not (torch is not None and isinstance(out, torch.Tensor) and out.dtype is torch.float32
+                    and tuple(out.shape) == shape and out.is_contiguous() and out.is_cuda
+                    and out.device.index == self.ctx.device):
+                raise RqError(1, f"logits_out: a contiguous float32 {list(shape)} on cuda:{self.ctx.device} is wanted")
+            # the library writes it on the legacy stream, before the call returns
+            torch.cuda.current_stream(out.device).synchronize()
+            return out, out.data_ptr()
+        logits = np.empty(shape, dtype=np.float32) if want else None
+        return logits, logits.ctypes.data if want else None
+
+    def forward(self, input_ids, index_pos: int, want_logits: bool = True, logits_out=None):
+        """Logits (f32 [vocab], single rank only; None when not wanted; in
+        logits_out, a CUDA tensor, where given) of the last position and the
+        greedy token."""
         ids = np.ascontiguousarray(input_ids, dtype=np.int32).reshape(-1)
-        logits = np.empty(self.cfg["vocab"], dtype=np.float32) if want_logits else None
+        logits, ptr = self._logits((self.cfg["vocab"],), want_logits, logits_out)
         nxt = ctypes.c_int32()
-        check(_lib.lib().rq_llama_forward(self.handle, ids.ctypes.data, ids.size, index_pos,
-                                          logits.ctypes.data if want_logits else None,
+        check(_lib.lib().rq_llama_forward(self.handle, ids.ctypes.data, ids.size, index_pos, ptr,
                                           ctypes.byref(nxt), None))
         return logits, int(nxt.value)
 
@@ -106,14 +144,14 @@ class StreamingLlamaQuantized:
                                          ctypes.byref(p)))
         return buf[:min(n.value, cap)].tolist(), p.value
 
-    def forward_all(self, input_ids, index_pos: int, want_logits: bool = False):
+    def forward_all(self, input_ids, index_pos: int, want_logits: bool = False, logits_out=None):
         """The verify forward (forward_all, src/streaming_quantized.rs:611-620):
-        greedy token at every position, and [T, vocab] logits when wanted."""
+        greedy token at every position, and [T, vocab] logits when wanted (in
+        logits_out, a CUDA tensor, where given)."""
         ids = np.ascontiguousarray(input_ids, dtype=np.int32).reshape(-1)
-        logits = np.empty((ids.size, self.cfg["vocab"]), dtype=np.float32) if want_logits else None
+        logits, ptr = self._logits((ids.size, self.cfg["vocab"]), want_logits, logits_out)
         amax = np.empty(ids.size, dtype=np.int32)
-        check(_lib.lib().rq_llama_forward_all(self.handle, ids.ctypes.data, ids.size, index_pos,
-                                              logits.ctypes.data if want_logits else None,
+        check(_lib.lib().rq_llama_forward_all(self.handle, ids.ctypes.data, ids.size, index_pos, ptr,
                                               amax.ctypes.data, None))
         return logits, amax.tolist()
 
