@@ -70,14 +70,14 @@ struct AttnP {
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // the same from a zero accumulator
 __device__ __forceinline__ void mma16816_0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
@@ -186,7 +186,7 @@ struct Warp {
     int rpos[H];      // position of the row's query; -1: no row
     float oacc[NB][4][4];
     float m[H], l[H];
-    int E;
+    float E;
     float bound;      // 2^E
     __half2 inv;      // 2^-E
     int full0, full1;      // tiles that every row sees whole
@@ -258,24 +258,21 @@ struct Warp {
         seen = min(o.held, o.pos0 + i1 + 1);
     }
     __device__ __forceinline__ void set_scale(int e) {
-        E = e;
+        E = (float)e;
         bound = __int_as_float((127 + e) << 23);
         inv = __float2half2_rn(__int_as_float((127 - e) << 23));
     }
     __device__ __forceinline__ void scale_rows(const float (&f)[H]) {
-        const float2 a = make_float2(f[0], f[0]), c = make_float2(f[H - 1], f[H - 1]), z = make_float2(0.0f, 0.0f);
         // rows g and g + 8 of the accumulators: in the 8-row modes both
         // halves belong to row g
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int n = 0; n < 4; n++) {
-                const float2 u = fma2(make_float2(oacc[b][n][0], oacc[b][n][1]), a, z);
-                const float2 v = fma2(make_float2(oacc[b][n][2], oacc[b][n][3]), c, z);
-                oacc[b][n][0] = u.x;
-                oacc[b][n][1] = u.y;
-                oacc[b][n][2] = v.x;
-                oacc[b][n][3] = v.y;
+                oacc[b][n][0] *= f[0];
+                oacc[b][n][1] *= f[0];
+                oacc[b][n][2] *= f[H - 1];
+                oacc[b][n][3] *= f[H - 1];
             }
     }
 
@@ -285,19 +282,29 @@ struct Warp {
     // tokens 4 t .. + 3.
     template <class KOp, class KSc, class VOp, class VSc>
     __device__ __forceinline__ void tile(const AttnP& p, int tile_at, int t, KOp kop, KSc ksc, VOp vop, VSc vsc) {
+        if (tile_at >= full0 && tile_at < full1) tile<true>(p, tile_at, t, kop, ksc, vop, vsc);
+        else tile<false>(p, tile_at, t, kop, ksc, vop, vsc);
+    }
+    template <bool full, class KOp, class KSc, class VOp, class VSc>
+    __device__ __forceinline__ void tile(const AttnP& p, int tile_at, int t, KOp kop, KSc ksc, VOp vop, VSc vsc) {
         float2 sc[2][H];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
 #pragma unroll
             for (int h = 0; h < H; h++) sc[n][h] = make_float2(0.0f, 0.0f);
+            float c[NB][4];  // all blocks' first steps, then the second ones: no product waits for the one before
+            uint4 w[NB];
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                float c[4];
-                const uint4 w = kop(n, b);
-                mma16816_0(c, aq[b][0], w.x, w.y);
-                mma16816(c, aq[b][1], w.z, w.w);
+                w[b] = kop(n, b);
+                mma16816_0(c[b], aq[b][0], w[b].x, w[b].y);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) mma16816(c[b], aq[b][1], w[b].z, w[b].w);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
                 const float2 d = unpack(ksc(n, b));
-                const float2 lo = make_float2(c[0], c[1]), hi = make_float2(c[2], c[3]);
+                const float2 lo = make_float2(c[b][0], c[b][1]), hi = make_float2(c[b][2], c[b][3]);
                 if (MODE == kOne16) {
                     sc[n][0] = fma2(lo, d, sc[n][0]);
                     sc[n][H - 1] = fma2(hi, d, sc[n][H - 1]);
@@ -309,21 +316,21 @@ struct Warp {
         uint2 vs[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) vs[b] = vsc(b);
-        const bool full = tile_at >= full0 && tile_at < full1;
         const int j0 = tile_at * kKv4Tile + 4 * t;
         uint32_t hid01[H], hid23[H];  // halves of all ones: tokens that the row sees
 #pragma unroll
         for (int h = 0; h < H; h++) hid01[h] = hid23[h] = 0xFFFFFFFFu;
-        if (!full) {
+        if constexpr (!full) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int j = j0 + i;
                 const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu;
                 if (j >= seen) {  // nobody's: whatever scale lies there counts for nothing
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
+                    for (int b = 0; b < NB; b++) {
                         if (i < 2) vs[b].x &= ~half;
                         else vs[b].y &= ~half;
+                    }
                 }
 #pragma unroll
                 for (int h = 0; h < H; h++)
@@ -346,7 +353,7 @@ struct Warp {
             pr[h][1] = sc[0][h].y * qs[h];
             pr[h][2] = sc[1][h].x * qs[h];
             pr[h][3] = sc[1][h].y * qs[h];
-            if (!full) {
+            if constexpr (!full) {
                 if (!(hid01[h] & 0xFFFFu)) pr[h][0] = -INFINITY;
                 if (!(hid01[h] >> 16)) pr[h][1] = -INFINITY;
                 if (!(hid23[h] & 0xFFFFu)) pr[h][2] = -INFINITY;
@@ -354,7 +361,7 @@ struct Warp {
             }
             top[h] = fmaxf(fmaxf(pr[h][0], pr[h][1]), fmaxf(pr[h][2], pr[h][3]));
         }
-        float lg = fmaxf(lg2(dmax) - (float)E, -7.0f);
+        float lg = fmaxf(lg2(dmax) - E, -7.0f);
         bool move = dmax > bound;
 #pragma unroll
         for (int h = 0; h < H; h++) {
@@ -370,13 +377,13 @@ struct Warp {
                 for (int o = 16; o > 0; o >>= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
                 int e;
                 frexpf(w, &e);  // w <= 2^e
-                const float down = __int_as_float((127 + E - e) << 23);
+                const float down = __int_as_float((127 + (int)E - e) << 23);
                 float f[H];
 #pragma unroll
                 for (int h = 0; h < H; h++) f[h] = down;
                 scale_rows(f);
                 set_scale(e);
-                lg = fmaxf(lg2(dmax) - (float)E, -7.0f);
+                lg = fmaxf(lg2(dmax) - E, -7.0f);
 #pragma unroll
                 for (int h = 0; h < H; h++) {
                     mx[h] = top[h] + lg;
@@ -394,7 +401,7 @@ struct Warp {
             }
             scale_rows(al);
         }
-        uint32_t ph[H][2], pl[H][2];
+        uint32_t ph[H][2], pl[H][2], nh[2];
 #pragma unroll
         for (int h = 0; h < H; h++) {
             const float base = m[h] == -INFINITY ? 0.0f : m[h];
@@ -406,7 +413,8 @@ struct Warp {
                 ph[h][i] = pack(pr[h][2 * i], pr[h][2 * i + 1]);
                 if (MODE == kSplit8) {
                     const float2 back = unpack(ph[h][i]);
-                    pl[h][i] = pack(pr[h][2 * i] - back.x, pr[h][2 * i + 1] - back.y);
+                    pl[h][i] = pack(back.x - pr[h][2 * i], back.y - pr[h][2 * i + 1]);  // -pl
+                    nh[i] = ph[h][i] ^ 0x80008000u;
                 }
             }
         }
@@ -425,11 +433,12 @@ struct Warp {
                     a[2] = as_u32(y);
                     a[1] = a[3] = 0u;
                     if (MODE == kSplit8) {
-                        a[1] = as_u32(__hfma2(as_h2(pl[h][0]), d01, __hfma2(as_h2(ph[h][0]), d01, __hneg2(x))));
-                        a[3] = as_u32(__hfma2(as_h2(pl[h][1]), d23, __hfma2(as_h2(ph[h][1]), d23, __hneg2(y))));
+                        // minus the low part, which spares the negations: value() subtracts
+                        a[1] = as_u32(__hfma2(as_h2(pl[h][0]), d01, __hfma2(as_h2(nh[0]), d01, x)));
+                        a[3] = as_u32(__hfma2(as_h2(pl[h][1]), d23, __hfma2(as_h2(nh[1]), d23, y)));
                     }
                 }
-                if (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
+                if constexpr (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
                     if (MODE == kOne16) {
                         a[h] &= hid01[h];
                         a[2 + h] &= hid23[h];
@@ -462,8 +471,8 @@ struct Warp {
     __device__ __forceinline__ float2 value(int b, int n, int h) const {
         float2 v = h ? make_float2(oacc[b][n][2], oacc[b][n][3]) : make_float2(oacc[b][n][0], oacc[b][n][1]);
         if (MODE == kSplit8) {
-            v.x += oacc[b][n][2];
-            v.y += oacc[b][n][3];
+            v.x -= oacc[b][n][2];
+            v.y -= oacc[b][n][3];
         }
         return make_float2(v.x * bound, v.y * bound);
     }

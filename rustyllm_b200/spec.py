@@ -14,6 +14,13 @@ from __future__ import annotations
 
 from collections import deque
 
+import torch
+
+from . import _lib
+from ._lib import check
+from .kv4 import _PAIR, dtype_of, int32, refuse, stream_of
+from .linear import Context
+
 
 def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
     """(tokens [batch, n + 1], accepted [batch]) int32: the drafted tokens
@@ -23,32 +30,27 @@ def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
     (float32); rq_spec_verify of include/rq.h.  n_drafts [batch] (int32)
     limits a row's drafts.  A row of tokens is the accepted drafts, one drawn
     token and -1s; with n = 0 the call samples from p."""
-    import ctypes
-
-    import torch
-
-    from . import _lib
-    from .kv4 import dtype_of, int32, need, stream_of
-    from .linear import Context
-    need(isinstance(p, torch.Tensor) and p.is_cuda and p.dim() == 3 and p.stride(2) == 1,
-         "p: a CUDA tensor [batch, n + 1, vocab] with contiguous rows is wanted")
+    if not (isinstance(p, torch.Tensor) and p.is_cuda and p.dim() == 3 and p.stride(2) == 1 and p.shape[1] > 0):
+        refuse("p: a CUDA tensor [batch, n + 1, vocab] with contiguous rows is wanted")
     b, n, vocab = p.shape[0], p.shape[1] - 1, p.shape[2]
     dev = p.device
-    need(q is None or (q.shape == (b, n, vocab) and q.dtype == p.dtype and q.device == dev
-                       and (q.stride(2) == 1 or q.numel() == 0)),
-         f"q: [{b}, {n}, {vocab}] {p.dtype} with contiguous rows on {dev} is wanted")
-    int32(drafts, "drafts", dev, (b, n))
-    for name, x, shape in (("u", u, (b, n)), ("r", r, (b,))):
-        need(x.dtype is torch.float32 and tuple(x.shape) == shape and x.device == dev and x.is_contiguous(),
-             f"{name}: a contiguous float32 {list(shape)} on {dev} is wanted")
+    if not (q is None or (q.shape == (b, n, vocab) and q.dtype == p.dtype and q.device == dev
+                          and (n == 0 or q.stride(2) == 1))):
+        refuse(f"q: [{b}, {n}, {vocab}] {p.dtype} with contiguous rows on {dev} is wanted")
+    int32(drafts, "drafts", dev)
+    if drafts.shape != (b, n):
+        refuse(f"drafts: [{b}, {n}] is wanted")
+    if not (u.dtype is torch.float32 and u.shape == (b, n) and u.device == dev and u.is_contiguous()):
+        refuse(f"u: a contiguous float32 [{b}, {n}] on {dev} is wanted")
+    if not (r.dtype is torch.float32 and r.shape == (b,) and r.device == dev and r.is_contiguous()):
+        refuse(f"r: a contiguous float32 [{b}] on {dev} is wanted")
     if n_drafts is not None:
-        int32(n_drafts, "n_drafts", dev, (b,))
+        int32(n_drafts, "n_drafts", dev, b)
     tokens = torch.empty((b, n + 1), dtype=torch.int32, device=dev)
     accepted = torch.empty(b, dtype=torch.int32, device=dev)
-    pair = ctypes.c_int64 * 2
-    _lib.check(_lib.lib().rq_spec_verify(
-        Context.get(dev.index).handle, dtype_of(p, "p"), p.data_ptr(), pair(p.stride(0), p.stride(1)),
-        None if q is None else q.data_ptr(), None if q is None else pair(q.stride(0), q.stride(1)), drafts.data_ptr(),
+    check(_lib.lib().rq_spec_verify(
+        Context.get(dev.index).handle, dtype_of(p, "p"), p.data_ptr(), _PAIR(p.stride(0), p.stride(1)),
+        None if q is None else q.data_ptr(), None if q is None else _PAIR(q.stride(0), q.stride(1)), drafts.data_ptr(),
         None if n_drafts is None else n_drafts.data_ptr(), u.data_ptr(), r.data_ptr(), b, n, vocab, tokens.data_ptr(),
         accepted.data_ptr(), stream_of(dev)))
     return tokens, accepted
@@ -62,7 +64,6 @@ class SpecDecoder:
         self.target, self.draft = target, draft
         self.temperature = float(temperature)
         if self.temperature > 0:
-            import torch
             self.device = torch.device("cuda", target.ctx.device)
             self.gen = torch.Generator(device=self.device).manual_seed(seed)
         self.k_max = k
@@ -73,7 +74,6 @@ class SpecDecoder:
     def _probs(self, model, ids, pos, every):
         """softmax(logits / temperature) of the last (or every) position,
         [1, rows, vocab]."""
-        import torch
         rows = len(ids) if every else 1
         out = torch.empty((rows, model.cfg["vocab"]), dtype=torch.float32, device=self.device)
         if every:
@@ -83,12 +83,10 @@ class SpecDecoder:
         return torch.softmax(out.div_(self.temperature), -1)[None]
 
     def _uniform(self, *shape):
-        import torch
         return torch.rand(*shape, device=self.device, generator=self.gen)
 
     def _draw(self, p):
         """A token from p [1, 1, vocab]: the verification of no draft."""
-        import torch
         none = torch.empty((1, 0), dtype=torch.int32, device=self.device)
         return spec_verify(p, none, self._uniform(1, 0), self._uniform(1))[0]
 
@@ -110,7 +108,6 @@ class SpecDecoder:
         k = len(drafts)
         self.stats["target_forwards"] += 1
         if self.temperature > 0:
-            import torch
             p = self._probs(self.target, [last] + drafts, index_pos, True)
             tokens, accepted = spec_verify(p, torch.tensor([drafts], dtype=torch.int32, device=self.device).reshape(1, k),
                                            self._uniform(1, k), self._uniform(1), q=torch.cat(probs, 1) if k else None)
