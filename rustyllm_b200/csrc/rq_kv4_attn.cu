@@ -26,7 +26,7 @@
 //    positions for the same rows, so one row tile uses all lanes of the GPU;
 //    its operands are built in registers from the record that one bulk copy
 //    brought to shared memory.  The warps join through shared memory, the
-//    splits of the long axis through a second launch.
+//    pieces of a unit that went to several CTAs through a second launch.
 //  - many rows (prompts): the warps hold different rows; each turns one record
 //    into f16 operands in shared memory and all use them, which takes the
 //    unpacking (144 of about 340 instructions a tile) off three of four warps.
@@ -39,12 +39,16 @@ namespace rq {
 namespace {
 
 constexpr int kWarps = 4;       // warps of a CTA
-constexpr int kStages = 4;      // records in flight per warp (few rows)
-constexpr int kStagesRows = 2;  // (many rows: a step of kWarps records each)
+constexpr int kStages = 3;      // pairs of tiles in flight per warp (few rows)
+constexpr int kStagesRows = 2;  // (many rows)
 constexpr float kLazy = 8.0f;   // log2 of the largest |P|
 constexpr float kFloor = 0.0078125f;  // 2^-7
 
-enum Mode { kSplit8 = 0, kOne8 = 1, kOne16 = 2 };  // rows 8 hi + lo, 8, 16
+enum Mode { kSplit8, kOne16 };  // 8 rows of hi + lo parts, 16 rows of one part
+
+struct Magic {  // see codes_even
+    uint32_t even, odd;
+};
 
 struct AttnP {
     const uint8_t* data;
@@ -64,8 +68,13 @@ struct AttnP {
     int table_slots;  // positions of a table row
     int window;       // 0: none
     float scale;      // times log2(e)
-    float* part;  // [n_tokens * n_heads][splits][head_dim]
-    float2* ml;   // [n_tokens * n_heads][splits]
+    // sums of pieces: few rows, [2 ctas][8 or 16 rows][head_dim], CTA i's piece
+    // at its range's start and one that starts later; many rows, [n_tokens *
+    // n_heads][splits][head_dim]
+    float* part;
+    float2* ml;  // their running maxima and sums
+    int4* desc;  // few rows, [ctas]: the unit that starts in CTA i and goes on behind it
+    Magic magic;
     int* err;
 };
 
@@ -111,12 +120,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 // nibbles 0 and 4 (even) or 1 and 5 (odd) of w as f16 pairs c - 8: a nibble
-// placed in the mantissa of 1024 (or, four bits up, of 64) is that value + c
-__device__ __forceinline__ uint32_t codes_even(uint32_t w) {
-    return as_u32(__hsub2(as_h2((w & 0x000F000Fu) | 0x64006400u), __half2half2(__ushort_as_half(0x6408))));
+// placed in the mantissa of 1024 (or, four bits up, of 64) is that value + c.
+// The two constants come from the launch's parameters: known ones would be
+// immediates, and a second immediate costs lop3 another instruction (33 of 400 a
+// tile).
+constexpr uint32_t kEven = 0x64006400u, kOdd = 0x54005400u;
+__device__ __forceinline__ uint32_t codes_even(uint32_t w, Magic m) {
+    uint32_t h;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(h) : "r"(w), "r"(m.even));
+    return as_u32(__hsub2(as_h2(h), __half2half2(__ushort_as_half(0x6408))));
 }
-__device__ __forceinline__ uint32_t codes_odd(uint32_t w) {
-    return as_u32(__hsub2(as_h2((w & 0x00F000F0u) | 0x54005400u), __half2half2(__ushort_as_half(0x5480))));
+__device__ __forceinline__ uint32_t codes_odd(uint32_t w, Magic m) {
+    uint32_t h;
+    asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(h) : "r"(w), "r"(m.odd));
+    return as_u32(__hsub2(as_h2(h), __half2half2(__ushort_as_half(0x5480))));
 }
 __device__ __forceinline__ uint32_t pack(float a, float b) { return as_u32(__floats2half2_rn(a, b)); }
 __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(as_h2(v)); }
@@ -141,39 +158,48 @@ __device__ __forceinline__ void load_words(const uint8_t* region, int lane, uint
 
 // The four operand words of one code word of K (two steps of two), of two
 // words of V (four column tiles of two)
-__device__ __forceinline__ uint4 k_operands(uint32_t w) {
-    return make_uint4(codes_even(w), codes_odd(w), codes_even(w >> 8), codes_odd(w >> 8));
+__device__ __forceinline__ uint4 k_operands(uint32_t w, Magic m) {
+    return make_uint4(codes_even(w, m), codes_odd(w, m), codes_even(w >> 8, m), codes_odd(w >> 8, m));
+}
+__device__ __forceinline__ uint4 v_operands(uint32_t w0, uint32_t w1, Magic m) {
+    return make_uint4(codes_even(w0, m), codes_even(w1, m), codes_odd(w0, m), codes_odd(w1, m));
 }
 
-// The rows of one (sequence, kv head, row tile of R): what the main and the
-// join kernel agree on.
-struct Rows {
-    int b, kvh, r0, rows, n_q, q0;
-    int pos0, held;         // position of query 0; positions that the table can hold
-    int tile0, tile1, per;  // tiles seen by any row; tiles of a split
+// A sequence's queries and positions
+struct Seq {
+    int n_q, q0;
+    int pos0, held;    // position of query 0; positions that the table can hold
+    __device__ __forceinline__ Seq(const AttnP& p, int b) {
+        q0 = p.cu_q ? p.cu_q[b] : b;
+        n_q = p.cu_q ? min(max(p.cu_q[b + 1] - q0, 0), p.max_q) : 1;
+        const int len = max(p.kv_lens[b], 0);
+        held = min(len, p.table_slots);
+        pos0 = len - n_q;
+    }
+    // tiles that queries i0 .. i1 see
+    __device__ __forceinline__ void tiles(const AttnP& p, int i0, int i1, int& tile0, int& tile1) const {
+        const int hi = max(0, min(held, pos0 + i1 + 1));
+        const int lo = p.window > 0 ? max(0, pos0 + i0 - p.window + 1) : 0;
+        tile0 = lo / kKv4Tile;
+        tile1 = max(tile0, hi / kKv4Tile + (hi % kKv4Tile != 0));
+    }
 };
-
+// A unit of work: rows r0 .. of kv head kvh of sequence b
+struct Rows : Seq {
+    int b, kvh, r0, rows;
+    __device__ __forceinline__ Rows(const AttnP& p, int b, int kvh, int r0)
+        : Seq(p, b), b(b), kvh(kvh), r0(r0), rows(n_q * p.group) {}
+};
+// Unit `unit` of the many-rows form, row tiles of R; false: no such rows
 template <int R>
-__device__ __forceinline__ bool find_rows(const AttnP& p, int64_t unit, Rows& o) {
-    const int rt = (int)(unit % p.row_tiles);
-    unit /= p.row_tiles;
-    o.kvh = (int)(unit % p.n_kv);
-    o.b = (int)(unit / p.n_kv);
-    o.q0 = p.cu_q ? p.cu_q[o.b] : o.b;
-    o.n_q = p.cu_q ? min(max(p.cu_q[o.b + 1] - o.q0, 0), p.max_q) : 1;
-    o.rows = o.n_q * p.group;
-    o.r0 = rt * R;
-    if (o.r0 >= o.rows) return false;
-    const int len = max(p.kv_lens[o.b], 0);
-    o.held = min(len, p.table_slots);
-    o.pos0 = len - o.n_q;
-    const int i0 = o.r0 / p.group, i1 = min(o.n_q - 1, (o.r0 + R - 1) / p.group);
-    const int hi = max(0, min(o.held, o.pos0 + i1 + 1));
-    const int lo = p.window > 0 ? max(0, o.pos0 + i0 - p.window + 1) : 0;
-    o.tile0 = lo / kKv4Tile;
-    o.tile1 = max(o.tile0, hi / kKv4Tile + (hi % kKv4Tile != 0));
-    o.per = max((o.tile1 - o.tile0 + p.splits - 1) / p.splits, kWarps);
-    return true;
+__device__ __forceinline__ Rows unit_rows(const AttnP& p, int unit) {
+    const int bk = unit / p.row_tiles, b = bk / p.n_kv;
+    return Rows(p, b, bk - b * p.n_kv, (unit - bk * p.row_tiles) * R);
+}
+template <int R>
+__device__ __forceinline__ void unit_tiles(const AttnP& p, const Rows& o, int& tile0, int& tile1, int& per) {
+    o.tiles(p, o.r0 / p.group, min(o.n_q - 1, (o.r0 + R - 1) / p.group), tile0, tile1);
+    per = max((tile1 - tile0 + 2 * p.splits - 1) / (2 * p.splits), kWarps) * 2;  // of a split, whole pairs
 }
 
 // One warp's query rows, running sums and the work on one tile.
@@ -196,7 +222,7 @@ struct Warp {
 #pragma unroll
         for (int h = 0; h < H; h++) {
             const int r = r0 + g + 8 * h;
-            const int i = r / p.group;
+            const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
             const int64_t tok = (int64_t)o.q0 + i;
             const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
             rpos[h] = ok ? o.pos0 + i : -1;
@@ -207,7 +233,7 @@ struct Warp {
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[b][e] = 0.0f;
                 if (ok)
-                    load8(static_cast<const T*>(p.q) + tok * p.qt + (o.kvh * p.group + r % p.group) * p.qh + 32 * b + 8 * t,
+                    load8(static_cast<const T*>(p.q) + tok * p.qt + head * p.qh + 32 * b + 8 * t,
                           p.wide, x[b]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[b][e]));
@@ -232,13 +258,9 @@ struct Warp {
                         if (MODE == kOne16) {
                             aq[b][s][2 * j + h] = hi;
                         } else {
+                            const float2 back = unpack(hi);
                             aq[b][s][2 * j] = hi;
-                            if (MODE == kSplit8) {
-                                const float2 back = unpack(hi);
-                                aq[b][s][2 * j + 1] = pack(f0 - back.x, f1 - back.y);
-                            } else {
-                                aq[b][s][2 * j + 1] = 0u;
-                            }
+                            aq[b][s][2 * j + 1] = pack(f0 - back.x, f1 - back.y);
                         }
                     }
             m[h] = -INFINITY;
@@ -276,91 +298,96 @@ struct Warp {
             }
     }
 
-    // kop(n, b): four operand words of score tile n, block b; ksc(n, b): the
-    // f16 pair of K scales of tokens 4 t + 2 n, + 1; vop(b, half): operand
-    // words of column tiles 2 half, 2 half + 1 of block b; vs: the V scales of
-    // tokens 4 t .. + 3.
-    template <class KOp, class KSc, class VOp, class VSc>
-    __device__ __forceinline__ void tile(const AttnP& p, int tile_at, int t, KOp kop, KSc ksc, VOp vop, VSc vsc) {
-        if (tile_at >= full0 && tile_at < full1) tile<true>(p, tile_at, t, kop, ksc, vop, vsc);
-        else tile<false>(p, tile_at, t, kop, ksc, vop, vsc);
-    }
-    template <bool full, class KOp, class KSc, class VOp, class VSc>
-    __device__ __forceinline__ void tile(const AttnP& p, int tile_at, int t, KOp kop, KSc ksc, VOp vop, VSc vsc) {
-        float2 sc[2][H];
+    // NT tiles at tile_at, + 1 that the operand source `src` holds:
+    //   src.k(i) / src.v(i)  make tile i's K / V operands available
+    //   src.kop(i, n, b)     four operand words of score tile n, block b
+    //   src.ksc(i, n, b)     the f16 pair of K scales of tokens 4 t + 2 n, + 1
+    //   src.vop(i, b, half)  operand words of column tiles 2 half, 2 half + 1
+    //   src.vsc(i, b)        the V scales of tokens 4 t .. + 3
+    // full: every row sees every position.
+    template <int NT, bool full, class Src>
+    __device__ __forceinline__ void tiles(const AttnP& p, int tile_at, int t, Src& src) {
+        float2 sc[NT][2][H];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
+        for (int i = 0; i < NT; i++) {
+            src.k(i);
 #pragma unroll
-            for (int h = 0; h < H; h++) sc[n][h] = make_float2(0.0f, 0.0f);
-            float c[NB][4];  // all blocks' first steps, then the second ones: no product waits for the one before
-            uint4 w[NB];
+            for (int n = 0; n < 2; n++) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                w[b] = kop(n, b);
-                mma16816_0(c[b], aq[b][0], w[b].x, w[b].y);
-            }
+                for (int h = 0; h < H; h++) sc[i][n][h] = make_float2(0.0f, 0.0f);
+                float c[NB][4];  // all blocks' first steps, then the second ones: no product waits for the one before
+                uint4 w[NB];
 #pragma unroll
-            for (int b = 0; b < NB; b++) mma16816(c[b], aq[b][1], w[b].z, w[b].w);
+                for (int b = 0; b < NB; b++) {
+                    w[b] = src.kop(i, n, b);
+                    mma16816_0(c[b], aq[b][0], w[b].x, w[b].y);
+                }
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const float2 d = unpack(ksc(n, b));
-                const float2 lo = make_float2(c[b][0], c[b][1]), hi = make_float2(c[b][2], c[b][3]);
-                if (MODE == kOne16) {
-                    sc[n][0] = fma2(lo, d, sc[n][0]);
-                    sc[n][H - 1] = fma2(hi, d, sc[n][H - 1]);
-                } else {
-                    sc[n][0] = fma2(MODE == kSplit8 ? add2(lo, hi) : lo, d, sc[n][0]);
+                for (int b = 0; b < NB; b++) mma16816(c[b], aq[b][1], w[b].z, w[b].w);
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float2 d = unpack(src.ksc(i, n, b));
+                    const float2 lo = make_float2(c[b][0], c[b][1]), hi = make_float2(c[b][2], c[b][3]);
+                    if (MODE == kOne16) {
+                        sc[i][n][0] = fma2(lo, d, sc[i][n][0]);
+                        sc[i][n][H - 1] = fma2(hi, d, sc[i][n][H - 1]);
+                    } else {
+                        sc[i][n][0] = fma2(add2(lo, hi), d, sc[i][n][0]);
+                    }
                 }
             }
         }
-        uint2 vs[NB];
+        uint2 vs[NT][NB];
+        uint32_t see[NT][H][2];  // halves of all ones: tokens that the row sees (used where !full)
+        float pr[NT][H][4], top[H];
+        __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
-        for (int b = 0; b < NB; b++) vs[b] = vsc(b);
-        const int j0 = tile_at * kKv4Tile + 4 * t;
-        uint32_t hid01[H], hid23[H];  // halves of all ones: tokens that the row sees
+        for (int h = 0; h < H; h++) top[h] = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < H; h++) hid01[h] = hid23[h] = 0xFFFFFFFFu;
-        if constexpr (!full) {
+        for (int i = 0; i < NT; i++) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int j = j0 + i;
-                const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu;
-                if (j >= seen) {  // nobody's: whatever scale lies there counts for nothing
+            for (int b = 0; b < NB; b++) vs[i][b] = src.vsc(i, b);
+            if constexpr (!full) {
 #pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        if (i < 2) vs[b].x &= ~half;
-                        else vs[b].y &= ~half;
+                for (int h = 0; h < H; h++) see[i][h][0] = see[i][h][1] = 0xFFFFFFFFu;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int j = (tile_at + i) * kKv4Tile + 4 * t + x;
+                    const uint32_t half = (x & 1) ? 0xFFFF0000u : 0x0000FFFFu;
+                    if (j >= seen) {  // nobody's: whatever scale lies there counts for nothing
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            if (x < 2) vs[i][b].x &= ~half;
+                            else vs[i][b].y &= ~half;
+                        }
                     }
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+                        if (j >= seen || j > rpos[h] || (p.window > 0 && rpos[h] - j >= p.window)) see[i][h][x >> 1] &= ~half;
+                }
+            }
+            // the largest V scale of this lane's tokens
+#pragma unroll
+            for (int b = 0; b < NB; b++) big = __hmax2(big, __hmax2(__habs2(as_h2(vs[i][b].x)), __habs2(as_h2(vs[i][b].y))));
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                pr[i][h][0] = sc[i][0][h].x * qs[h];
+                pr[i][h][1] = sc[i][0][h].y * qs[h];
+                pr[i][h][2] = sc[i][1][h].x * qs[h];
+                pr[i][h][3] = sc[i][1][h].y * qs[h];
+                if constexpr (!full) {
+                    if (!(see[i][h][0] & 0xFFFFu)) pr[i][h][0] = -INFINITY;
+                    if (!(see[i][h][0] >> 16)) pr[i][h][1] = -INFINITY;
+                    if (!(see[i][h][1] & 0xFFFFu)) pr[i][h][2] = -INFINITY;
+                    if (!(see[i][h][1] >> 16)) pr[i][h][3] = -INFINITY;
                 }
 #pragma unroll
-                for (int h = 0; h < H; h++)
-                    if (j >= seen || j > rpos[h] || (p.window > 0 && rpos[h] - j >= p.window)) {
-                        if (i < 2) hid01[h] &= ~half;
-                        else hid23[h] &= ~half;
-                    }
+                for (int x = 0; x < 4; x++) top[h] = fmaxf(top[h], pr[i][h][x]);
             }
         }
-        // the largest V scale of this lane's tokens
-        __half2 big = __hmax2(__habs2(as_h2(vs[0].x)), __habs2(as_h2(vs[0].y)));
-#pragma unroll
-        for (int b = 1; b < NB; b++) big = __hmax2(big, __hmax2(__habs2(as_h2(vs[b].x)), __habs2(as_h2(vs[b].y))));
         const float2 big2 = __half22float2(big);
         const float dmax = fmaxf(big2.x, big2.y);
-        float pr[H][4], top[H], mx[H];
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            pr[h][0] = sc[0][h].x * qs[h];
-            pr[h][1] = sc[0][h].y * qs[h];
-            pr[h][2] = sc[1][h].x * qs[h];
-            pr[h][3] = sc[1][h].y * qs[h];
-            if constexpr (!full) {
-                if (!(hid01[h] & 0xFFFFu)) pr[h][0] = -INFINITY;
-                if (!(hid01[h] >> 16)) pr[h][1] = -INFINITY;
-                if (!(hid23[h] & 0xFFFFu)) pr[h][2] = -INFINITY;
-                if (!(hid23[h] >> 16)) pr[h][3] = -INFINITY;
-            }
-            top[h] = fmaxf(fmaxf(pr[h][0], pr[h][1]), fmaxf(pr[h][2], pr[h][3]));
-        }
+        float mx[H];
         float lg = fmaxf(lg2(dmax) - E, -7.0f);
         bool move = dmax > bound;
 #pragma unroll
@@ -401,62 +428,78 @@ struct Warp {
             }
             scale_rows(al);
         }
-        uint32_t ph[H][2], pl[H][2], nh[2];
 #pragma unroll
-        for (int h = 0; h < H; h++) {
-            const float base = m[h] == -INFINITY ? 0.0f : m[h];
-#pragma unroll
-            for (int i = 0; i < 4; i++) pr[h][i] = ex2(pr[h][i] - base);
-            l[h] += (pr[h][0] + pr[h][1]) + (pr[h][2] + pr[h][3]);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                ph[h][i] = pack(pr[h][2 * i], pr[h][2 * i + 1]);
-                if (MODE == kSplit8) {
-                    const float2 back = unpack(ph[h][i]);
-                    pl[h][i] = pack(back.x - pr[h][2 * i], back.y - pr[h][2 * i + 1]);  // -pl
-                    nh[i] = ph[h][i] ^ 0x80008000u;
-                }
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const __half2 d01 = __hmul2(as_h2(vs[b].x), inv), d23 = __hmul2(as_h2(vs[b].y), inv);
-            uint32_t a[4];
+        for (int i = 0; i < NT; i++) {
+            uint32_t ph[H][2], pl[2], nh[2];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                const __half2 x = __hmul2(as_h2(ph[h][0]), d01), y = __hmul2(as_h2(ph[h][1]), d23);
-                if (MODE == kOne16) {
-                    a[h] = as_u32(x);
-                    a[2 + h] = as_u32(y);
-                } else {
-                    a[0] = as_u32(x);
-                    a[2] = as_u32(y);
-                    a[1] = a[3] = 0u;
+                const float base = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll
+                for (int x = 0; x < 4; x++) pr[i][h][x] = ex2(pr[i][h][x] - base);
+                l[h] += (pr[i][h][0] + pr[i][h][1]) + (pr[i][h][2] + pr[i][h][3]);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    ph[h][x] = pack(pr[i][h][2 * x], pr[i][h][2 * x + 1]);
                     if (MODE == kSplit8) {
-                        // minus the low part, which spares the negations: value() subtracts
-                        a[1] = as_u32(__hfma2(as_h2(pl[h][0]), d01, __hfma2(as_h2(nh[0]), d01, x)));
-                        a[3] = as_u32(__hfma2(as_h2(pl[h][1]), d23, __hfma2(as_h2(nh[1]), d23, y)));
-                    }
-                }
-                if constexpr (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
-                    if (MODE == kOne16) {
-                        a[h] &= hid01[h];
-                        a[2 + h] &= hid23[h];
-                    } else {
-                        a[0] &= hid01[h];
-                        a[1] &= hid01[h];
-                        a[2] &= hid23[h];
-                        a[3] &= hid23[h];
+                        const float2 back = unpack(ph[h][x]);
+                        pl[x] = pack(back.x - pr[i][h][2 * x], back.y - pr[i][h][2 * x + 1]);  // -pl
+                        nh[x] = ph[h][x] ^ 0x80008000u;
                     }
                 }
             }
+            src.v(i);
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const uint4 w = vop(b, half);
-                mma16816(oacc[b][2 * half], a, w.x, w.y);
-                mma16816(oacc[b][2 * half + 1], a, w.z, w.w);
+            for (int b = 0; b < NB; b++) {
+                const __half2 d01 = __hmul2(as_h2(vs[i][b].x), inv), d23 = __hmul2(as_h2(vs[i][b].y), inv);
+                uint32_t a[4];
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    const __half2 x = __hmul2(as_h2(ph[h][0]), d01), y = __hmul2(as_h2(ph[h][1]), d23);
+                    if (MODE == kOne16) {
+                        a[h] = as_u32(x);
+                        a[2 + h] = as_u32(y);
+                    } else {
+                        a[0] = as_u32(x);
+                        a[2] = as_u32(y);
+                        // minus the low part, which spares the negations: value() subtracts
+                        a[1] = as_u32(__hfma2(as_h2(pl[0]), d01, __hfma2(as_h2(nh[0]), d01, x)));
+                        a[3] = as_u32(__hfma2(as_h2(pl[1]), d23, __hfma2(as_h2(nh[1]), d23, y)));
+                    }
+                    if constexpr (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
+                        if (MODE == kOne16) {
+                            a[h] &= see[i][h][0];
+                            a[2 + h] &= see[i][h][1];
+                        } else {
+                            a[0] &= see[i][h][0];
+                            a[1] &= see[i][h][0];
+                            a[2] &= see[i][h][1];
+                            a[3] &= see[i][h][1];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const uint4 w = src.vop(i, b, half);
+                    mma16816(oacc[b][2 * half], a, w.x, w.y);
+                    mma16816(oacc[b][2 * half + 1], a, w.z, w.w);
+                }
             }
         }
+    }
+    // Tiles tile_at, + 1, of which bits of `there` are in the cache.
+    template <class Src>
+    __device__ __forceinline__ void pair(const AttnP& p, int tile_at, uint32_t there, int t, Src& src) {
+        if (there == 3u && tile_at >= full0 && tile_at + 1 < full1) {
+            tiles<2, true>(p, tile_at, t, src);
+            return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < 2; i++)
+            if ((there >> i) & 1u) {
+                src.first = i;
+                tiles<1, false>(p, tile_at + i, t, src);
+            }
+        src.first = 0;
     }
 
     // Row sums complete, accumulators back at the values' scale.
@@ -478,64 +521,127 @@ struct Warp {
     }
 };
 
-// The records of one warp's tiles t0 + warp, + kWarps, ...: `Stages` bulk copies in
-// flight, pages looked up 32 tiles at a time.
-template <int Stages, int Bytes>
+// The records of a warp's pairs of tiles: pair k is tiles first + 2 Lists k
+// and the next one, below `end` (Lists: such streams a CTA); `Stages` pairs in
+// flight, one bulk copy a tile, issued by two lanes of the warp that `issues`.
+// Pages are looked up 16 pairs (one tile a lane) at a time.
+template <int Stages, int Bytes, int Lists>
 struct Stream {
-    uint32_t ring, bar;
     const AttnP& p;
-    const Rows& o;
-    int first, n, lane, tiles;
-    int base = -32;
-    int64_t addr = -1;  // of tile base + lane: byte offset of its record, -1: not in the cache
-    uint32_t phase = 0, absent = 0;
+    uint32_t ring, bar;
+    int lane, tiles;
+    bool issues;
+    const int32_t* table;
+    int kvh, first, end, n = 0, base;
+    int64_t addr;   // of this lane's tile: byte offset of its record
+    uint32_t mask;  // lanes whose tile is in the cache
+    uint32_t phase = 0, have = 0;  // bit per stage; two bits per stage: tiles that are there
 
-    __device__ __forceinline__ Stream(const AttnP& p, const Rows& o, uint32_t ring, uint32_t bar, int first, int n, int lane)
-        : ring(ring), bar(bar), p(p), o(o), first(first), n(n), lane(lane), tiles(p.page_size / kKv4Tile) {
-        if (lane == 0) {
+    __device__ __forceinline__ Stream(const AttnP& p, uint32_t ring, uint32_t bar, int lane, bool issues = true)
+        : p(p), ring(ring), bar(bar), lane(lane), tiles(p.page_size / kKv4Tile), issues(issues) {
+        if (lane == 0 && issues) {
             for (int s = 0; s < Stages; s++) mbar_init(bar + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
-        for (int k = 0; k < min(Stages, n); k++) issue(k);
     }
-    __device__ __forceinline__ void issue(int k) {
-        if (k >= base + 32) {
-            base = k & ~31;
+    __device__ __forceinline__ void begin(int b, int kv_head, int first_tile, int end_tile) {
+        table = p.table + b * p.table_stride;
+        kvh = kv_head;
+        first = first_tile;
+        end = end_tile;
+        n = end > first ? (end - first + 2 * Lists - 1) / (2 * Lists) : 0;
+        base = -16;
+        have = 0;
+        for (int k = 0; k < min(Stages, n); k++) issue(k, k);
+    }
+    // pair k into stage s
+    __device__ __forceinline__ void issue(int k, int s) {
+        if (k >= base + 16) {
+            base = k & ~15;
             addr = -1;
-            if (base + lane < n) {
-                const int tile = first + (base + lane) * kWarps, col = tile / tiles;
-                const int pg = p.table[o.b * p.table_stride + col];
-                if (pg >= 0 && pg < p.n_pages)
-                    addr = (((int64_t)pg * p.n_kv + o.kvh) * tiles + (tile - col * tiles)) * Bytes;
+            const int tile = first + 2 * Lists * (base + (lane >> 1)) + (lane & 1);
+            if (tile < end) {
+                const int col = tile / tiles;
+                const int pg = table[col];
+                if (pg >= 0 && pg < p.n_pages) addr = (((int64_t)pg * p.n_kv + kvh) * tiles + (tile - col * tiles)) * Bytes;
             }
+            mask = __ballot_sync(0xffffffffu, addr >= 0);
         }
-        const int s = k % Stages;
-        const int64_t a = __shfl_sync(0xffffffffu, addr, k & 31);
-        absent = (absent & ~(1u << s)) | ((a < 0 ? 1u : 0u) << s);
-        if (a >= 0 && lane == 0) {
-            mbar_expect_tx(bar + 8 * s, Bytes);
-            bulk_g2s(ring + s * Bytes, p.data + a, Bytes, bar + 8 * s, policy_evict_normal());
-        }
+        const uint32_t there = (mask >> (2 * (k - base))) & 3u;
+        have = (have & ~(3u << (2 * s))) | (there << (2 * s));
+        if (!issues || (lane >> 1) != k - base) return;
+        // one lane expects both tiles' bytes, before either copy can arrive:
+        // the other one's is issued behind the group's own barrier
+        const uint32_t two = 3u << (lane & ~1);
+        if (there && (lane & 1) == 0) mbar_expect_tx(bar + 8 * s, __popc(there) * Bytes);
+        __syncwarp(two);
+        if ((there >> (lane & 1)) & 1u)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             ring + (2 * s + (lane & 1)) * Bytes),
+                         "l"(p.data + addr), "r"((uint32_t)Bytes), "r"(bar + 8 * s)
+                         : "memory");
     }
-    __device__ __forceinline__ bool missing(int k) const { return (absent >> (k % Stages)) & 1u; }
-    // false: the copy did not arrive within the bound
-    __device__ __forceinline__ bool wait(int k) {
-        const int s = k % Stages;
+    __device__ __forceinline__ uint32_t there(int s) const { return (have >> (2 * s)) & 3u; }
+    // false: a copy did not arrive within the bound
+    __device__ __forceinline__ bool wait(int s) {
         const bool ok = mbar_wait(bar + 8 * s, (phase >> s) & 1u);
         if (!__all_sync(0xffffffffu, ok)) return false;
         phase ^= 1u << s;
         return true;
     }
-    // after a wait that gave up: the same bound for the copies still in
-    // flight, before their memory goes
+    // after a wait that gave up: the same bound for the copies of pairs k .. k +
+    // Stages - 1, before their memory goes
     __device__ __forceinline__ void abandon(int k) {
         if (lane == 0) {
             atomicExch(p.err, 1);
             for (int i = k; i < min(k + Stages, n); i++)
-                if (!missing(i)) mbar_wait(bar + 8 * (i % Stages), (phase >> (i % Stages)) & 1u);
+                if (there(i % Stages)) mbar_wait(bar + 8 * (i % Stages), (phase >> (i % Stages)) & 1u);
         }
         __syncwarp();
+    }
+};
+
+// Operands built in registers from the records of a pair
+template <int NB>
+struct RecordSrc {
+    const uint8_t* rec;
+    Magic magic;
+    int lane, t, first = 0;
+    uint32_t w[2 * NB];
+    __device__ __forceinline__ const uint8_t* at(int i) const { return rec + (first + i) * Kv4Rec<NB>::kBytes; }
+    __device__ __forceinline__ void k(int i) { load_words<NB>(at(i), lane, w); }
+    __device__ __forceinline__ void v(int i) { load_words<NB>(at(i) + Kv4Rec<NB>::kV, lane, w); }
+    __device__ __forceinline__ uint4 kop(int, int n, int b) const { return k_operands(w[2 * b + n], magic); }
+    __device__ __forceinline__ uint32_t ksc(int i, int n, int b) const {
+        return *reinterpret_cast<const uint32_t*>(at(i) + Kv4Rec<NB>::kKs + t * 8 * NB + 8 * b + 4 * n);
+    }
+    __device__ __forceinline__ uint4 vop(int, int b, int half) const {
+        return v_operands(w[2 * b] >> (8 * half), w[2 * b + 1] >> (8 * half), magic);
+    }
+    __device__ __forceinline__ uint2 vsc(int i, int b) const {
+        return *reinterpret_cast<const uint2*>(at(i) + Kv4Rec<NB>::kVs + t * 8 * NB + 8 * b);
+    }
+};
+// Operands that some warp has put into shared memory
+template <int NB>
+struct SharedSrc {
+    static constexpr int kOps = 2048 * NB;  // K and V operands of a tile, 1024 NB each
+    const uint8_t *ops, *scl;               // [..][kOps], [..][64 NB]: K scales, V scales
+    int lane, t, first = 0;
+    __device__ __forceinline__ void k(int) {}
+    __device__ __forceinline__ void v(int) {}
+    __device__ __forceinline__ uint4 kop(int i, int n, int b) const {
+        return reinterpret_cast<const uint4*>(ops + (first + i) * kOps)[(2 * b + n) * 32 + lane];
+    }
+    __device__ __forceinline__ uint32_t ksc(int i, int n, int b) const {
+        return *reinterpret_cast<const uint32_t*>(scl + (first + i) * 64 * NB + t * 8 * NB + 8 * b + 4 * n);
+    }
+    __device__ __forceinline__ uint4 vop(int i, int b, int half) const {
+        return reinterpret_cast<const uint4*>(ops + (first + i) * kOps)[(2 * NB + 2 * b + half) * 32 + lane];
+    }
+    __device__ __forceinline__ uint2 vsc(int i, int b) const {
+        return *reinterpret_cast<const uint2*>(scl + (first + i) * 64 * NB + 32 * NB + t * 8 * NB + 8 * b);
     }
 };
 
@@ -551,176 +657,351 @@ __device__ __forceinline__ void store2(T* p, bool pair, float a, float b) {
     p[1] = from_f32<T>(b);
 }
 
+// CTAs of an SM: what 168 (head_dim 96, 128) or 128 registers a thread allow
+template <int NB>
+constexpr int kPerSm = NB > 2 ? 3 : 4;
+
+// Few rows.  The work is the line of all units' pairs of tiles (units in the
+// order of sequence, kv head, row tile), each unit headed by kHead empty places
+// for what starting and joining it costs (5 us of a CTA, about 8 pairs); CTA i of
+// n takes places [P i / n, P (i + 1) / n) of it, whatever the sequences' lengths,
+// so one wave of CTAs ends together.  A border inside a head counts as the
+// unit's start.  A unit that lies in one CTA is written out; of one that goes
+// over several, each CTA leaves its sums in `part` (slot 2 i where the piece
+// begins its range, 2 i + 1 where it starts later) and the CTA that starts it
+// says in desc[i] how many there are.
+constexpr int kHead = 8;
+constexpr int kChunk = 128;  // sequences looked up at a time
+
+struct Piece {
+    int b, kvh, r0, t0, t1, slot, whole, more;
+};
+// A CTA's way along the line, in shared memory; warp 0 walks it one piece ahead
+// of the work.
+template <int R>
+struct Line {
+    int64_t total, x0, x1, at, before, end;  // places; `before`: of the chunks so far; `end`: of sequence b
+    int64_t ends[kChunk];                    // of the chunk's sequences
+    int b0, b, tile0, tile1, places, row_tiles, cta, ctas;
+    Piece piece[2];
+
+    // places of a unit of sequence q, and of the sequence (a pair at least:
+    // rows that see nothing are written too)
+    static __device__ __forceinline__ int places_of(const AttnP& p, const Seq& q, int& tile0, int& tile1) {
+        q.tiles(p, 0, q.n_q - 1, tile0, tile1);
+        return max((tile1 - tile0 + 1) / 2, 1) + kHead;
+    }
+    static __device__ __forceinline__ int64_t line_of(const AttnP& p, int b) {
+        if (b >= p.batch) return 0;
+        const Seq q(p, b);
+        int tile0, tile1;
+        const int row_tiles = (q.n_q * p.group + R - 1) / R;
+        return (int64_t)places_of(p, q, tile0, tile1) * p.n_kv * row_tiles;
+    }
+    // warp 0: the next piece
+    __device__ __noinline__ void next(const AttnP& p, Piece& o) {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) o.more = 0;
+        if (at >= x1) return;
+        if (at >= end) {
+            while (at >= before) {  // the chunk that holds the place
+                const int first = b0 + kChunk;
+                if (first >= p.batch) return;
+                int64_t v[kChunk / 32], sum = 0;
+#pragma unroll
+                for (int i = 0; i < kChunk / 32; i++) v[i] = line_of(p, first + lane * (kChunk / 32) + i);
+#pragma unroll
+                for (int i = 0; i < kChunk / 32; i++) sum += v[i];
+                int64_t upto = sum;
+#pragma unroll
+                for (int i = 1; i < 32; i <<= 1) {
+                    const int64_t u = __shfl_up_sync(0xffffffffu, upto, i);
+                    if (lane >= i) upto += u;
+                }
+                int64_t e = before + upto - sum;
+#pragma unroll
+                for (int i = 0; i < kChunk / 32; i++) ends[lane * (kChunk / 32) + i] = e += v[i];
+                const int64_t all = before + __shfl_sync(0xffffffffu, upto, 31);
+                __syncwarp();
+                if (lane == 0) {
+                    b0 = first;
+                    before = all;
+                }
+                __syncwarp();
+            }
+            int lo = 0, hi = kChunk - 1;  // the first sequence whose end lies behind it
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ends[mid] > at) hi = mid;
+                else lo = mid + 1;
+            }
+            const Seq q(p, b0 + lo);
+            int ta, tb;
+            const int n = places_of(p, q, ta, tb);
+            __syncwarp();
+            if (lane == 0) {
+                b = b0 + lo;
+                end = ends[lo];
+                tile0 = ta;
+                tile1 = tb;
+                places = n;
+                row_tiles = (q.n_q * p.group + R - 1) / R;
+            }
+            __syncwarp();
+        }
+        if (lane != 0) return;
+        // counted from the sequence's end, which needs no start
+        const int64_t left = end - at;
+        const int unit = (int)(((int64_t)p.n_kv * row_tiles * places - left) / places);
+        int off = places - (int)((left - 1) % places) - 1;
+        const bool first = at == x0;
+        if (off <= kHead) {  // (only the range's start can lie inside a head)
+            at -= off;
+            off = 0;
+        }
+        const int stop = (int)min((int64_t)places, off + (x1 - at));
+        if (stop <= kHead) {  // the next CTA's
+            at = x1;
+            return;
+        }
+        o.whole = off == 0 && stop == places;
+        o.slot = 2 * cta + (first ? 0 : 1);
+        o.b = b;
+        o.kvh = unit / row_tiles;
+        o.r0 = (unit - o.kvh * row_tiles) * R;
+        o.t0 = tile0 + 2 * max(off - kHead, 0);
+        o.t1 = min(tile0 + 2 * (stop - kHead), tile1);
+        o.more = 1;
+        at += stop - off;
+        if (off == 0 && !o.whole) {
+            // the CTA that holds the unit's last place: the largest i with
+            // total * i / ctas <= it
+            const int64_t behind = at - stop + places;
+            p.desc[cta] = make_int4(b, unit, (int)((behind * ctas + total - 1) / total - cta), o.slot);
+        }
+    }
+};
+
 template <int NB, int MODE, typename T>
-__global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_kernel(const __grid_constant__ AttnP p) {
+__global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
     using W = Warp<NB, MODE, T>;
-    constexpr int R = W::R, H = W::H;
+    constexpr int R = W::R, H = W::H, HD = 32 * NB, kThreads = kWarps * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
-    __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+    __shared__ float s_m[kWarps][R], s_l[kWarps][R], s_f[R][kWarps];
+    __shared__ int64_t s_at[R], s_sum[kWarps];
+    __shared__ Line<R> line;
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = (int)(blockIdx.x % p.splits);
-    Rows o;
-    if (!find_rows<R>(p, blockIdx.x / p.splits, o)) return;
-    const int t0 = o.tile0 + split * o.per, t1 = min(t0 + o.per, o.tile1);
-    if (p.splits > 1 && t0 >= t1) return;  // the join does not read this split
-    const int n_mine = t1 > t0 + warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;
-    const uint8_t* ring = smem + warp * kStages * Rec::kBytes;
-    Stream<kStages, Rec::kBytes> in(p, o, smem_u32(ring), smem_u32(&bars[warp][0]), t0 + warp, n_mine, lane);
-    W w;
-    w.init(p, o, o.r0, g, t);
-    for (int k = 0; k < n_mine; k++) {
-        if (in.missing(k)) {  // not in the cache: nothing to see
-            if (k + kStages < n_mine) in.issue(k + kStages);
-            continue;
-        }
-        if (!in.wait(k)) {
-            in.abandon(k);
-            break;
-        }
-        const uint8_t* rec = ring + (k % kStages) * Rec::kBytes;
-        uint32_t kw[2 * NB], vw[2 * NB];
-        uint2 ks[NB], vs[NB];  // scales of tokens 4 t .. 4 t + 3
-        load_words<NB>(rec, lane, kw);
-        load_words<NB>(rec + Rec::kV, lane, vw);
+    const int cta = (int)blockIdx.x;
+    // the line's length: every thread sums some sequences
+    int64_t total = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) total += Line<R>::line_of(p, b);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            ks[b] = *reinterpret_cast<const uint2*>(rec + Rec::kKs + t * 8 * NB + 8 * b);
-            vs[b] = *reinterpret_cast<const uint2*>(rec + Rec::kVs + t * 8 * NB + 8 * b);
+    for (int i = 16; i > 0; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+    if (lane == 0) s_sum[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int x = 0; x < kWarps; x++) total += s_sum[x];
+    if (threadIdx.x == 0 && p.desc) p.desc[cta] = make_int4(0, 0, 0, 0);
+    // no more CTAs than places, so that none in the middle of a unit is idle
+    const int ctas = (int)min((int64_t)gridDim.x, total);
+    if (cta >= ctas) return;
+    if (warp == 0) {
+        if (lane == 0) {
+            line.total = total;
+            line.at = line.x0 = total * cta / ctas;
+            line.x1 = total * (cta + 1) / ctas;
+            line.before = line.end = 0;
+            line.b0 = -kChunk;
+            line.cta = cta;
+            line.ctas = ctas;
         }
         __syncwarp();
-        if (k + kStages < n_mine) in.issue(k + kStages);
-        w.tile(
-            p, t0 + warp + k * kWarps, t, [&](int n, int b) { return k_operands(kw[2 * b + n]); },
-            [&](int n, int b) { return n ? ks[b].y : ks[b].x; },
-            [&](int b, int half) {
-                const uint32_t w0 = vw[2 * b] >> (8 * half), w1 = vw[2 * b + 1] >> (8 * half);
-                return make_uint4(codes_even(w0), codes_even(w1), codes_odd(w0), codes_odd(w1));
-            },
-            [&](int b) { return vs[b]; });
+        line.next(p, line.piece[0]);
     }
-    w.finish();
-    // ---- join the warps: each one's m, l and row sums through shared memory
-    // (the rings are drained: every issued copy has been waited for)
-    float* so = reinterpret_cast<float*>(smem) + warp * (R * 32 * NB);
+    const uint8_t* ring = smem + warp * kStages * 2 * Rec::kBytes;
+    Stream<kStages, Rec::kBytes, kWarps> in(p, smem_u32(ring), smem_u32(&bars[warp][0]), lane);
+    RecordSrc<NB> src;
+    src.lane = lane;
+    src.t = t;
+    src.magic = p.magic;
+    float* const joint = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * Rec::kBytes);
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < H; h++) {
-        if (t == 0) {
-            s_m[warp][g + 8 * h] = w.m[h];
-            s_l[warp][g + 8 * h] = w.l[h];
+    if (line.piece[0].more) in.begin(line.piece[0].b, line.piece[0].kvh, line.piece[0].t0 + 2 * warp, line.piece[0].t1);
+    bool bad = false;
+    for (int turn = 0; line.piece[turn].more; turn ^= 1) {
+        const Piece& cur = line.piece[turn];
+        if (warp == 0) line.next(p, line.piece[turn ^ 1]);
+        const Rows o(p, cur.b, cur.kvh, cur.r0);
+        W w;
+        w.init(p, o, o.r0, g, t);
+        const int t0 = cur.t0;
+        int s = 0;
+        for (int k = 0; k < in.n; k++) {
+            const uint32_t there = in.there(s);
+            if (there) {  // what is not in the cache is not seen
+                if (!in.wait(s)) {
+                    in.abandon(k);
+                    bad = true;
+                    break;
+                }
+                src.rec = ring + s * 2 * Rec::kBytes;
+                w.pair(p, t0 + 2 * (warp + k * kWarps), there, t, src);
+                __syncwarp();
+            }
+            if (k + kStages < in.n) in.issue(k + kStages, s);
+            s = s + 1 == kStages ? 0 : s + 1;
         }
+        w.finish();
+        // ---- join the warps: each one's m, l and row sums through shared
+        // memory, while the next piece's first copies are under way
+        float* so = joint + warp * (R * HD);
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int h = 0; h < H; h++) {
+            if (t == 0) {
+                s_m[warp][g + 8 * h] = w.m[h];
+                s_l[warp][g + 8 * h] = w.l[h];
+            }
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-                *reinterpret_cast<float2*>(so + (g + 8 * h) * 32 * NB + 32 * b + 8 * n + 2 * t) = w.value(b, n, h);
-    }
-    __syncthreads();
-    const float* all = reinterpret_cast<const float*>(smem);
-    for (int e = threadIdx.x; e < R * 32 * NB; e += kWarps * 32) {
-        const int row = e / (32 * NB), d = e % (32 * NB);
-        const int r = o.r0 + row;
-        if (r >= o.rows) break;
-        const int64_t tok = (int64_t)o.q0 + r / p.group;
-        if (tok < 0 || tok >= p.n_tokens) continue;
-        float M = -INFINITY;
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int i = 0; i < kWarps; i++) M = fmaxf(M, s_m[i][row]);
-        float L = 0.0f, acc = 0.0f;
-        if (M > -INFINITY) {
+                for (int n = 0; n < 4; n++)
+                    *reinterpret_cast<float2*>(so + (g + 8 * h) * HD + 32 * b + 8 * n + 2 * t) = w.value(b, n, h);
+        }
+        if (__syncthreads_or(bad)) return;
+        {
+            const Piece& nxt = line.piece[turn ^ 1];
+            if (nxt.more) in.begin(nxt.b, nxt.kvh, nxt.t0 + 2 * warp, nxt.t1);
+        }
+        if (threadIdx.x < R) {  // a thread a row: the warps' weights, and where the row goes
+            const int row = threadIdx.x, r = o.r0 + row;
+            const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+            const int64_t tok = (int64_t)o.q0 + i;
+            float M = -INFINITY, L = 0.0f, f[kWarps];
 #pragma unroll
-            for (int i = 0; i < kWarps; i++) {
-                const float f = ex2(s_m[i][row] - M);
-                L = fmaf(f, s_l[i][row], L);
-                acc = fmaf(f, all[i * (R * 32 * NB) + e], acc);
+            for (int x = 0; x < kWarps; x++) M = fmaxf(M, s_m[x][row]);
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) {
+                f[x] = M > -INFINITY ? ex2(s_m[x][row] - M) : 0.0f;
+                if (M > -INFINITY) L = fmaf(f[x], s_l[x][row], L);
+            }
+            const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
+            const float scale = cur.whole && M > -INFINITY ? 1.0f / L : 1.0f;
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) s_f[row][x] = f[x] * scale;
+            s_at[row] = !ok ? -1 : cur.whole ? tok * p.ot + head * p.oh : ((int64_t)cur.slot * R + row) * HD;
+            if (ok && !cur.whole) p.ml[cur.slot * R + row] = make_float2(M, L);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = threadIdx.x * 2; e < R * HD; e += kThreads * 2) {
+            const int row = e / HD, d = e % HD;
+            const int64_t to = s_at[row];
+            const float4 f = *reinterpret_cast<const float4*>(s_f[row]);
+            const float ff[kWarps] = {f.x, f.y, f.z, f.w};
+            float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) {
+                const float2 v = *reinterpret_cast<const float2*>(joint + x * (R * HD) + e);
+                acc.x = fmaf(ff[x], v.x, acc.x);
+                acc.y = fmaf(ff[x], v.y, acc.y);
+            }
+            if (to < 0) continue;
+            if (cur.whole) {
+                T* dst = static_cast<T*>(p.out) + to + d;
+                dst[0] = from_f32<T>(acc.x);
+                dst[1] = from_f32<T>(acc.y);
+            } else {
+                *reinterpret_cast<float2*>(p.part + to + d) = acc;
             }
         }
-        const int head = o.kvh * p.group + r % p.group;
-        if (p.splits == 1) {
-            static_cast<T*>(p.out)[tok * p.ot + head * p.oh + d] = from_f32<T>(M > -INFINITY ? acc / L : 0.0f);
-        } else {
-            const int64_t at = (tok * p.n_heads + head) * p.splits + split;
-            p.part[at * (32 * NB) + d] = acc;
-            if (d == 0) p.ml[at] = make_float2(M, L);
-        }
+        __syncthreads();  // the sums (and this piece) have been read
     }
 }
 
-// Many rows: warp i holds rows r0 + i R ..; a step is kWarps tiles, each
-// unpacked by one warp into f16 operands that all four use.
+// Many rows: warp i holds rows r0 + i R ..; a step is kWarps tiles, two to a
+// stream.  Two warps share a stream: one unpacks its K, the other its V into
+// f16 operands that all four use.
 template <int NB, int MODE, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
     using W = Warp<NB, MODE, T>;
-    constexpr int R = W::R, H = W::H;
-    constexpr int kOps = 2048 * NB;  // K and V operands of a tile, 1024 NB each
+    constexpr int R = W::R, H = W::H, HD = 32 * NB, kLists = kWarps / 2;
+    constexpr int kOps = SharedSrc<NB>::kOps;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kWarps][kStagesRows];
-    __shared__ int s_state[kWarps];  // of the step's tiles: 1 there, 0 not in the cache, -1 gave up
+    __shared__ __align__(8) uint64_t bars[kLists][kStagesRows];
+    __shared__ uint32_t s_there[kWarps];  // of the step's pairs; bit 2: a copy did not arrive
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = (int)(blockIdx.x % p.splits);
-    Rows o;
-    if (!find_rows<R * kWarps>(p, blockIdx.x / p.splits, o)) return;
-    const int t0 = o.tile0 + split * o.per, t1 = min(t0 + o.per, o.tile1);
-    if (p.splits > 1 && t0 >= t1) return;
-    const int n_mine = t1 > t0 + warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;
+    const int list = warp >> 1, is_v = warp & 1;
+    const int unit = (int)(blockIdx.x / p.splits), split = (int)blockIdx.x - unit * p.splits;
+    const Rows o = unit_rows<R * kWarps>(p, unit);
+    if (o.r0 >= o.rows) return;
+    int tile0, tile1, per;
+    unit_tiles<R * kWarps>(p, o, tile0, tile1, per);
+    const int t0 = tile0 + split * per, t1 = min(t0 + per, tile1);
+    if (p.splits > 1 && t0 >= t1) return;  // the join does not read this split
+    uint8_t* ops = smem;                  // [kWarps][kOps]
+    uint8_t* scl = smem + kWarps * kOps;  // [kWarps][64 NB]
+    const uint8_t* ring = scl + kWarps * 64 * NB + list * kStagesRows * 2 * Rec::kBytes;
+    Stream<kStagesRows, Rec::kBytes, kLists> in(p, smem_u32(ring), smem_u32(&bars[list][0]), lane, !is_v);
+    in.begin(o.b, o.kvh, t0 + 2 * list, t1);
     const int steps = t1 > t0 ? (t1 - t0 + kWarps - 1) / kWarps : 0;
-    uint8_t* ops = smem;                                 // [kWarps][kOps]
-    uint8_t* scl = smem + kWarps * kOps;                 // [kWarps][64 NB]: K scales, V scales
-    const uint8_t* ring = scl + kWarps * 64 * NB + warp * kStagesRows * Rec::kBytes;
-    Stream<kStagesRows, Rec::kBytes> in(p, o, smem_u32(ring), smem_u32(&bars[warp][0]), t0 + warp, n_mine, lane);
     W w;
     const int r0 = o.r0 + warp * R;
     w.init(p, o, r0, g, t);
     // tiles that this warp's rows see
     const int last = r0 < o.rows ? (max(w.seen, 0) + kKv4Tile - 1) / kKv4Tile : 0;
+    SharedSrc<NB> src;
+    src.lane = lane;
+    src.t = t;
+    __syncthreads();  // the barriers are there
+    int s = 0;
     for (int k = 0; k < steps; k++) {
-        int state = 0;
-        if (k < n_mine && !in.missing(k)) {
-            state = in.wait(k) ? 1 : -1;
-            if (state > 0) {
-                const uint8_t* rec = ring + (k % kStagesRows) * Rec::kBytes;
-                uint32_t kw[2 * NB], vw[2 * NB];
-                load_words<NB>(rec, lane, kw);
-                load_words<NB>(rec + Rec::kV, lane, vw);
-                uint4* dst = reinterpret_cast<uint4*>(ops + warp * kOps) + lane;
+        uint32_t there = k < in.n ? in.there(s) : 0;
+        if (there && !in.wait(s)) there = 4;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (!((there >> i) & 1u)) continue;
+            const uint8_t* rec = ring + (2 * s + i) * Rec::kBytes;
+            uint4* dst = reinterpret_cast<uint4*>(ops + (2 * list + i) * kOps) + lane;
+            uint32_t x[2 * NB];
+            load_words<NB>(rec + is_v * Rec::kV, lane, x);
+            if (is_v) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        dst[(2 * b + n) * 32] = k_operands(kw[2 * b + n]);
-                        const uint32_t w0 = vw[2 * b] >> (8 * n), w1 = vw[2 * b + 1] >> (8 * n);
-                        dst[(2 * NB + 2 * b + n) * 32] =
-                            make_uint4(codes_even(w0), codes_even(w1), codes_odd(w0), codes_odd(w1));
-                    }
-                if (lane < 4 * NB)
-                    reinterpret_cast<uint4*>(scl + warp * 64 * NB)[lane] = reinterpret_cast<const uint4*>(rec + Rec::kKs)[lane];
+                    for (int n = 0; n < 2; n++)
+                        dst[(2 * NB + 2 * b + n) * 32] = v_operands(x[2 * b] >> (8 * n), x[2 * b + 1] >> (8 * n), p.magic);
+            } else {
+#pragma unroll
+                for (int b = 0; b < 2 * NB; b++) dst[b * 32] = k_operands(x[b], p.magic);
             }
+            if (lane < 2 * NB)  // its scales
+                reinterpret_cast<uint4*>(scl + (2 * list + i) * 64 * NB)[is_v * 2 * NB + lane] =
+                    reinterpret_cast<const uint4*>(rec + Rec::kKs)[is_v * 2 * NB + lane];
         }
-        if (lane == 0) s_state[warp] = state;
+        if (lane == 0) s_there[warp] = there;
         __syncthreads();
-        if (k + kStagesRows < n_mine && state >= 0) in.issue(k + kStagesRows);
+        if (k + kStagesRows < in.n && there < 4) in.issue(k + kStagesRows, s);
+        s = s + 1 == kStagesRows ? 0 : s + 1;
         bool stop = false;
 #pragma unroll 1
-        for (int i = 0; i < kWarps; i++) {
-            const int st = s_state[i], tile = t0 + k * kWarps + i;
-            stop |= st < 0;
-            if (st <= 0 || tile >= last) continue;
-            const uint4* src = reinterpret_cast<const uint4*>(ops + i * kOps) + lane;
-            const uint8_t* sc = scl + i * 64 * NB + t * 8 * NB;
-            w.tile(
-                p, tile, t, [&](int n, int b) { return src[(2 * b + n) * 32]; },
-                [&](int n, int b) { return *reinterpret_cast<const uint32_t*>(sc + 8 * b + 4 * n); },
-                [&](int b, int half) { return src[(2 * NB + 2 * b + half) * 32]; },
-                [&](int b) { return *reinterpret_cast<const uint2*>(sc + 32 * NB + 8 * b); });
+        for (int i = 0; i < kLists; i++) {
+            const int tile = t0 + 2 * (k * kLists + i);
+            uint32_t at = s_there[2 * i];
+            stop |= at >= 4 || s_there[2 * i + 1] >= 4;
+            if (tile + 1 >= last) at &= tile < last ? 1u : 0u;
+            src.ops = ops + 2 * i * kOps;
+            src.scl = scl + 2 * i * 64 * NB;
+            w.pair(p, tile, at & 3u, t, src);
         }
         __syncthreads();
         if (stop) {
-            in.abandon(k + (state >= 0 ? 1 : 0));
+            in.abandon(k + (there < 4 ? 1 : 0));
             break;
         }
     }
@@ -728,19 +1009,20 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __g
 #pragma unroll
     for (int h = 0; h < H; h++) {
         const int r = r0 + g + 8 * h;
-        const int64_t tok = (int64_t)o.q0 + r / p.group;
+        const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+        const int64_t tok = (int64_t)o.q0 + i;
         if (r >= o.rows || tok < 0 || tok >= p.n_tokens) continue;
-        const int head = o.kvh * p.group + r % p.group;
         if (p.splits == 1) {
             T* dst = static_cast<T*>(p.out) + tok * p.ot + head * p.oh + 2 * t;
-            const bool pair = ((uintptr_t)dst & 7) == 0;
-            const float f = w.m[h] > -INFINITY ? 1.0f / w.l[h] : 0.0f;
+            const bool two = ((uintptr_t)dst & 7) == 0;
+            const bool any = w.m[h] > -INFINITY;
+            const float f = any ? 1.0f / w.l[h] : 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
                     const float2 v = w.value(b, n, h);
-                    store2(dst + 32 * b + 8 * n, pair, w.m[h] > -INFINITY ? v.x * f : 0.0f, w.m[h] > -INFINITY ? v.y * f : 0.0f);
+                    store2(dst + 32 * b + 8 * n, two, any ? v.x * f : 0.0f, any ? v.y * f : 0.0f);
                 }
         } else {
             const int64_t at = (tok * p.n_heads + head) * p.splits + split;
@@ -748,32 +1030,24 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __g
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int n = 0; n < 4; n++)
-                    *reinterpret_cast<float2*>(p.part + at * (32 * NB) + 32 * b + 8 * n + 2 * t) = w.value(b, n, h);
+                    *reinterpret_cast<float2*>(p.part + at * HD + 32 * b + 8 * n + 2 * t) = w.value(b, n, h);
             if (t == 0) p.ml[at] = make_float2(w.m[h], w.l[h]);
         }
     }
 }
 
-// Joins the splits of a row, a CTA a row: groups of 8 NB threads (four
-// elements each) take every kJoin / (8 NB)-th split, and add up in group order.
+// Joins the pieces of a row, a CTA a row: groups of 8 NB threads (four elements
+// each) take every kJoin / (8 NB)-th piece, and add up in group order.  slot(s):
+// where piece s lies.
 constexpr int kJoin = 256;
-template <int NB, int R, typename T>
-__global__ void __launch_bounds__(kJoin) kv4_join_kernel(const __grid_constant__ AttnP p) {
-    pdl_wait();
-    Rows o;
-    if (!find_rows<R>(p, blockIdx.x / R, o)) return;
-    const int r = o.r0 + (int)(blockIdx.x % R);
-    if (r >= o.rows) return;
-    const int64_t tok = (int64_t)o.q0 + r / p.group;
-    if (tok < 0 || tok >= p.n_tokens) return;
+template <int NB, typename T, class Slot>
+__device__ __forceinline__ void join_row(const AttnP& p, int64_t dst, int used, Slot slot) {
     constexpr int per = 8 * NB, groups = kJoin / per;
     __shared__ float4 s_o[groups][per];
     __shared__ float s_l[groups], s_m[kJoin / 32];
-    const int head = o.kvh * p.group + r % p.group, tid = threadIdx.x;
-    const int used = (o.tile1 - o.tile0 + o.per - 1) / o.per;  // splits that had tiles
-    const int64_t at = (tok * p.n_heads + head) * p.splits;
+    const int tid = threadIdx.x;
     float M = -INFINITY;
-    for (int s = tid; s < used; s += kJoin) M = fmaxf(M, p.ml[at + s].x);
+    for (int s = tid; s < used; s += kJoin) M = fmaxf(M, p.ml[slot(s)].x);
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
     if ((tid & 31) == 0) s_m[tid >> 5] = M;
@@ -787,8 +1061,9 @@ __global__ void __launch_bounds__(kJoin) kv4_join_kernel(const __grid_constant__
         if (M > -INFINITY) {
 #pragma unroll 4
             for (int s = grp; s < used; s += groups) {
-                const float2 v = p.ml[at + s];
-                const float4 x = reinterpret_cast<const float4*>(p.part + (at + s) * (32 * NB))[e];
+                const int64_t at = slot(s);
+                const float2 v = p.ml[at];
+                const float4 x = reinterpret_cast<const float4*>(p.part + at * (32 * NB))[e];
                 const float f = ex2(v.x - M);
                 L = fmaf(f, v.y, L);
                 acc.x = fmaf(f, x.x, acc.x);
@@ -808,45 +1083,78 @@ __global__ void __launch_bounds__(kJoin) kv4_join_kernel(const __grid_constant__
             l += s_l[i];
             sum += reinterpret_cast<const float*>(s_o[i])[tid];
         }
-        static_cast<T*>(p.out)[tok * p.ot + head * p.oh + tid] = from_f32<T>(M > -INFINITY ? sum / l : 0.0f);
+        static_cast<T*>(p.out)[dst + tid] = from_f32<T>(M > -INFINITY ? sum / l : 0.0f);
     }
+}
+// Few rows: CTA i R + row joins row `row` of the unit that starts in CTA i.
+template <int NB, int R, typename T>
+__global__ void __launch_bounds__(kJoin) kv4_join_kernel(const __grid_constant__ AttnP p) {
+    pdl_wait();
+    const int i = (int)(blockIdx.x / R), row = (int)blockIdx.x - i * R;
+    const int4 d = p.desc[i];
+    if (d.z < 2) return;
+    const Seq q(p, d.x);
+    const int row_tiles = (q.n_q * p.group + R - 1) / R, kvh = d.y / row_tiles;
+    const int r = (d.y - kvh * row_tiles) * R + row;
+    const int64_t tok = (int64_t)q.q0 + r / p.group;
+    if (r >= q.n_q * p.group || tok < 0 || tok >= p.n_tokens) return;
+    join_row<NB, T>(p, tok * p.ot + (kvh * p.group + r % p.group) * p.oh, d.z,
+                    [&](int s) { return (int64_t)(s ? 2 * (i + s) : d.w) * R + row; });
+}
+// Many rows: the splits of every row.
+template <int NB, int R, typename T>
+__global__ void __launch_bounds__(kJoin) kv4_join_rows_kernel(const __grid_constant__ AttnP p) {
+    pdl_wait();
+    const Rows o = unit_rows<R>(p, (int)(blockIdx.x / R));
+    const int r = o.r0 + (int)(blockIdx.x % R);
+    if (r >= o.rows) return;
+    const int64_t tok = (int64_t)o.q0 + r / p.group;
+    if (tok < 0 || tok >= p.n_tokens) return;
+    int tile0, tile1, per;
+    unit_tiles<R>(p, o, tile0, tile1, per);
+    const int head = o.kvh * p.group + r % p.group;
+    const int64_t at = (tok * p.n_heads + head) * p.splits;
+    join_row<NB, T>(p, tok * p.ot + head * p.oh, (tile1 - tile0 + per - 1) / per, [&](int s) { return at + s; });
 }
 
-// f32 queries take the hi + lo rows, 16-bit ones one operand row each (eight
-// or sixteen rows a tile)
-enum Which { kMain, kRows, kJoinSplits };
+struct Fns {
+    const void *main, *join;
+};
 template <int NB, int MODE, typename T>
-const void* fn_of(Which which, bool rows) {
+Fns fns_of(bool rows) {
     constexpr int R = MODE == kOne16 ? 16 : 8;
-    if (which == kMain) return (const void*)kv4_attn_kernel<NB, MODE, T>;
-    if constexpr (MODE == kOne8) return (const void*)kv4_join_kernel<NB, R, T>;  // 8 rows have no rows form
-    else if (which == kRows) return (const void*)kv4_attn_rows_kernel<NB, MODE, T>;
-    else return rows ? (const void*)kv4_join_kernel<NB, R * kWarps, T> : (const void*)kv4_join_kernel<NB, R, T>;
+    if constexpr (sizeof(T) == 4 || MODE == kOne16)  // 16-bit queries have no form of many rows in tiles of eight
+        if (rows)
+            return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, R * kWarps, T>};
+    return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
 }
 template <int NB, typename T>
-const void* fn_of(Which which, int mode, bool rows) {
-    if constexpr (sizeof(T) == 4) return fn_of<NB, kSplit8, T>(which, rows);
-    else return mode == kOne8 ? fn_of<NB, kOne8, T>(which, rows) : fn_of<NB, kOne16, T>(which, rows);
+Fns fns_of(int mode, bool rows) {
+    if constexpr (sizeof(T) == 2)
+        if (mode == kOne16) return fns_of<NB, kOne16, T>(rows);
+    return fns_of<NB, kSplit8, T>(rows);
 }
 template <typename T>
-const void* fn_of(int nb, Which which, int mode, bool rows) {
+Fns fns_of(int nb, int mode, bool rows) {
     switch (nb) {
-    case 1: return fn_of<1, T>(which, mode, rows);
-    case 2: return fn_of<2, T>(which, mode, rows);
-    case 3: return fn_of<3, T>(which, mode, rows);
-    default: return fn_of<4, T>(which, mode, rows);
+    case 1: return fns_of<1, T>(mode, rows);
+    case 2: return fns_of<2, T>(mode, rows);
+    case 3: return fns_of<3, T>(mode, rows);
+    default: return fns_of<4, T>(mode, rows);
     }
 }
-const void* fn_of(int dtype, int nb, Which which, int mode, bool rows) {
-    return dtype == RQ_F32 ? fn_of<float>(nb, which, mode, rows)
-           : dtype == RQ_F16 ? fn_of<__half>(nb, which, mode, rows)
-                             : fn_of<__nv_bfloat16>(nb, which, mode, rows);
+Fns fns_of(int dtype, int nb, int mode, bool rows) {
+    return dtype == RQ_F32 ? fns_of<float>(nb, mode, rows)
+           : dtype == RQ_F16 ? fns_of<__half>(nb, mode, rows)
+                             : fns_of<__nv_bfloat16>(nb, mode, rows);
 }
 
 struct Plan {
-    int mode, R, row_tiles, splits;  // R: rows of a CTA
-    bool rows;                       // the many-rows form
-    int64_t units;
+    int mode, R;       // R: rows of a CTA
+    bool rows;         // the many-rows form
+    int64_t ctas;      // of the main launch
+    int row_tiles, splits;  // many rows
+    int64_t pieces;    // row sums kept for the join: 0, no join
 };
 
 int check_query(const rq_kv4* c, const rq_kv4_query* a, const char* fn) {
@@ -875,42 +1183,51 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
     Plan pl{};
     const int64_t group = a->n_heads / c->n_kv;
     const int64_t rows = group * (a->cu_q ? a->max_q : 1);
-    pl.mode = a->dtype == RQ_F32 ? kSplit8 : rows <= 8 ? kOne8 : kOne16;
+    // f32 queries need the two parts; up to eight 16-bit rows take them too,
+    // since the other half of the operand would be empty
+    pl.mode = a->dtype == RQ_F32 || rows <= 8 ? kSplit8 : kOne16;
     pl.R = pl.mode == kOne16 ? 16 : 8;
     pl.rows = rows > 2 * pl.R;
-    if (pl.rows) pl.R *= kWarps;
-    pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
-    pl.units = a->batch * c->n_kv * pl.row_tiles;
-    // Splits of the long axis: one CTA for each place on the device (three an
-    // SM) where the rows are few, four where the sequences' different lengths
-    // have to even out, but none shorter than two tiles a warp
+    const int64_t tiles_of_row = (rows + pl.R - 1) / pl.R;
     int64_t len = a->table_width * c->page_size;
     if (a->max_len > 0) len = std::min(len, a->max_len);
     if (a->window > 0) len = std::min(len, a->window + a->max_q);
-    const int64_t tiles = (len + kKv4Tile - 1) / kKv4Tile;
-    const int64_t places = (int64_t)c->ctx->sm_count * 3;
-    const int64_t want = a->batch == 1 ? places / std::max<int64_t>(pl.units, 1)
-                                       : (4 * places + pl.units - 1) / std::max<int64_t>(pl.units, 1);
+    const int64_t tiles = (len + kKv4Tile - 1) / kKv4Tile, sms = c->ctx->sm_count;
+    if (!pl.rows) {
+        // one wave, but no CTA shorter than a pair a warp at the longest lengths
+        const int64_t pairs = a->batch * c->n_kv * tiles_of_row * (std::max<int64_t>((tiles + 1) / 2, 1) + kHead);
+        const int64_t places = sms * (c->head_dim > 64 ? kPerSm<4> : kPerSm<2>);
+        pl.ctas = std::max<int64_t>(1, std::min(places, pairs / (kWarps + 1)));
+        pl.pieces = pl.ctas > 1 ? 2 * pl.ctas * pl.R : 0;
+        return pl;
+    }
+    pl.R *= kWarps;
+    pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
+    const int64_t units = a->batch * c->n_kv * pl.row_tiles;
+    // splits of the long axis where the units leave the device's places (three
+    // CTAs an SM) empty, none shorter than two steps
+    const int64_t want = sms * 3 / std::max<int64_t>(units, 1);
     pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / (2 * kWarps)));
+    pl.ctas = units * pl.splits;
+    pl.pieces = pl.splits > 1 ? a->n_tokens * a->n_heads * pl.splits : 0;
     return pl;
 }
 
-size_t plan_bytes(const rq_kv4* c, const rq_kv4_query* a, const Plan& pl) {
-    if (pl.splits == 1) return 0;
-    return (size_t)a->n_tokens * a->n_heads * pl.splits * ((size_t)c->head_dim * 4 + 8);
+size_t plan_bytes(const rq_kv4* c, const Plan& pl) {
+    return (size_t)pl.pieces * ((size_t)c->head_dim * 4 + 8) + (pl.pieces && !pl.rows ? (size_t)pl.ctas * 16 : 0);
 }
 
 }  // namespace
 
 int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t st) {
     const Plan pl = make_plan(c, a);
-    const size_t need = plan_bytes(c, a, pl);
+    const size_t need = plan_bytes(c, pl);
     if (need) {
         if (a->workspace_bytes < need)
             return set_error(RQ_ERR_INVALID, "rq_kv4_attention: workspace of %zu bytes, need %zu", a->workspace_bytes, need);
         if (!a->workspace || (uintptr_t)a->workspace & 15) return set_error(RQ_ERR_INVALID, "rq_kv4_attention: workspace is NULL or not 16-byte aligned");
     }
-    if (pl.units * pl.splits > INT32_MAX || pl.units * pl.R > INT32_MAX)
+    if (pl.ctas * (pl.rows ? 1 : pl.R) > INT32_MAX || (pl.rows && a->batch * c->n_kv * pl.row_tiles * pl.R > INT32_MAX))
         return set_error(RQ_ERR_INVALID, "rq_kv4_attention: too many rows for one call");
     const size_t size = a->dtype == RQ_F32 ? 4 : 2;
     AttnP p{};
@@ -943,24 +1260,26 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.scale = a->scale * 1.44269504088896340736f;
     p.part = static_cast<float*>(a->workspace);
     if (need) {
-        const int64_t rows = a->n_tokens * a->n_heads * pl.splits;
-        p.ml = reinterpret_cast<float2*>(p.part + rows * c->head_dim);
+        // sums, then the pairs (descriptions first: they want 16 bytes)
+        p.desc = pl.rows ? nullptr : reinterpret_cast<int4*>(p.part + pl.pieces * c->head_dim);
+        p.ml = pl.rows ? reinterpret_cast<float2*>(p.part + pl.pieces * c->head_dim) : reinterpret_cast<float2*>(p.desc + pl.ctas);
     }
+    p.magic = Magic{kEven, kOdd};
     p.err = err;
     const int nb = c->head_dim / 32;
     const size_t smem = pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb)
-                                : (size_t)kWarps * std::max(kStages * 576 * nb, pl.R * 32 * nb * 4);
-    const void* fn = fn_of(a->dtype, nb, pl.rows ? kRows : kMain, pl.mode, pl.rows);
+                                : (size_t)kWarps * (kStages * 2 * 576 * nb + pl.R * 32 * nb * 4);
+    const Fns fn = fns_of(a->dtype, nb, pl.mode, pl.rows);
     if (smem > 48 * 1024) {
-        const int rc = cuda_error(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+        const int rc = cuda_error(cudaFuncSetAttribute(fn.main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                                   "kv4 attention kernel");
         if (rc) return rc;
     }
     void* args[] = {&p};
-    const int rc = launch_pdl(fn, (unsigned)(pl.units * pl.splits), kWarps * 32, smem, st, args, "kv4 attention kernel");
-    if (rc || pl.splits == 1) return rc;
-    const void* jf = fn_of(a->dtype, nb, kJoinSplits, pl.mode, pl.rows);
-    return launch_pdl(jf, (unsigned)(pl.units * pl.R), kJoin, 0, st, args, "kv4 join kernel");
+    const int rc = launch_pdl(fn.main, (unsigned)pl.ctas, kWarps * 32, smem, st, args, "kv4 attention kernel");
+    if (rc || !pl.pieces) return rc;
+    const int64_t joins = pl.rows ? a->batch * c->n_kv * pl.row_tiles * pl.R : pl.ctas * pl.R;
+    return launch_pdl(fn.join, (unsigned)joins, kJoin, 0, st, args, "kv4 join kernel");
 }
 
 
@@ -974,7 +1293,7 @@ int rq_kv4_attention_workspace(const rq_kv4* c, const rq_kv4_query* a, size_t* b
     if (!bytes) return set_error(RQ_ERR_INVALID, "rq_kv4_attention_workspace: NULL argument");
     int rc = check_query(c, a, "rq_kv4_attention_workspace");
     if (rc) return rc;
-    *bytes = plan_bytes(c, a, make_plan(c, a));
+    *bytes = plan_bytes(c, make_plan(c, a));
     return RQ_OK;
 }
 
