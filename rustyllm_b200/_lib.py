@@ -20,12 +20,7 @@ BLOCK_BYTES = {Q4_0: 18, Q8_0: 34, Q2_K: 84, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6
 BLOCK_ELEMS = {Q4_0: 32, Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 
 
-RQ_F32, RQ_F16, RQ_BF16 = 0, 1, 2
-try:  # torch element types of the paged serving operators
-    import torch
-    DTYPES = {torch.float32: RQ_F32, torch.float16: RQ_F16, torch.bfloat16: RQ_BF16}
-except Exception:  # pragma: no cover
-    DTYPES = {}
+RQ_F32, RQ_F16, RQ_BF16 = 0, 1, 2  # rq_dtype
 
 
 class RqError(RuntimeError):

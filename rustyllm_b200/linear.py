@@ -49,6 +49,13 @@ class Context:
             ctx = cls._per_device[device] = Context(device)
         return ctx
 
+    @classmethod
+    def of(cls, t) -> int:
+        """The handle (an address) of the context of a CUDA tensor's device."""
+        if torch is None or not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RqError(1, "a CUDA tensor is wanted")
+        return cls.get(t.device.index).handle.value
+
     def close(self) -> None:
         if self.handle:
             _lib.lib().rq_destroy(self.handle)

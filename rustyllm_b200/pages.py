@@ -8,19 +8,11 @@ from collections import namedtuple
 
 import torch
 
-from . import _lib
-from ._lib import check
-from .kv4 import int32, refuse, stream_of
 from .linear import Context
 
+from . import _rqtorch  # isort: skip  (needs torch's libraries loaded)
+
 Extended = namedtuple("Extended", "free kv_lens cu_new positions slots")
-
-
-def _table(table, batch: int):
-    if not (isinstance(table, torch.Tensor) and table.is_cuda and table.dtype is torch.int32 and table.dim() == 2
-            and table.shape[0] == batch and (table.shape[1] < 2 or table.stride(1) == 1)):
-        refuse(f"table: a CUDA int32 [{batch}, width] with contiguous rows is wanted")
-    return table.device
 
 
 def pages_extend(ctx_lens, new_lens, table, ring, free, page_size: int, n_tokens: int, free_out=None, kv_lens_out=None):
@@ -31,44 +23,14 @@ def pages_extend(ctx_lens, new_lens, table, ring, free, page_size: int, n_tokens
     new lengths (``kv_lens_out``, which may be ctx_lens), the offsets of the
     new tokens [batch + 1], and position and slot of each of n_tokens rows (-1
     for padding and for tokens that no page is left for)."""
-    batch = new_lens.shape[0]
-    dev = _table(table, batch)
-    int32(ctx_lens, "ctx_lens", dev, batch)
-    int32(new_lens, "new_lens", dev, batch)
-    int32(ring, "ring", dev)
-    int32(free, "free", dev, 3)
-    # one allocation: state, lengths, offsets, positions, slots
-    buf = torch.empty(4 + 2 * batch + 2 * n_tokens, dtype=torch.int32, device=dev)
-    state, kv, cu, pos, slots = buf.split_with_sizes((3, batch, batch + 1, n_tokens, n_tokens))
-    if free_out is None:
-        free_out = state
-    else:
-        int32(free_out, "free_out", dev, 3)
-    if kv_lens_out is None:
-        kv_lens_out = kv
-    else:
-        int32(kv_lens_out, "kv_lens_out", dev, batch)
-    base = buf.data_ptr() + 4 * (3 + batch)
-    at = base + 4 * (batch + 1)
-    check(_lib.lib().rq_pages_extend(
-        Context.get(dev.index).handle, batch, page_size, ctx_lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(),
-        table.stride(0), table.shape[1], ring.data_ptr(), ring.shape[0], free.data_ptr(), free_out.data_ptr(),
-        kv_lens_out.data_ptr(), base, at, at + 4 * n_tokens, n_tokens, stream_of(dev)))
-    return Extended(free_out, kv_lens_out, cu, pos, slots)
+    return Extended(*_rqtorch.pages_extend(Context.of(new_lens), ctx_lens, new_lens, table, ring, free, page_size, n_tokens,
+                                           free_out, kv_lens_out))
 
 
 def pages_release(held_lens, keep_lens, table, ring, free, page_size: int) -> None:
     """Gives the pages behind the first keep_lens [batch] of held_lens [batch]
     positions back to the ring; table, ring and free change in place."""
-    batch = held_lens.shape[0]
-    dev = _table(table, batch)
-    int32(held_lens, "held_lens", dev, batch)
-    int32(keep_lens, "keep_lens", dev, batch)
-    int32(ring, "ring", dev)
-    int32(free, "free", dev, 3)
-    check(_lib.lib().rq_pages_release(
-        Context.get(dev.index).handle, batch, page_size, held_lens.data_ptr(), keep_lens.data_ptr(), table.data_ptr(),
-        table.stride(0), table.shape[1], ring.data_ptr(), ring.shape[0], free.data_ptr(), stream_of(dev)))
+    _rqtorch.pages_release(Context.of(held_lens), held_lens, keep_lens, table, ring, free, page_size)
 
 
 class PageTable:

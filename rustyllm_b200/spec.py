@@ -16,10 +16,9 @@ from collections import deque
 
 import torch
 
-from . import _lib
-from ._lib import check
-from .kv4 import _PAIR, dtype_of, int32, refuse, stream_of
 from .linear import Context
+
+from . import _rqtorch  # isort: skip  (needs torch's libraries loaded)
 
 
 def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
@@ -30,30 +29,7 @@ def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
     (float32); rq_spec_verify of include/rq.h.  n_drafts [batch] (int32)
     limits a row's drafts.  A row of tokens is the accepted drafts, one drawn
     token and -1s; with n = 0 the call samples from p."""
-    if not (isinstance(p, torch.Tensor) and p.is_cuda and p.dim() == 3 and p.stride(2) == 1 and p.shape[1] > 0):
-        refuse("p: a CUDA tensor [batch, n + 1, vocab] with contiguous rows is wanted")
-    b, n, vocab = p.shape[0], p.shape[1] - 1, p.shape[2]
-    dev = p.device
-    if not (q is None or (q.shape == (b, n, vocab) and q.dtype == p.dtype and q.device == dev
-                          and (n == 0 or q.stride(2) == 1))):
-        refuse(f"q: [{b}, {n}, {vocab}] {p.dtype} with contiguous rows on {dev} is wanted")
-    int32(drafts, "drafts", dev)
-    if drafts.shape != (b, n):
-        refuse(f"drafts: [{b}, {n}] is wanted")
-    if not (u.dtype is torch.float32 and u.shape == (b, n) and u.device == dev and u.is_contiguous()):
-        refuse(f"u: a contiguous float32 [{b}, {n}] on {dev} is wanted")
-    if not (r.dtype is torch.float32 and r.shape == (b,) and r.device == dev and r.is_contiguous()):
-        refuse(f"r: a contiguous float32 [{b}] on {dev} is wanted")
-    if n_drafts is not None:
-        int32(n_drafts, "n_drafts", dev, b)
-    tokens = torch.empty((b, n + 1), dtype=torch.int32, device=dev)
-    accepted = torch.empty(b, dtype=torch.int32, device=dev)
-    check(_lib.lib().rq_spec_verify(
-        Context.get(dev.index).handle, dtype_of(p, "p"), p.data_ptr(), _PAIR(p.stride(0), p.stride(1)),
-        None if q is None else q.data_ptr(), None if q is None else _PAIR(q.stride(0), q.stride(1)), drafts.data_ptr(),
-        None if n_drafts is None else n_drafts.data_ptr(), u.data_ptr(), r.data_ptr(), b, n, vocab, tokens.data_ptr(),
-        accepted.data_ptr(), stream_of(dev)))
-    return tokens, accepted
+    return _rqtorch.spec_verify(Context.of(p), p, drafts, u, r, q, n_drafts)
 
 
 class SpecDecoder:
