@@ -53,8 +53,9 @@ bool wide_ok(const void* p, int64_t s0, int64_t s1, size_t size) {
 
 // ------------------------------------------------------------------ append
 //
-// One thread per 8 elements, the aligned four lanes holding a block of 32.
-// Bound by memory: 16 (or 32) bytes in, 4.5 out, per thread.
+// One thread per 8 elements, the aligned four lanes holding a block of 32; a
+// CTA takes `per_cta` tokens (about two items a thread), so that indexes are
+// 32-bit inside it.  Bound by memory: 16 (or 32) bytes in, 4.5 out, per item.
 struct AppendP {
     const void* x[2];          // k, v
     int64_t tok[2], head[2];   // strides in elements
@@ -62,26 +63,38 @@ struct AppendP {
     const int32_t* slots;
     int64_t n, n_slots;
     uint8_t* data;
-    int page_size, n_kv, nb;
+    int page_size, n_kv, nb, per_cta;
+};
+
+// Item i of a CTA's tokens: row (K's heads, then V's, of a token) and 8 elements
+struct Item {
+    int64_t n;
+    int head, e;
+    bool is_v;
+    __device__ __forceinline__ Item(unsigned i, int64_t first, int n_kv, int nb) {
+        const unsigned per = 4 * nb, row = i / per;
+        const unsigned tok = row / (2u * n_kv), r = row - tok * 2u * n_kv;
+        e = (int)(i - row * per);
+        is_v = r >= (unsigned)n_kv;
+        head = (int)(is_v ? r - n_kv : r);
+        n = first + tok;
+    }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendP p) {
     pdl_wait();
-    const int per = 4 * p.nb;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t row = i / per;
-    if (row >= p.n * 2 * p.n_kv) return;
-    const int e = (int)(i - row * per);
-    const int64_t n = row / (2 * p.n_kv);
-    const int r = (int)(row - n * 2 * p.n_kv);
-    const bool is_v = r >= p.n_kv;
-    const int head = is_v ? r - p.n_kv : r;
-    const int32_t slot = p.slots[n];
-    float x[8];
-    load8(static_cast<const T*>(p.x[is_v]) + n * p.tok[is_v] + head * p.head[is_v] + 8 * e, p.wide[is_v], x);
-    uint8_t* rec = kv4_record(p.data, p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, head);
-    kv4_store(rec, p.nb, slot & 15, e >> 2, is_v, x);
+    const int64_t first = (int64_t)blockIdx.x * p.per_cta;
+    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * p.nb);
+    for (unsigned i = threadIdx.x; i < items; i += 256) {
+        const Item it(i, first, p.n_kv, p.nb);
+        const int32_t slot = p.slots[it.n];
+        float x[8];
+        load8(static_cast<const T*>(p.x[it.is_v]) + it.n * p.tok[it.is_v] + it.head * p.head[it.is_v] + 8 * it.e,
+              p.wide[it.is_v], x);
+        uint8_t* rec = kv4_record(p.data, p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, it.head);
+        kv4_store(rec, p.nb, slot & 15, it.e >> 2, it.is_v, x);
+    }
 }
 
 // k and v rows of the given slots, dequantized; zeros for a slot outside the
@@ -90,7 +103,7 @@ struct ReadP {
     const uint8_t* data;
     const int32_t* slots;
     int64_t n, n_slots;
-    int page_size, n_kv, nb;
+    int page_size, n_kv, nb, per_cta;
     void* x[2];  // [n][n_kv][head_dim]
     bool wide;
 };
@@ -98,21 +111,17 @@ struct ReadP {
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ ReadP p) {
     pdl_wait();
-    const int per = 4 * p.nb;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t row = i / per;
-    if (row >= p.n * 2 * p.n_kv) return;
-    const int e = (int)(i - row * per);
-    const int64_t n = row / (2 * p.n_kv);
-    const int r = (int)(row - n * 2 * p.n_kv);
-    const bool is_v = r >= p.n_kv;
-    const int head = is_v ? r - p.n_kv : r;
-    const int32_t slot = p.slots[n];
-    const uint8_t* rec =
-        kv4_record(const_cast<uint8_t*>(p.data), p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, head);
-    float x[8];
-    kv4_load(rec, p.nb, slot & 15, e >> 2, is_v, x);
-    store8(static_cast<T*>(p.x[is_v]) + (n * p.n_kv + head) * (32 * p.nb) + 8 * e, p.wide, x);
+    const int64_t first = (int64_t)blockIdx.x * p.per_cta;
+    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * p.nb);
+    for (unsigned i = threadIdx.x; i < items; i += 256) {
+        const Item it(i, first, p.n_kv, p.nb);
+        const int32_t slot = p.slots[it.n];
+        const uint8_t* rec =
+            kv4_record(const_cast<uint8_t*>(p.data), p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, it.head);
+        float x[8];
+        kv4_load(rec, p.nb, slot & 15, it.e >> 2, it.is_v, x);
+        store8(static_cast<T*>(p.x[it.is_v]) + (it.n * p.n_kv + it.head) * (32 * p.nb) + 8 * it.e, p.wide, x);
+    }
 }
 
 // --------------------------------------------------- norm and rotation
@@ -122,8 +131,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ R
 // is cut into units of E elements (16 bytes, or one element where alignment
 // or sizes forbid that); a lane holds the unit with the first halves of its
 // pairs and the one with the second, so the rotation needs no exchange and a
-// row may be its own output.  Bound by memory; the lanes of a group keep
-// their cosines, sines and weights in registers over `hpg` heads of a token.
+// row may be its own output.  Bound by memory; a group of lanes loads U heads of
+// a token before it uses the first, and keeps cosines, sines and weights in
+// registers over them.
 struct RopeP {
     const void* x[2];  // q, k
     void* y[2];
@@ -134,43 +144,30 @@ struct RopeP {
     const int32_t* pos;
     int64_t n, max_pos;
     int heads[2];
-    int hd, rot, inter, lpr, hpg;
+    int hd, rot, inter, lpr, lpr_log;
     float eps;
 };
 
 template <typename T, int E>
-__device__ __forceinline__ void load_unit(const T* __restrict__ p, float (&x)[E]) {
-    if constexpr (E == 1) {
-        x[0] = to_f32(p[0]);
-    } else {
-        T tmp[E];
-        *reinterpret_cast<uint4*>(tmp) = *reinterpret_cast<const uint4*>(p);
+struct alignas(sizeof(T) * E) Unit {
+    T v[E];
+    Unit() = default;
+    __device__ __forceinline__ explicit Unit(const float (&x)[E]) {
 #pragma unroll
-        for (int i = 0; i < E; i++) x[i] = to_f32(tmp[i]);
+        for (int i = 0; i < E; i++) v[i] = from_f32<T>(x[i]);
     }
-}
-template <typename T, int E>
-__device__ __forceinline__ void store_unit(T* p, const float (&x)[E]) {
-    if constexpr (E == 1) {
-        p[0] = from_f32<T>(x[0]);
-    } else {
-        T tmp[E];
-#pragma unroll
-        for (int i = 0; i < E; i++) tmp[i] = from_f32<T>(x[i]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(tmp);
-    }
-}
+};
 
-template <typename T, int E, int S>
+template <typename T, int E, int S, int U>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeP p) {
     pdl_wait();
     const int lpr = p.lpr, lane = threadIdx.x & 31, sl = lane & (lpr - 1);
     const unsigned group = (lpr == 32 ? 0xffffffffu : ((1u << lpr) - 1u)) << (lane & ~(lpr - 1));
-    const int64_t gi = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
-    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
-    const int64_t n = gi / (gq + gk);
+    const unsigned gi = blockIdx.x * (256u >> p.lpr_log) + (threadIdx.x >> p.lpr_log);
+    const int gq = (p.heads[0] + U - 1) / U, gk = (p.heads[1] + U - 1) / U;
+    const int64_t n = gi / (unsigned)(gq + gk);
     if (n >= p.n) return;
-    int sub = (int)(gi - n * (gq + gk));
+    int sub = (int)(gi - (unsigned)n * (unsigned)(gq + gk));
     const int which = sub >= gq;
     if (which) sub -= gq;
     const int64_t pos = p.pos[n];
@@ -210,21 +207,33 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant
             w1[s][e] = w && u1[s] >= 0 ? w[u1[s] * E + e] : 1.0f;
         }
     }
-    const int h0 = sub * p.hpg, h1 = min(h0 + p.hpg, p.heads[which]);
-    const T* xr = static_cast<const T*>(p.x[which]) + n * p.xt[which];
-    T* yr = static_cast<T*>(p.y[which]) + n * p.yt[which];
-    for (int h = h0; h < h1; h++) {
-        const T* x = xr + h * p.xh[which];
+    const int h0 = sub * U, hn = min(U, p.heads[which] - h0);
+    const T* xr = static_cast<const T*>(p.x[which]) + n * p.xt[which] + h0 * p.xh[which];
+    T* yr = static_cast<T*>(p.y[which]) + n * p.yt[which] + h0 * p.yh[which];
+    Unit<T, E> ra[U][S], rb[U][S];  // all heads' loads before the first use
+#pragma unroll
+    for (int h = 0; h < U; h++)
+        if (h < hn) {
+            const T* x = xr + h * p.xh[which];
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                if (u0[s] >= 0) ra[h][s] = *reinterpret_cast<const Unit<T, E>*>(x + u0[s] * E);
+                if (u1[s] >= 0) rb[h][s] = *reinterpret_cast<const Unit<T, E>*>(x + u1[s] * E);
+            }
+        }
+#pragma unroll
+    for (int h = 0; h < U; h++) {
+        if (h >= hn) break;
         T* y = yr + h * p.yh[which];
         float a[S][E], b[S][E];
         float ss = 0.0f;
 #pragma unroll
-        for (int s = 0; s < S; s++) {
+        for (int s = 0; s < S; s++)
 #pragma unroll
-            for (int e = 0; e < E; e++) a[s][e] = b[s][e] = 0.0f;
-            if (u0[s] >= 0) load_unit<T, E>(x + u0[s] * E, a[s]);
-            if (u1[s] >= 0) load_unit<T, E>(x + u1[s] * E, b[s]);
-        }
+            for (int e = 0; e < E; e++) {
+                a[s][e] = u0[s] >= 0 ? to_f32(ra[h][s].v[e]) : 0.0f;
+                b[s][e] = u1[s] >= 0 ? to_f32(rb[h][s].v[e]) : 0.0f;
+            }
         if (w) {
 #pragma unroll
             for (int s = 0; s < S; s++)
@@ -263,8 +272,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant
                     }
                 }
             }
-            if (u0[s] >= 0) store_unit<T, E>(y + u0[s] * E, a[s]);
-            if (u1[s] >= 0) store_unit<T, E>(y + u1[s] * E, b[s]);
+            if (u0[s] >= 0) *reinterpret_cast<Unit<T, E>*>(y + u0[s] * E) = Unit<T, E>(a[s]);
+            if (u1[s] >= 0) *reinterpret_cast<Unit<T, E>*>(y + u1[s] * E) = Unit<T, E>(b[s]);
         }
     }
 }
@@ -423,6 +432,14 @@ int check_grid(int64_t blocks, const char* fn) {
     return blocks > INT32_MAX ? set_error(RQ_ERR_INVALID, "%s: too many rows for one call", fn) : RQ_OK;
 }
 
+// Tokens of an append or read CTA: about four items a thread where the tokens
+// fill the device anyway, else one.
+int tokens_per_cta(const rq_kv4* c, int64_t n) {
+    const int64_t items = (int64_t)2 * c->n_kv * (c->head_dim / 8);
+    const int64_t want = n * items > (int64_t)c->ctx->sm_count * 2048 * 4 ? 1024 : 256;
+    return (int)std::max<int64_t>(1, want / items);
+}
+
 AppendP append_params(const rq_kv4* c, const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh,
                       const int32_t* slots, int64_t n, size_t size) {
     AppendP p{};
@@ -441,6 +458,7 @@ AppendP append_params(const rq_kv4* c, const void* k, int64_t kt, int64_t kh, co
     p.page_size = c->page_size;
     p.n_kv = c->n_kv;
     p.nb = c->head_dim / 32;
+    p.per_cta = tokens_per_cta(c, n);
     return p;
 }
 
@@ -456,23 +474,28 @@ int qk_norm_rope(const rq_ctx* ctx, const rq_qk_rope* a, cudaStream_t st) {
     const int E = vec ? wide : 1;
     const int slots = p.rot / (2 * E) + ((p.hd - p.rot) / E + 1) / 2;
     p.lpr = 1;
-    while (p.lpr < slots && p.lpr < 32) p.lpr *= 2;
+    for (; p.lpr < slots && p.lpr < 32; p.lpr *= 2) p.lpr_log++;
     const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
-    // heads a group goes over: one while the rows do not fill the device's
-    // threads, else four (the tables' loads shared)
-    p.hpg = rows * p.lpr <= (int64_t)ctx->sm_count * 2048 ? 1 : 4;
-    const int gq = (p.heads[0] + p.hpg - 1) / p.hpg, gk = (p.heads[1] + p.hpg - 1) / p.hpg;
+    // one head a group while the rows do not fill the device's threads, else
+    // four (8191 tokens, 64 + 8 heads of 128, bf16: 112 -> XX us)
+    const bool four = vec && rows * p.lpr > (int64_t)ctx->sm_count * 2048;
+    const int U = four ? 4 : 1;
+    const int gq = (p.heads[0] + U - 1) / U, gk = (p.heads[1] + U - 1) / U;
     const int64_t blocks = (p.n * (gq + gk) * p.lpr + 255) / 256;
-    const int rc = check_grid(blocks, "rq_qk_norm_rope");
-    if (rc) return rc;
+    if (p.n * (gq + gk) > INT32_MAX) return set_error(RQ_ERR_INVALID, "rq_qk_norm_rope: too many rows for one call");
     const void* fn;
     if (a->dtype == RQ_F32)
-        fn = vec ? (const void*)qk_norm_rope_kernel<float, 4, 1> : (const void*)qk_norm_rope_kernel<float, 1, 4>;
+        fn = four  ? (const void*)qk_norm_rope_kernel<float, 4, 1, 4>
+             : vec ? (const void*)qk_norm_rope_kernel<float, 4, 1, 1>
+                   : (const void*)qk_norm_rope_kernel<float, 1, 4, 1>;
     else if (a->dtype == RQ_F16)
-        fn = vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1> : (const void*)qk_norm_rope_kernel<__half, 1, 4>;
+        fn = four  ? (const void*)qk_norm_rope_kernel<__half, 8, 1, 4>
+             : vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1, 1>
+                   : (const void*)qk_norm_rope_kernel<__half, 1, 4, 1>;
     else
-        fn = vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1>
-                 : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4>;
+        fn = four  ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1, 4>
+             : vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1, 1>
+                   : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4, 1>;
     void* args[] = {&p};
     return launch_pdl(fn, (unsigned)blocks, 256, 0, st, args, "q/k norm and rotation kernel");
 }
@@ -571,7 +594,7 @@ int rq_kv4_append(rq_kv4* c, int dtype, const void* k, const int64_t k_stride[2]
     if (!rc) rc = check_device_ptr(c->ctx, slots, "rq_kv4_append", "slots");
     if (rc) return rc;
     AppendP p = append_params(c, k, k_stride[0], k_stride[1], v, v_stride[0], v_stride[1], slots, n, size);
-    const int64_t blocks = (n * 2 * c->n_kv * 4 * p.nb + 255) / 256;
+    const int64_t blocks = (n + p.per_cta - 1) / p.per_cta;
     rc = check_grid(blocks, "rq_kv4_append");
     if (rc) return rc;
     const void* fn = dtype == RQ_F32 ? (const void*)kv4_append_kernel<float>
@@ -604,7 +627,8 @@ int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, void* k, 
     p.x[0] = k;
     p.x[1] = v;
     p.wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
-    const int64_t blocks = (n * 2 * c->n_kv * 4 * p.nb + 255) / 256;
+    p.per_cta = tokens_per_cta(c, n);
+    const int64_t blocks = (n + p.per_cta - 1) / p.per_cta;
     rc = check_grid(blocks, "rq_kv4_read");
     if (rc) return rc;
     const void* fn = dtype == RQ_F32 ? (const void*)kv4_read_kernel<float>

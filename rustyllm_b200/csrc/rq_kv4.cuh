@@ -67,7 +67,7 @@ __host__ __device__ __forceinline__ int kv4_v_at(int nb, int tok, int b, int g) 
 __device__ __forceinline__ uint8_t* kv4_record(uint8_t* data, int64_t n_slots, int page_size, int n_kv, int rec_bytes,
                                                int32_t slot, int head) {
     if (slot < 0 || slot >= n_slots) return nullptr;
-    const int page = slot / page_size, off = slot % page_size;
+    const int page = (int)((unsigned)slot / (unsigned)page_size), off = slot - page * page_size;
     return data + (((int64_t)page * n_kv + head) * (page_size / kKv4Tile) + off / kKv4Tile) * rec_bytes;
 }
 
@@ -113,89 +113,97 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool wide, const float
     }
 }
 
-// The four lanes of an aligned group hold a block, 8 elements each.  Returns
-// the block's scale (f16 value in f32) and this lane's 8 codes as nibbles in
-// element order.  d = f16(m / -8), m the element of the largest magnitude
-// (the lowest index of equals); m / 8 is exact, so d is one rounding.  A code
-// is the nearest multiple of d (ties to the higher code): (c - 8.5) * d has at
-// most 16 bits, exact in f32, so the comparisons below decide exactly where
-// an f32 quotient would be off near a border.  A NaN makes the scale NaN (the
-// block reads back as NaN); infinities saturate the scale at 65504.
-__device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], float& d_out) {
-    float m = x[0];
-    bool nan = x[0] != x[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) {
-        nan |= x[i] != x[i];
-        if (fabsf(x[i]) > fabsf(m)) m = x[i];
-    }
-    const unsigned lane = threadIdx.x & 31;
-    const unsigned group = 0xFu << (lane & 28);
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-        const float other = __shfl_xor_sync(group, m, o);
-        const bool lower = (lane & o) != 0;  // the other lane holds lower indexes
-        if (lower ? fabsf(other) >= fabsf(m) : fabsf(other) > fabsf(m)) m = other;
-    }
-    nan = (__ballot_sync(group, nan) & group) != 0;
-    const float d = __half2float(__float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f)));
-    uint32_t w = 0;
-    if (nan) {
-        d_out = __int_as_float(0x7fffffff);
-        return 0x88888888u;
-    }
-    d_out = d;
-    if (d == 0.0f) return 0x88888888u;
-    const float inv = 1.0f / d;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float t = fminf(fmaxf(floorf(x[i] * inv + 8.5f), 0.0f), 15.0f);
-        const float lo = (t - 8.5f) * d, hi = (t - 7.5f) * d;
-        if (t > 0.0f && (d > 0.0f ? x[i] < lo : x[i] > lo)) t -= 1.0f;
-        else if (t < 15.0f && (d > 0.0f ? x[i] >= hi : x[i] <= hi)) t += 1.0f;
-        w |= (uint32_t)t << (4 * i);
-    }
-    return w;
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
 }
 
-// element-order nibbles -> K word (element 2 i + h to nibble i + 4 h) and back
-__device__ __forceinline__ uint32_t kv4_k_word(uint32_t w) {
-    uint32_t r = 0;
+// The four lanes of an aligned group hold a block, 8 elements each.  Returns
+// the block's scale (f16 value in f32) and this lane's 8 codes.  d = f16(m /
+// -8), m the element of the largest magnitude (the lowest index of equals); m /
+// 8 is exact, so d is one rounding.  A code is the nearest multiple of d (ties
+// to the higher code).  x * (1 / d) is within 2^-20 of x / d where |x / d| <= 8,
+// so rounding it decides all but what lies that near to a half; there (rare,
+// but for 16-bit inputs exact ties are not) the comparison of x with (c - 8.5) d
+// decides, a product of at most 16 bits and so exact in f32.  A NaN makes the
+// scale NaN (the block reads back as NaN); infinities saturate it at 65504.
+__device__ __forceinline__ float kv4_quantize(const float (&x)[8], uint32_t (&c)[8]) {
+    float big = fabsf(x[0]);
 #pragma unroll
-    for (int i = 0; i < 8; i++) r |= ((w >> (4 * i)) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
-    return r;
-}
-__device__ __forceinline__ uint32_t kv4_k_unword(uint32_t r) {
-    uint32_t w = 0;
+    for (int i = 1; i < 8; i++) big = max_nan(big, fabsf(x[i]));
+    const unsigned lane = threadIdx.x & 31;
+    const unsigned group = 0xFu << (lane & 28);
+    big = max_nan(big, __shfl_xor_sync(group, big, 1));
+    big = max_nan(big, __shfl_xor_sync(group, big, 2));
+    float m = x[7];
+    bool here = fabsf(x[7]) == big;
 #pragma unroll
-    for (int i = 0; i < 8; i++) w |= ((r >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) << (4 * i);
-    return w;
+    for (int i = 6; i >= 0; i--) {
+        const bool is = fabsf(x[i]) == big;
+        m = is ? x[i] : m;
+        here |= is;
+    }
+    const unsigned who = __ballot_sync(group, here) & group;
+    m = __shfl_sync(group, m, who ? __ffs((int)who) - 1 : (int)lane);
+    const float d = __half2float(__float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f)));
+    if (!(big == big) || d == 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = 8;
+        return big == big ? d : __int_as_float(0x7fffffff);
+    }
+    const float inv = 1.0f / d;
+    bool near_half = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = fminf(fmaxf(x[i] * inv, -8.0f), 7.0f);
+        const float z = v + 12582912.0f;  // 1.5 * 2^23: rounds v to an integer in the low bits
+        near_half |= fabsf(v - (z - 12582912.0f)) > 0.499996f;
+        c[i] = (__float_as_uint(z) + 8u) & 15u;
+    }
+    if (near_half) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float t = fminf(fmaxf(floorf(x[i] * inv + 8.5f), 0.0f), 15.0f);
+            const float lo = (t - 8.5f) * d, hi = (t - 7.5f) * d;
+            if (t > 0.0f && (d > 0.0f ? x[i] < lo : x[i] > lo)) t -= 1.0f;
+            else if (t < 15.0f && (d > 0.0f ? x[i] >= hi : x[i] <= hi)) t += 1.0f;
+            c[i] = (uint32_t)t;
+        }
+    }
+    return d;
 }
 
 // Writes one lane's share of a token's block: x holds elements 32 b + 8 t ..
 // + 7 (t = lane % 4; the aligned four lanes hold the block).  rec NULL: the
 // lane takes part in the group's exchange and writes nothing.
 __device__ __forceinline__ void kv4_store(uint8_t* rec, int nb, int tok, int b, bool is_v, const float (&x)[8]) {
-    float d;
-    const uint32_t w = kv4_quantize(x, d);
+    uint32_t c[8];
+    const float d = kv4_quantize(x, c);
     const unsigned lane = threadIdx.x & 31, t = lane & 3;
     const unsigned group = 0xFu << (lane & 28);
     uint8_t* codes = rec + (is_v ? 256 * nb : 0);
     if (!is_v) {
-        if (rec) *reinterpret_cast<uint32_t*>(codes + kv4_k_at(nb, tok, b, (int)t)) = kv4_k_word(w);
+        uint32_t w = 0;  // element 2 i + h in nibble i + 4 h
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= c[i] << (4 * ((i >> 1) + 4 * (i & 1)));
+        if (rec) *reinterpret_cast<uint32_t*>(codes + kv4_k_at(nb, tok, b, (int)t)) = w;
     } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= c[i] << (4 * i);
         // element 8 k + g of lane k goes to nibble k of item g: lane t writes
-        // items 2 t and 2 t + 1
-        uint32_t a = 0, c = 0;
+        // items 2 t and 2 t + 1, bytes t of the four words
+        uint32_t a = 0, e = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint32_t o = __shfl_sync(group, w, (int)((lane & 28) + k));
-            a |= ((o >> (8 * t)) & 15u) << (4 * k);
-            c |= ((o >> (8 * t + 4)) & 15u) << (4 * k);
+            const uint32_t o = __shfl_sync(group, w, (int)((lane & 28) + k)) >> (8 * t);
+            a |= (o & 15u) << (4 * k);
+            e |= ((o >> 4) & 15u) << (4 * k);
         }
         if (rec) {
             *reinterpret_cast<uint16_t*>(codes + kv4_v_at(nb, tok, b, (int)(2 * t))) = (uint16_t)a;
-            *reinterpret_cast<uint16_t*>(codes + kv4_v_at(nb, tok, b, (int)(2 * t + 1))) = (uint16_t)c;
+            *reinterpret_cast<uint16_t*>(codes + kv4_v_at(nb, tok, b, (int)(2 * t + 1))) = (uint16_t)e;
         }
     }
     if (rec && t == 0)
@@ -206,12 +214,14 @@ __device__ __forceinline__ void kv4_store(uint8_t* rec, int nb, int tok, int b, 
 __device__ __forceinline__ void kv4_load(const uint8_t* rec, int nb, int tok, int b, bool is_v, float (&x)[8]) {
     const unsigned lane = threadIdx.x & 31, t = lane & 3;
     const unsigned group = 0xFu << (lane & 28);
-    uint32_t w = 0;
     float d = 0.0f;
     if (rec) d = __half2float(*reinterpret_cast<const __half*>(rec + 512 * nb + (is_v ? 32 * nb : 0) + kv4_scale(nb, tok, b)));
     if (!is_v) {
-        if (rec) w = kv4_k_unword(*reinterpret_cast<const uint32_t*>(rec + kv4_k_at(nb, tok, b, (int)t)));
+        const uint32_t w = rec ? *reinterpret_cast<const uint32_t*>(rec + kv4_k_at(nb, tok, b, (int)t)) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = ((float)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - 8.0f) * d;
     } else {
+        uint32_t w = 0;
         uint32_t items = 0;
         if (rec)
             items = *reinterpret_cast<const uint16_t*>(rec + 256 * nb + kv4_v_at(nb, tok, b, (int)(2 * t))) |
@@ -222,9 +232,9 @@ __device__ __forceinline__ void kv4_load(const uint8_t* rec, int nb, int tok, in
             w |= ((o >> (4 * t)) & 15u) << (8 * k);
             w |= ((o >> (16 + 4 * t)) & 15u) << (8 * k + 4);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = ((float)((w >> (4 * i)) & 15u) - 8.0f) * d;
+        for (int i = 0; i < 8; i++) x[i] = ((float)((w >> (4 * i)) & 15u) - 8.0f) * d;
+    }
 }
 
 // shared host helpers of the paged operators (rq_kv4.cu)

@@ -12,9 +12,10 @@
 //
 // Bound by memory: one row of p and of q per sequence.  A cluster of up to 8
 // CTAs takes a sequence; each CTA sums a contiguous share of the row in groups
-// of kGroup consecutive elements (one warp a group, so loads are whole lines),
-// the CTAs exchange their sums through distributed shared memory, and the one
-// whose share holds the target re-reads one group (from L2) and scans it.
+// of kGroup consecutive elements (one warp a group, 2 x 16 whole lines in
+// flight), the CTAs exchange their sums through distributed shared memory, and
+// the one whose share holds the target re-reads one group (from L2), 16
+// elements a lane, and scans it.
 #include <algorithm>
 
 #include "rq_kv4.cuh"
@@ -23,8 +24,8 @@ namespace rq {
 namespace {
 
 constexpr int kThreads = 512, kWarpsV = kThreads / 32;
-constexpr int kGroup = 128;       // elements a warp sums at a time
-constexpr int kMaxGroups = 2048;  // groups of a CTA's share kept in shared memory
+constexpr int kPer = 16, kGroup = 32 * kPer;  // elements a warp sums at a time
+constexpr int kMaxGroups = 512;               // groups of a CTA's share kept in shared memory
 
 struct VerifyP {
     const void* p;
@@ -51,12 +52,7 @@ struct Row {  // the weights that the token is drawn from
     int64_t hole;   // element without weight (a certain draft), or -1
 };
 
-template <typename T>
-__device__ __forceinline__ double weight(const Row& w, int64_t j) {
-    double a = mass(to_f32(static_cast<const T*>(w.p)[j]));
-    if (w.q) a = fmax(a - mass(to_f32(static_cast<const T*>(w.q)[j])), 0.0);
-    return j == w.hole ? 0.0 : a;
-}
+__device__ __forceinline__ double weight(float p, float q) { return fmax(mass(p) - mass(q), 0.0); }
 
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
@@ -121,8 +117,17 @@ __global__ void __launch_bounds__(kThreads) spec_verify_kernel(const __grid_cons
     for (int pass = 0; pass < 2; pass++) {
         for (int64_t g = g0 + warp; g < g1; g += kWarpsV) {
             double a = 0.0;
-            const int64_t e1 = min((g + 1) * glen, p.vocab);
-            for (int64_t j = g * glen + lane; j < e1; j += 32) a += weight<T>(w, j);
+            for (int64_t j0 = g * glen; j0 < min((g + 1) * glen, p.vocab); j0 += kGroup) {
+                float x[kPer], y[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const int64_t j = j0 + 32 * i + lane;
+                    x[i] = j < p.vocab ? to_f32(static_cast<const T*>(w.p)[j]) : 0.0f;
+                    y[i] = w.q && j < p.vocab ? to_f32(static_cast<const T*>(w.q)[j]) : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < kPer; i++) a += j0 + 32 * i + lane == w.hole ? 0.0 : weight(x[i], y[i]);
+            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
             if (lane == 0) sums[g - g0] = a;
@@ -196,26 +201,59 @@ __global__ void __launch_bounds__(kThreads) spec_verify_kernel(const __grid_cons
         pick = last;
         pick_run = last_run;
     }
-    // the element: 32 at a time, a warp scan
+    // the element: kPer consecutive ones a lane, a scan over the lanes, and the
+    // lane that passes goes over its own
     const int64_t e0 = (g0 + pick) * glen, e1 = min(e0 + glen, p.vocab);
-    int64_t found = -1, lastpos = -1;
+    int64_t last_el = -1;
     double upto = pick_run;
-    for (int64_t j0 = e0; j0 < e1 && found < 0; j0 += 32) {
-        const int64_t j = j0 + lane;
-        const double x = j < e1 ? weight<T>(w, j) : 0.0;
-        double s = x;
+    for (int64_t j0 = e0; j0 < e1; j0 += kGroup) {
+        double x[kPer], sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int64_t j = j0 + lane * kPer + i;
+            x[i] = 0.0;
+            if (j < e1 && j != w.hole)
+                x[i] = weight(to_f32(static_cast<const T*>(w.p)[j]), w.q ? to_f32(static_cast<const T*>(w.q)[j]) : 0.0f);
+        }
+        int mine_last = -1;  // this lane's last element with weight
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            sum += x[i];
+            if (x[i] > 0.0) mine_last = i;
+        }
+        double s = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double v = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += v;
         }
-        const unsigned pos = __ballot_sync(0xffffffffu, x > 0.0);
-        const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && upto + s > target);
-        if (hit) found = j0 + __ffs((int)hit) - 1;
-        if (pos) lastpos = j0 + 31 - __clz((int)pos);
+        int hit = -1;
+        if (mine_last >= 0 && upto + s > target) {
+            double r = upto + (s - sum);
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                r += x[i];
+                if (!found && x[i] > 0.0 && r > target) {
+                    found = true;
+                    hit = i;
+                }
+            }
+            if (!found) hit = mine_last;  // rounding let no single one pass
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
+        if (who) {
+            if (lane == __ffs((int)who) - 1) out[acc] = (int32_t)(j0 + lane * kPer + hit);
+            return;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, mine_last >= 0);
+        if (some) {
+            const int l = 31 - __clz((int)some);
+            last_el = j0 + l * kPer + __shfl_sync(0xffffffffu, mine_last, l);
+        }
         upto += __shfl_sync(0xffffffffu, s, 31);
     }
-    if (lane == 0) out[acc] = (int32_t)(found >= 0 ? found : lastpos);
+    if (lane == 0) out[acc] = (int32_t)last_el;  // rounding let none pass: the last with weight
 }
 
 }  // namespace
@@ -261,7 +299,7 @@ extern "C" int rq_spec_verify(rq_ctx* ctx, int dtype, const void* p, const int64
     v.tokens = tokens;
     v.accepted = accepted;
     v.ctas = 1;
-    while (v.ctas < 8 && (int64_t)v.ctas * kGroup * kWarpsV * 2 < vocab) v.ctas *= 2;
+    while (v.ctas < 8 && (int64_t)v.ctas * kGroup * kWarpsV < vocab) v.ctas *= 2;
     v.per_group = (int)((vocab + (int64_t)kGroup * kMaxGroups * v.ctas - 1) / ((int64_t)kGroup * kMaxGroups * v.ctas));
     const void* fn = dtype == RQ_F32 ? (const void*)spec_verify_kernel<float>
                      : dtype == RQ_F16 ? (const void*)spec_verify_kernel<__half>

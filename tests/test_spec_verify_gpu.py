@@ -74,7 +74,7 @@ def test_tokens_match_the_rule(rq_ctx, kind, B, n, V):
 def test_large_group_runs_and_strided_rows(rq_ctx):
     """A vocabulary whose share of a CTA passes the sums kept in shared
     memory, and rows of a wider matrix."""
-    V = 128 * 2048 * 8 + 77
+    V = 512 * 512 * 8 + 77
     g = torch.Generator(device="cuda").manual_seed(1)
     wide = torch.rand(2, 2, V + 5, generator=g, device="cuda")
     run(wide[:, :, 3:V + 3], None, torch.tensor([[V - 1], [5]], dtype=torch.int32, device="cuda"),
