@@ -71,7 +71,7 @@ struct Item {
     int64_t n;
     int head, e;
     bool is_v;
-    __device__ __forceinline__ Item(unsigned i, int64_t first, int n_kv, int nb) {
+    __device__ __forceinline__ Item(unsigned i, int64_t first, int n_kv, unsigned nb) {
         const unsigned per = 4 * nb, row = i / per;
         const unsigned tok = row / (2u * n_kv), r = row - tok * 2u * n_kv;
         e = (int)(i - row * per);
@@ -81,19 +81,19 @@ struct Item {
     }
 };
 
-template <typename T>
+template <typename T, int NB>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendP p) {
     pdl_wait();
     const int64_t first = (int64_t)blockIdx.x * p.per_cta;
-    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * p.nb);
+    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * NB);
     for (unsigned i = threadIdx.x; i < items; i += 256) {
-        const Item it(i, first, p.n_kv, p.nb);
+        const Item it(i, first, p.n_kv, NB);
         const int32_t slot = p.slots[it.n];
         float x[8];
         load8(static_cast<const T*>(p.x[it.is_v]) + it.n * p.tok[it.is_v] + it.head * p.head[it.is_v] + 8 * it.e,
               p.wide[it.is_v], x);
-        uint8_t* rec = kv4_record(p.data, p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, it.head);
-        kv4_store(rec, p.nb, slot & 15, it.e >> 2, it.is_v, x);
+        uint8_t* rec = kv4_record(p.data, p.n_slots, p.page_size, p.n_kv, 576 * NB, slot, it.head);
+        kv4_store(rec, NB, slot & 15, it.e >> 2, it.is_v, x);
     }
 }
 
@@ -103,24 +103,24 @@ struct ReadP {
     const uint8_t* data;
     const int32_t* slots;
     int64_t n, n_slots;
-    int page_size, n_kv, nb, per_cta;
+    int page_size, n_kv, per_cta;
     void* x[2];  // [n][n_kv][head_dim]
     bool wide;
 };
 
-template <typename T>
+template <typename T, int NB>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ ReadP p) {
     pdl_wait();
     const int64_t first = (int64_t)blockIdx.x * p.per_cta;
-    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * p.nb);
+    const unsigned items = (unsigned)(min((int64_t)p.per_cta, p.n - first) * 2 * p.n_kv * 4 * NB);
     for (unsigned i = threadIdx.x; i < items; i += 256) {
-        const Item it(i, first, p.n_kv, p.nb);
+        const Item it(i, first, p.n_kv, NB);
         const int32_t slot = p.slots[it.n];
         const uint8_t* rec =
-            kv4_record(const_cast<uint8_t*>(p.data), p.n_slots, p.page_size, p.n_kv, 576 * p.nb, slot, it.head);
+            kv4_record(const_cast<uint8_t*>(p.data), p.n_slots, p.page_size, p.n_kv, 576 * NB, slot, it.head);
         float x[8];
-        kv4_load(rec, p.nb, slot & 15, it.e >> 2, it.is_v, x);
-        store8(static_cast<T*>(p.x[it.is_v]) + (it.n * p.n_kv + it.head) * (32 * p.nb) + 8 * it.e, p.wide, x);
+        kv4_load(rec, NB, slot & 15, it.e >> 2, it.is_v, x);
+        store8(static_cast<T*>(p.x[it.is_v]) + (it.n * p.n_kv + it.head) * (32 * NB) + 8 * it.e, p.wide, x);
     }
 }
 
@@ -128,12 +128,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ R
 //
 // y = x / sqrt(mean(x^2) + eps) * w per head (w NULL: y = x), then the first
 // rot elements rotated in pairs by the angles of the token's position.  A row
-// is cut into units of E elements (16 bytes, or one element where alignment
-// or sizes forbid that); a lane holds the unit with the first halves of its
+// is cut into units of E elements (four, or one where alignment or sizes forbid
+// that); a lane holds the unit with the first halves of its
 // pairs and the one with the second, so the rotation needs no exchange and a
-// row may be its own output.  Bound by memory; a group of lanes loads U heads of
-// a token before it uses the first, and keeps cosines, sines and weights in
-// registers over them.
+// row may be its own output.  Bound by memory.
+constexpr int kRopeRows = 2;  // heads that a group of lanes takes at once where the rows are many
 struct RopeP {
     const void* x[2];  // q, k
     void* y[2];
@@ -145,11 +144,12 @@ struct RopeP {
     int64_t n, max_pos;
     int heads[2];
     int hd, rot, inter, lpr, lpr_log;
-    float eps;
+    unsigned q_ctas;
+    float eps, inv_hd;
 };
 
 template <typename T, int E>
-struct alignas(sizeof(T) * E) Unit {
+struct alignas(sizeof(T) * E > 16 ? 16 : sizeof(T) * E) Unit {
     T v[E];
     Unit() = default;
     __device__ __forceinline__ explicit Unit(const float (&x)[E]) {
@@ -158,123 +158,239 @@ struct alignas(sizeof(T) * E) Unit {
     }
 };
 
-template <typename T, int E, int S, int U>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeP p) {
-    pdl_wait();
-    const int lpr = p.lpr, lane = threadIdx.x & 31, sl = lane & (lpr - 1);
-    const unsigned group = (lpr == 32 ? 0xffffffffu : ((1u << lpr) - 1u)) << (lane & ~(lpr - 1));
-    const unsigned gi = blockIdx.x * (256u >> p.lpr_log) + (threadIdx.x >> p.lpr_log);
-    const int gq = (p.heads[0] + U - 1) / U, gk = (p.heads[1] + U - 1) / U;
-    const int64_t n = gi / (unsigned)(gq + gk);
-    if (n >= p.n) return;
-    int sub = (int)(gi - (unsigned)n * (unsigned)(gq + gk));
-    const int which = sub >= gq;
-    if (which) sub -= gq;
-    const int64_t pos = p.pos[n];
-    if (pos < 0 || pos >= p.max_pos) return;  // the row stays as it was
-    const int P = p.rot / (2 * E), rest = (p.hd - p.rot) / E;
-    int u0[S], u1[S];
-    float c0[S][E], s0[S][E], w0[S][E], w1[S][E];
-    const float* w = p.w[which];
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-        const int i = sl + s * lpr;
-        const int r = 2 * (i - P);
-        u0[s] = i < P ? i : r < rest ? 2 * P + r : -1;
-        u1[s] = i < P ? i + P : r + 1 < rest ? 2 * P + r + 1 : -1;
-        // halves: the pair (e of u0, e of u1) turns by angle i E + e;
-        // interleaved: neighbours inside a unit, E / 2 angles a unit (E = 1
-        // is paired by index below)
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            c0[s][e] = 1.0f;
-            s0[s][e] = 0.0f;
-            if (i < P) {
-                int64_t a;
-                if (!p.inter || E == 1) a = (int64_t)i * E + e;
-                else a = e < E / 2 ? (int64_t)u0[s] * (E / 2) + e : (int64_t)u1[s] * (E / 2) + (e - E / 2);
-                c0[s][e] = p.cos[pos * (p.rot / 2) + a];
-                s0[s][e] = p.sin[pos * (p.rot / 2) + a];
-            }
-        }
-        if (p.inter && E == 1 && i < P) {  // single elements: the pair is (2 i, 2 i + 1)
-            u0[s] = 2 * i;
-            u1[s] = 2 * i + 1;
-        }
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            w0[s][e] = w && u0[s] >= 0 ? w[u0[s] * E + e] : 1.0f;
-            w1[s][e] = w && u1[s] >= 0 ? w[u1[s] * E + e] : 1.0f;
+// What a lane holds of one head's row: units u0 and u1 (-1: none), the first and
+// second halves of its pairs where i < P = rot / 2 E (interleaved: its pairs are
+// neighbours), elements that are not rotated behind them.
+template <int E>
+struct Lane {
+    int u0, u1;
+    bool turns;
+    __device__ __forceinline__ Lane(const RopeP& p, int i) {
+        const int P = p.rot / (2 * E), rest = (p.hd - p.rot) / E, r = 2 * (i - P);
+        turns = i < P;
+        u0 = turns ? i : r < rest ? 2 * P + r : -1;
+        u1 = turns ? i + P : r + 1 < rest ? 2 * P + r + 1 : -1;
+        if (p.inter && E == 1 && turns) {  // single elements: the pair is (2 i, 2 i + 1)
+            u0 = 2 * i;
+            u1 = 2 * i + 1;
         }
     }
-    const int h0 = sub * U, hn = min(U, p.heads[which] - h0);
-    const T* xr = static_cast<const T*>(p.x[which]) + n * p.xt[which] + h0 * p.xh[which];
-    T* yr = static_cast<T*>(p.y[which]) + n * p.yt[which] + h0 * p.yh[which];
-    Unit<T, E> ra[U][S], rb[U][S];  // all heads' loads before the first use
+};
+// The angles of a position for a lane's pairs, in element order of u0 and u1
+// (halves: a pair takes one of each; interleaved: the pairs of u0 first)
+template <int E>
+struct Angles {
+    Unit<float, E> cs, sn;
+    __device__ __forceinline__ void load(const RopeP& p, const Lane<E>& l, int64_t pos) {
+        if (!l.turns || pos < 0 || pos >= p.max_pos) return;
+        const float* c = p.cos + pos * (p.rot / 2);
+        const float* z = p.sin + pos * (p.rot / 2);
+        if (E == 1 || !p.inter) {
+            const int at = E == 1 && p.inter ? l.u0 / 2 : l.u0 * E;
+            cs = *reinterpret_cast<const Unit<float, E>*>(c + at);
+            sn = *reinterpret_cast<const Unit<float, E>*>(z + at);
+        } else if constexpr (E > 1) {
+            using Half = Unit<float, E / 2>;
+            const Half c0 = *reinterpret_cast<const Half*>(c + l.u0 * (E / 2)), c1 = *reinterpret_cast<const Half*>(c + l.u1 * (E / 2));
+            const Half z0 = *reinterpret_cast<const Half*>(z + l.u0 * (E / 2)), z1 = *reinterpret_cast<const Half*>(z + l.u1 * (E / 2));
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) {
+                cs.v[e] = c0.v[e];
+                sn.v[e] = z0.v[e];
+                cs.v[E / 2 + e] = c1.v[e];
+                sn.v[E / 2 + e] = z1.v[e];
+            }
+        }
+    }
+};
+// The norm's weights taken into the rotation: per pair (f, g) of elements
+//   f' = r (f A + g B), g' = r (f C + g D)   (A = wf cos, B = -wg sin, ..);
+// elements that are not rotated use A and D alone.
+template <int E>
+struct Coeffs {
+    float A[E], B[E], C[E], D[E];
+    __device__ __forceinline__ Coeffs(const RopeP& p, const Lane<E>& l, const Angles<E>& t, const float* w) {
+        Unit<float, E> w0, w1;
+#pragma unroll
+        for (int e = 0; e < E; e++) w0.v[e] = w1.v[e] = 1.0f;
+        if (w) {
+            if (l.u0 >= 0) w0 = *reinterpret_cast<const Unit<float, E>*>(w + l.u0 * E);
+            if (l.u1 >= 0) w1 = *reinterpret_cast<const Unit<float, E>*>(w + l.u1 * E);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            float f = w0.v[e], g = w1.v[e];
+            if (E > 1 && p.inter && l.turns) {
+                f = 2 * e < E ? w0.v[2 * e % E] : w1.v[2 * e % E];
+                g = 2 * e < E ? w0.v[(2 * e + 1) % E] : w1.v[(2 * e + 1) % E];
+            }
+            const float cs = l.turns ? t.cs.v[e] : 1.0f, sn = l.turns ? t.sn.v[e] : 0.0f;
+            A[e] = f * cs;
+            B[e] = -g * sn;
+            C[e] = f * sn;
+            D[e] = g * cs;
+        }
+    }
+    __device__ __forceinline__ void turn(const RopeP& p, const Lane<E>& l, float (&a)[E], float (&b)[E]) const {
+        if (!l.turns) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                a[e] *= A[e];
+                b[e] *= D[e];
+            }
+        } else if (E == 1 || !p.inter) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float2 v = fma2(make_float2(a[e], a[e]), make_float2(A[e], C[e]),
+                                      mul2(make_float2(b[e], b[e]), make_float2(B[e], D[e])));
+                a[e] = v.x;
+                b[e] = v.y;
+            }
+        } else if constexpr (E > 1) {
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) {
+                float f = a[2 * e], g = a[2 * e + 1];
+                a[2 * e] = f * A[e] + g * B[e];
+                a[2 * e + 1] = f * C[e] + g * D[e];
+                f = b[2 * e];
+                g = b[2 * e + 1];
+                b[2 * e] = f * A[E / 2 + e] + g * B[E / 2 + e];
+                b[2 * e + 1] = f * C[E / 2 + e] + g * D[E / 2 + e];
+            }
+        }
+    }
+};
+__device__ __forceinline__ float group_sum(float v, int lpr, unsigned group) {
+    for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(group, v, o);
+    return v;
+}
+__device__ __forceinline__ unsigned group_mask(int lpr, int lane) {
+    return (lpr == 32 ? 0xffffffffu : ((1u << lpr) - 1u)) << (lane & ~(lpr - 1));
+}
+
+// q (0) or k (1), the same for a whole CTA: selected once, since a pointer
+// picked from the parameters by a thread's index costs every access
+template <typename T>
+struct Side {
+    const T* x;
+    T* y;
+    const float* w;
+    int64_t xt, xh, yt, yh;
+    int heads;
+    __device__ __forceinline__ Side(const RopeP& p, bool k)
+        : x(static_cast<const T*>(k ? p.x[1] : p.x[0])), y(static_cast<T*>(k ? p.y[1] : p.y[0])), w(k ? p.w[1] : p.w[0]),
+          xt(k ? p.xt[1] : p.xt[0]), xh(k ? p.xh[1] : p.xh[0]), yt(k ? p.yt[1] : p.yt[0]), yh(k ? p.yh[1] : p.yh[0]),
+          heads(k ? p.heads[1] : p.heads[0]) {}
+};
+
+// One row a group of lanes: few rows, and what the units of four cannot take.
+// The first q_ctas CTAs take q's rows, the others k's.
+template <typename T, int E, int S>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeP p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, sl = lane & (p.lpr - 1);
+    const unsigned group = group_mask(p.lpr, lane);
+    const bool is_k = blockIdx.x >= p.q_ctas;
+    const Side<T> o(p, is_k);
+    const unsigned gi = (blockIdx.x - (is_k ? p.q_ctas : 0)) * (256u >> p.lpr_log) + (threadIdx.x >> p.lpr_log);
+    const int64_t n = gi / (unsigned)o.heads;
+    if (n >= p.n) return;
+    const int head = (int)(gi - (unsigned)n * (unsigned)o.heads);
+    const T* x = o.x + n * o.xt + head * o.xh;
+    T* y = o.y + n * o.yt + head * o.yh;
+    // the row's loads come first: the position, the tables behind it and the
+    // row are then not three round trips to memory
+    float a[S][E], b[S][E], ss = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const Lane<E> l(p, sl + s * p.lpr);
+        Unit<T, E> ra, rb;
+        if (l.u0 >= 0) ra = *reinterpret_cast<const Unit<T, E>*>(x + l.u0 * E);
+        if (l.u1 >= 0) rb = *reinterpret_cast<const Unit<T, E>*>(x + l.u1 * E);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            a[s][e] = l.u0 >= 0 ? to_f32(ra.v[e]) : 0.0f;
+            b[s][e] = l.u1 >= 0 ? to_f32(rb.v[e]) : 0.0f;
+            ss = fmaf(a[s][e], a[s][e], fmaf(b[s][e], b[s][e], ss));
+        }
+    }
+    const int64_t pos = p.pos[n];
+    if (pos < 0 || pos >= p.max_pos) return;  // the row stays as it was
+    const float r = o.w ? rsqrtf(fmaf(group_sum(ss, p.lpr, group), p.inv_hd, p.eps)) : 1.0f;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const Lane<E> l(p, sl + s * p.lpr);
+        Angles<E> t;
+        t.load(p, l, pos);
+        const Coeffs<E> c(p, l, t, o.w);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            a[s][e] *= r;
+            b[s][e] *= r;
+        }
+        c.turn(p, l, a[s], b[s]);
+        if (l.u0 >= 0) *reinterpret_cast<Unit<T, E>*>(y + l.u0 * E) = Unit<T, E>(a[s]);
+        if (l.u1 >= 0) *reinterpret_cast<Unit<T, E>*>(y + l.u1 * E) = Unit<T, E>(b[s]);
+    }
+}
+
+// Many rows: a group of lanes takes U heads of a token (E = 8 elements a unit
+// for 16-bit types, 4 for f32: 16 bytes), all rows' loads before the first use.
+// Bound by the loads that three CTAs an SM keep in flight: 8191 tokens of 64 + 8
+// heads of 128 in bf16 take 88 us (3.4 TB/s read and written) with two heads a
+// group, 93 with four (fewer CTAs), 112 with one (the angles loaded for each).
+template <typename T, int U>
+__global__ void __launch_bounds__(256, 3) qk_norm_rope_rows_kernel(const __grid_constant__ RopeP p) {
+    constexpr int E = 16 / sizeof(T);
+    pdl_wait();
+    const int lane = threadIdx.x & 31, sl = lane & (p.lpr - 1);
+    const unsigned group = group_mask(p.lpr, lane);
+    const bool is_k = blockIdx.x >= p.q_ctas;
+    const Side<T> o(p, is_k);
+    const unsigned i = (blockIdx.x - (is_k ? p.q_ctas : 0)) * (256u >> p.lpr_log) + (threadIdx.x >> p.lpr_log);
+    const unsigned per = (unsigned)(o.heads + U - 1) / U;
+    const unsigned n = i / per;
+    if (n >= p.n) return;
+    const int h0 = (int)(i - n * per) * U, hn = min(U, o.heads - h0);
+    const Lane<E> l(p, sl);
+    const T* x = o.x + n * o.xt + h0 * o.xh;
+    T* y = o.y + n * o.yt + h0 * o.yh;
+    Unit<T, E> ra[U], rb[U];
 #pragma unroll
     for (int h = 0; h < U; h++)
         if (h < hn) {
-            const T* x = xr + h * p.xh[which];
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                if (u0[s] >= 0) ra[h][s] = *reinterpret_cast<const Unit<T, E>*>(x + u0[s] * E);
-                if (u1[s] >= 0) rb[h][s] = *reinterpret_cast<const Unit<T, E>*>(x + u1[s] * E);
-            }
+            if (l.u0 >= 0) ra[h] = *reinterpret_cast<const Unit<T, E>*>(x + h * o.xh + l.u0 * E);
+            if (l.u1 >= 0) rb[h] = *reinterpret_cast<const Unit<T, E>*>(x + h * o.xh + l.u1 * E);
         }
+    const int64_t pos = p.pos[n];
+    if (pos < 0 || pos >= p.max_pos) return;  // the rows stay as they were
+    Angles<E> t;
+    t.load(p, l, pos);
+    const Coeffs<E> c(p, l, t, o.w);
 #pragma unroll
     for (int h = 0; h < U; h++) {
         if (h >= hn) break;
-        T* y = yr + h * p.yh[which];
-        float a[S][E], b[S][E];
-        float ss = 0.0f;
+        float a[E], b[E];
 #pragma unroll
-        for (int s = 0; s < S; s++)
+        for (int e = 0; e < E; e++) {
+            a[e] = l.u0 >= 0 ? to_f32(ra[h].v[e]) : 0.0f;
+            b[e] = l.u1 >= 0 ? to_f32(rb[h].v[e]) : 0.0f;
+        }
+        if (o.w) {
+            float2 s2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int e = 0; e < E; e++) s2 = fma2(make_float2(a[e], b[e]), make_float2(a[e], b[e]), s2);
+            const float r = rsqrtf(fmaf(group_sum(s2.x + s2.y, p.lpr, group), p.inv_hd, p.eps));
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                a[s][e] = u0[s] >= 0 ? to_f32(ra[h][s].v[e]) : 0.0f;
-                b[s][e] = u1[s] >= 0 ? to_f32(rb[h][s].v[e]) : 0.0f;
+                const float2 v = mul2(make_float2(a[e], b[e]), make_float2(r, r));
+                a[e] = v.x;
+                b[e] = v.y;
             }
-        if (w) {
-#pragma unroll
-            for (int s = 0; s < S; s++)
-#pragma unroll
-                for (int e = 0; e < E; e++) ss = fmaf(a[s][e], a[s][e], fmaf(b[s][e], b[s][e], ss));
-            for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-            const float r = 1.0f / sqrtf(ss / (float)p.hd + p.eps);
-#pragma unroll
-            for (int s = 0; s < S; s++)
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    a[s][e] = a[s][e] * r * w0[s][e];
-                    b[s][e] = b[s][e] * r * w1[s][e];
-                }
         }
-#pragma unroll
-        for (int s = 0; s < S; s++) {
-            if (sl + s * lpr < P) {
-                if (E == 1 || !p.inter) {
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const float f = a[s][e], g = b[s][e];
-                        a[s][e] = f * c0[s][e] - g * s0[s][e];
-                        b[s][e] = f * s0[s][e] + g * c0[s][e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e + 1 < E; e += 2) {
-                        float f = a[s][e], g = a[s][e + 1];
-                        a[s][e] = f * c0[s][e / 2] - g * s0[s][e / 2];
-                        a[s][e + 1] = f * s0[s][e / 2] + g * c0[s][e / 2];
-                        f = b[s][e];
-                        g = b[s][e + 1];
-                        b[s][e] = f * c0[s][E / 2 + e / 2] - g * s0[s][E / 2 + e / 2];
-                        b[s][e + 1] = f * s0[s][E / 2 + e / 2] + g * c0[s][E / 2 + e / 2];
-                    }
-                }
-            }
-            if (u0[s] >= 0) *reinterpret_cast<Unit<T, E>*>(y + u0[s] * E) = Unit<T, E>(a[s]);
-            if (u1[s] >= 0) *reinterpret_cast<Unit<T, E>*>(y + u1[s] * E) = Unit<T, E>(b[s]);
-        }
+        c.turn(p, l, a, b);
+        if (l.u0 >= 0) *reinterpret_cast<Unit<T, E>*>(y + h * o.yh + l.u0 * E) = Unit<T, E>(a);
+        if (l.u1 >= 0) *reinterpret_cast<Unit<T, E>*>(y + h * o.yh + l.u1 * E) = Unit<T, E>(b);
     }
 }
 
@@ -319,7 +435,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(const __grid_c
             for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffu << (lane & 16), ss, o);
-            const float s = 1.0f / sqrtf(ss / (float)hd + p.r.eps);
+            const float s = rsqrtf(fmaf(ss, p.r.inv_hd, p.r.eps));
             if (mine)
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = x[i] * s * w[8 * sl + i];
@@ -422,6 +538,7 @@ RopeP rope_params(const rq_qk_rope* a) {
     p.heads[0] = (int)a->n_heads;
     p.heads[1] = (int)a->n_kv_heads;
     p.hd = (int)a->head_dim;
+    p.inv_hd = 1.0f / (float)p.hd;
     p.rot = (int)a->rot_dim;
     p.inter = a->interleaved != 0;
     p.eps = a->eps;
@@ -430,6 +547,27 @@ RopeP rope_params(const rq_qk_rope* a) {
 
 int check_grid(int64_t blocks, const char* fn) {
     return blocks > INT32_MAX ? set_error(RQ_ERR_INVALID, "%s: too many rows for one call", fn) : RQ_OK;
+}
+
+template <typename T>
+const void* append_fn(int nb) {
+    return nb == 1   ? (const void*)kv4_append_kernel<T, 1>
+           : nb == 2 ? (const void*)kv4_append_kernel<T, 2>
+           : nb == 3 ? (const void*)kv4_append_kernel<T, 3>
+                     : (const void*)kv4_append_kernel<T, 4>;
+}
+const void* append_fn(int dtype, int nb) {
+    return dtype == RQ_F32 ? append_fn<float>(nb) : dtype == RQ_F16 ? append_fn<__half>(nb) : append_fn<__nv_bfloat16>(nb);
+}
+template <typename T>
+const void* read_fn(int nb) {
+    return nb == 1   ? (const void*)kv4_read_kernel<T, 1>
+           : nb == 2 ? (const void*)kv4_read_kernel<T, 2>
+           : nb == 3 ? (const void*)kv4_read_kernel<T, 3>
+                     : (const void*)kv4_read_kernel<T, 4>;
+}
+const void* read_fn(int dtype, int nb) {
+    return dtype == RQ_F32 ? read_fn<float>(nb) : dtype == RQ_F16 ? read_fn<__half>(nb) : read_fn<__nv_bfloat16>(nb);
 }
 
 // Tokens of an append or read CTA: about four items a thread where the tokens
@@ -467,35 +605,38 @@ AppendP append_params(const rq_kv4* c, const void* k, int64_t kt, int64_t kh, co
 int qk_norm_rope(const rq_ctx* ctx, const rq_qk_rope* a, cudaStream_t st) {
     RopeP p = rope_params(a);
     const size_t size = dtype_size(a->dtype);
-    const int wide = (int)(16 / size);
-    bool vec = p.hd % wide == 0 && p.rot % (2 * wide) == 0;
+    // units of E elements: 16 bytes for many rows, four elements for few (twice
+    // the lanes for 16-bit types), one where sizes or alignment ask for it
+    auto fits = [&](int e) { return p.hd % e == 0 && p.rot % (2 * e) == 0; };
+    bool vec = fits(4);
     for (int i = 0; i < 2; i++)
-        if (p.heads[i]) vec = vec && wide_ok(p.x[i], p.xt[i], p.xh[i], size) && wide_ok(p.y[i], p.yt[i], p.yh[i], size);
-    const int E = vec ? wide : 1;
+        if (p.heads[i])
+            vec = vec && wide_ok(p.x[i], p.xt[i], p.xh[i], size) && wide_ok(p.y[i], p.yt[i], p.yh[i], size) &&
+                  ((uintptr_t)p.w[i] & 15) == 0;
+    vec = vec && (((uintptr_t)p.cos | (uintptr_t)p.sin) & 15) == 0;
+    const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
+    if (rows > INT32_MAX) return set_error(RQ_ERR_INVALID, "rq_qk_norm_rope: too many rows for one call");
+    const bool many = vec && fits((int)(16 / size)) && rows * (p.hd / 8) > 2 * (int64_t)ctx->sm_count * 2048;
+    const int E = many ? (int)(16 / size) : vec ? 4 : 1, U = many ? kRopeRows : 1;
     const int slots = p.rot / (2 * E) + ((p.hd - p.rot) / E + 1) / 2;
     p.lpr = 1;
     for (; p.lpr < slots && p.lpr < 32; p.lpr *= 2) p.lpr_log++;
-    const int64_t rows = p.n * (p.heads[0] + p.heads[1]);
-    // one head a group while the rows do not fill the device's threads, else
-    // four (8191 tokens, 64 + 8 heads of 128, bf16: 112 -> XX us)
-    const bool four = vec && rows * p.lpr > (int64_t)ctx->sm_count * 2048;
-    const int U = four ? 4 : 1;
-    const int gq = (p.heads[0] + U - 1) / U, gk = (p.heads[1] + U - 1) / U;
-    const int64_t blocks = (p.n * (gq + gk) * p.lpr + 255) / 256;
-    if (p.n * (gq + gk) > INT32_MAX) return set_error(RQ_ERR_INVALID, "rq_qk_norm_rope: too many rows for one call");
+    const int64_t groups = 256 >> p.lpr_log;
+    p.q_ctas = (unsigned)((p.n * ((p.heads[0] + U - 1) / U) + groups - 1) / groups);
+    const int64_t blocks = p.q_ctas + (p.n * ((p.heads[1] + U - 1) / U) + groups - 1) / groups;
     const void* fn;
     if (a->dtype == RQ_F32)
-        fn = four  ? (const void*)qk_norm_rope_kernel<float, 4, 1, 4>
-             : vec ? (const void*)qk_norm_rope_kernel<float, 4, 1, 1>
-                   : (const void*)qk_norm_rope_kernel<float, 1, 4, 1>;
+        fn = many  ? (const void*)qk_norm_rope_rows_kernel<float, kRopeRows>
+             : vec ? (const void*)qk_norm_rope_kernel<float, 4, 1>
+                   : (const void*)qk_norm_rope_kernel<float, 1, 4>;
     else if (a->dtype == RQ_F16)
-        fn = four  ? (const void*)qk_norm_rope_kernel<__half, 8, 1, 4>
-             : vec ? (const void*)qk_norm_rope_kernel<__half, 8, 1, 1>
-                   : (const void*)qk_norm_rope_kernel<__half, 1, 4, 1>;
+        fn = many  ? (const void*)qk_norm_rope_rows_kernel<__half, kRopeRows>
+             : vec ? (const void*)qk_norm_rope_kernel<__half, 4, 1>
+                   : (const void*)qk_norm_rope_kernel<__half, 1, 4>;
     else
-        fn = four  ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1, 4>
-             : vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 8, 1, 1>
-                   : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4, 1>;
+        fn = many  ? (const void*)qk_norm_rope_rows_kernel<__nv_bfloat16, kRopeRows>
+             : vec ? (const void*)qk_norm_rope_kernel<__nv_bfloat16, 4, 1>
+                   : (const void*)qk_norm_rope_kernel<__nv_bfloat16, 1, 4>;
     void* args[] = {&p};
     return launch_pdl(fn, (unsigned)blocks, 256, 0, st, args, "q/k norm and rotation kernel");
 }
@@ -597,9 +738,7 @@ int rq_kv4_append(rq_kv4* c, int dtype, const void* k, const int64_t k_stride[2]
     const int64_t blocks = (n + p.per_cta - 1) / p.per_cta;
     rc = check_grid(blocks, "rq_kv4_append");
     if (rc) return rc;
-    const void* fn = dtype == RQ_F32 ? (const void*)kv4_append_kernel<float>
-                     : dtype == RQ_F16 ? (const void*)kv4_append_kernel<__half>
-                                       : (const void*)kv4_append_kernel<__nv_bfloat16>;
+    const void* fn = append_fn(dtype, c->head_dim / 32);
     void* args[] = {&p};
     return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "kv4 append kernel");
 }
@@ -623,7 +762,6 @@ int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, void* k, 
     p.n_slots = c->n_pages * c->page_size;
     p.page_size = c->page_size;
     p.n_kv = c->n_kv;
-    p.nb = c->head_dim / 32;
     p.x[0] = k;
     p.x[1] = v;
     p.wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
@@ -631,9 +769,7 @@ int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, void* k, 
     const int64_t blocks = (n + p.per_cta - 1) / p.per_cta;
     rc = check_grid(blocks, "rq_kv4_read");
     if (rc) return rc;
-    const void* fn = dtype == RQ_F32 ? (const void*)kv4_read_kernel<float>
-                     : dtype == RQ_F16 ? (const void*)kv4_read_kernel<__half>
-                                       : (const void*)kv4_read_kernel<__nv_bfloat16>;
+    const void* fn = read_fn(dtype, c->head_dim / 32);
     void* args[] = {&p};
     return launch_pdl(fn, (unsigned)blocks, 256, 0, (cudaStream_t)stream, args, "kv4 read kernel");
 }

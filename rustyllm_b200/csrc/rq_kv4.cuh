@@ -83,6 +83,30 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// two f32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // 8 consecutive elements as f32; `wide`: p is 16-byte aligned
 template <typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, bool wide, float (&x)[8]) {
@@ -118,58 +142,65 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
     return c;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float c;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
 
 // The four lanes of an aligned group hold a block, 8 elements each.  Returns
 // the block's scale (f16 value in f32) and this lane's 8 codes.  d = f16(m /
 // -8), m the element of the largest magnitude (the lowest index of equals); m /
 // 8 is exact, so d is one rounding.  A code is the nearest multiple of d (ties
-// to the higher code).  x * (1 / d) is within 2^-20 of x / d where |x / d| <= 8,
-// so rounding it decides all but what lies that near to a half; there (rare,
-// but for 16-bit inputs exact ties are not) the comparison of x with (c - 8.5) d
-// decides, a product of at most 16 bits and so exact in f32.  A NaN makes the
-// scale NaN (the block reads back as NaN); infinities saturate it at 65504.
+// to the higher code): k = rint(x / d) by an approximate quotient is off by one
+// at most, and what is left, r = x - k d (k d has at most 15 bits), compares with
+// d / 2 exactly, whatever the quotient's rounding.  A NaN makes the scale NaN
+// (the block reads back as NaN); infinities saturate it at 65504.
 __device__ __forceinline__ float kv4_quantize(const float (&x)[8], uint32_t (&c)[8]) {
-    float big = fabsf(x[0]);
+    float top = x[0], low = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) big = max_nan(big, fabsf(x[i]));
+    for (int i = 1; i < 8; i++) {
+        top = max_nan(top, x[i]);
+        low = min_nan(low, x[i]);
+    }
     const unsigned lane = threadIdx.x & 31;
     const unsigned group = 0xFu << (lane & 28);
-    big = max_nan(big, __shfl_xor_sync(group, big, 1));
-    big = max_nan(big, __shfl_xor_sync(group, big, 2));
-    float m = x[7];
-    bool here = fabsf(x[7]) == big;
 #pragma unroll
-    for (int i = 6; i >= 0; i--) {
-        const bool is = fabsf(x[i]) == big;
-        m = is ? x[i] : m;
-        here |= is;
+    for (int o = 1; o <= 2; o <<= 1) {
+        top = max_nan(top, __shfl_xor_sync(group, top, o));
+        low = min_nan(low, __shfl_xor_sync(group, low, o));
     }
-    const unsigned who = __ballot_sync(group, here) & group;
-    m = __shfl_sync(group, m, who ? __ffs((int)who) - 1 : (int)lane);
+    float m = top > -low ? top : low;
+    if (top == -low) {  // both signs reach it: the first element decides
+        int first = 8;  // 2 * index + (negative)
+#pragma unroll
+        for (int i = 7; i >= 0; i--)
+            if (fabsf(x[i]) == top) first = 2 * i + (x[i] < 0.0f ? 1 : 0);
+        bool here = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) here |= fabsf(x[i]) == top;
+        const unsigned who = __ballot_sync(group, here) & group;
+        if (__shfl_sync(group, first, who ? __ffs((int)who) - 1 : (int)lane) & 1) m = low;
+        else m = top;
+    }
     const float d = __half2float(__float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f)));
-    if (!(big == big) || d == 0.0f) {
+    if (!(top == top) || d == 0.0f) {
 #pragma unroll
         for (int i = 0; i < 8; i++) c[i] = 8;
-        return big == big ? d : __int_as_float(0x7fffffff);
+        return top == top ? d : __int_as_float(0x7fffffff);
     }
-    const float inv = 1.0f / d;
-    bool near_half = false;
+    // with the sign of d taken into x
+    const uint32_t sign = __float_as_uint(d) & 0x80000000u;
+    const float D = fabsf(d), inv = __frcp_rn(D), half = 0.5f * D;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float v = fminf(fmaxf(x[i] * inv, -8.0f), 7.0f);
-        const float z = v + 12582912.0f;  // 1.5 * 2^23: rounds v to an integer in the low bits
-        near_half |= fabsf(v - (z - 12582912.0f)) > 0.499996f;
-        c[i] = (__float_as_uint(z) + 8u) & 15u;
-    }
-    if (near_half) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float t = fminf(fmaxf(floorf(x[i] * inv + 8.5f), 0.0f), 15.0f);
-            const float lo = (t - 8.5f) * d, hi = (t - 7.5f) * d;
-            if (t > 0.0f && (d > 0.0f ? x[i] < lo : x[i] > lo)) t -= 1.0f;
-            else if (t < 15.0f && (d > 0.0f ? x[i] >= hi : x[i] <= hi)) t += 1.0f;
-            c[i] = (uint32_t)t;
-        }
+        const float v = __uint_as_float(__float_as_uint(x[i]) ^ sign);
+        const float z = fmaf(v, inv, 12582912.0f);  // 1.5 * 2^23: an integer in the low bits
+        const float r = fmaf(12582912.0f - z, D, v);
+        int k = __float_as_int(z) - 0x4B400000 + 8;
+        if (r >= half) k++;
+        if (r < -half) k--;
+        c[i] = (uint32_t)min(max(k, 0), 15);
     }
     return d;
 }

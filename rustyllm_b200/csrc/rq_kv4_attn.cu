@@ -101,22 +101,6 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two f32 operations an instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 // nibbles 0 and 4 (even) or 1 and 5 (odd) of w as f16 pairs c - 8: a nibble
@@ -1198,6 +1182,9 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
         const int64_t pairs = a->batch * c->n_kv * tiles_of_row * (std::max<int64_t>((tiles + 1) / 2, 1) + kHead);
         const int64_t places = sms * (c->head_dim > 64 ? kPerSm<4> : kPerSm<2>);
         pl.ctas = std::max<int64_t>(1, std::min(places, pairs / (kWarps + 1)));
+        // units of one length (a single sequence's) then begin where CTAs do
+        const int64_t units = a->batch * c->n_kv * tiles_of_row;
+        if (pl.ctas > units) pl.ctas -= pl.ctas % units;
         pl.pieces = pl.ctas > 1 ? 2 * pl.ctas * pl.R : 0;
         return pl;
     }

@@ -114,16 +114,38 @@ __global__ void __launch_bounds__(kThreads) pages_extend_kernel(const __grid_con
             const int b = owner(pg, n, i);
             p.table[(b0 + b) * p.table_stride + held[b] + (i - pg[b])] = taken(pg0 + i);
         }
-        for (int64_t i = me; i < tok[n]; i += step) {
-            if (tok0 + i >= p.n_tokens) break;
-            const int b = owner(tok, n, i);
-            const int64_t pos = ctx[b] + (i - tok[b]), col = pos / ps;
-            int32_t page = -1;
-            if (col < held[b]) page = p.table[(b0 + b) * p.table_stride + col];
-            else if (col < p.table_width) page = taken(pg0 + pg[b] + (col - held[b]));
-            p.positions[tok0 + i] = (int32_t)min(pos, (int64_t)INT32_MAX);
-            const int64_t slot = (int64_t)page * ps + pos % ps;
-            p.slots[tok0 + i] = page < 0 || slot > INT32_MAX ? -1 : (int32_t)slot;
+        // token rows: a warp takes a run of them, so that a lane bisects once and
+        // then walks; four pages at a time are on their way
+        {
+            const int64_t all = min(tok[n], max(p.n_tokens - tok0, (int64_t)0)), warps = step / 32;
+            const int64_t run = ((all + warps - 1) / warps + 127) & ~(int64_t)127;
+            const int64_t i0 = me / 32 * run, i1 = min(i0 + run, all);
+            int b = i0 < i1 ? owner(tok, n, min(i0 + (tid & 31), all - 1)) : 0;
+            for (int64_t i = i0 + (tid & 31); i < i1; i += 128) {
+                int32_t pos[4], off[4], page[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int64_t at = i + 32 * x;
+                    page[x] = -1;
+                    pos[x] = off[x] = 0;
+                    if (at >= i1) continue;
+                    while (tok[b + 1] <= at) b++;
+                    const int64_t ps64 = ctx[b] + (at - tok[b]);
+                    pos[x] = (int32_t)min(ps64, (int64_t)INT32_MAX);
+                    const int64_t col = (uint32_t)pos[x] / (uint32_t)p.page_size;
+                    off[x] = (int32_t)(pos[x] - col * ps);
+                    if (col < held[b]) page[x] = p.table[(b0 + b) * p.table_stride + col];
+                    else if (col < p.table_width) page[x] = taken(pg0 + pg[b] + (col - held[b]));
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int64_t at = i + 32 * x;
+                    if (at >= i1) continue;
+                    const int64_t slot = (int64_t)page[x] * ps + off[x];
+                    p.positions[tok0 + at] = pos[x];
+                    p.slots[tok0 + at] = page[x] < 0 || slot > INT32_MAX ? -1 : (int32_t)slot;
+                }
+            }
         }
         tok0 += tok[n];
         pg0 += pg[n];

@@ -72,36 +72,46 @@ __global__ void __launch_bounds__(kThreads) spec_verify_kernel(const __grid_cons
     pdl_wait();
     __shared__ double sums[kMaxGroups];
     __shared__ double total_s;   // this CTA's mass, read by the cluster
-    __shared__ int s_acc;
+    __shared__ int s_acc, s_n;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % p.ctas);
     const int64_t b = blockIdx.x / p.ctas;
     const T* P = static_cast<const T*>(p.p) + b * p.ps;
     const T* Q = p.q ? static_cast<const T*>(p.q) + b * p.qs : nullptr;
     const int32_t* drafts = p.drafts + b * p.max_drafts;
-    const int n = p.n_drafts ? min(max(p.n_drafts[b], 0), p.max_drafts) : p.max_drafts;
-    // ---- accepted drafts (every CTA by itself)
+    // ---- accepted drafts (every CTA by itself).  The first 32 drafts and their
+    // numbers are loaded beside the count, not behind it.
     if (warp == 0) {
+        int32_t x0 = 0;
+        float u0 = 0.0f;
+        if (lane < p.max_drafts) {
+            x0 = drafts[lane];
+            u0 = p.u[b * p.max_drafts + lane];
+        }
+        const int n = p.n_drafts ? min(max(p.n_drafts[b], 0), p.max_drafts) : p.max_drafts;
         int acc = n;
         for (int i0 = 0; i0 < n && acc == n; i0 += 32) {
             const int i = i0 + lane;
             bool good = true;
             if (i < n) {
-                const int64_t x = drafts[i];
+                const int64_t x = i0 ? drafts[i] : x0;
                 good = x >= 0 && x < p.vocab;
                 if (good) {
                     const double px = mass(to_f32(P[i * p.pr + x]));
                     const double qx = Q ? mass(to_f32(Q[i * p.qr + x])) : 1.0;
-                    good = (double)p.u[b * p.max_drafts + i] * qx < px;
+                    good = (double)(i0 ? p.u[b * p.max_drafts + i] : u0) * qx < px;
                 }
             }
             const unsigned no = __ballot_sync(0xffffffffu, !good);
             if (no) acc = i0 + __ffs((int)no) - 1;
         }
-        if (lane == 0) s_acc = acc;
+        if (lane == 0) {
+            s_acc = acc;
+            s_n = n;
+        }
     }
     __syncthreads();
-    const int acc = s_acc;
+    const int acc = s_acc, n = s_n;
     Row w{P + (int64_t)acc * p.pr, nullptr, -1};
     bool leftover = acc < n;
     if (leftover) {
