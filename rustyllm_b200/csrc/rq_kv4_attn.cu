@@ -27,9 +27,10 @@
 //    its operands are built in registers from the record that one bulk copy
 //    brought to shared memory.  The warps join through shared memory, the
 //    pieces of a unit that went to several CTAs through a second launch.
-//  - many rows (prompts): the warps hold different rows; each turns one record
-//    into f16 operands in shared memory and all use them, which takes the
-//    unpacking (144 of about 340 instructions a tile) off three of four warps.
+//  - many rows (prompts): the warps hold different rows, two operand tiles each;
+//    the records are turned into f16 operands in shared memory once for all
+//    four, and an operand read from there serves two tiles of rows (with one
+//    tile a warp, reading them took as long as the products).
 #include <algorithm>
 
 #include "rq_async.cuh"
@@ -186,15 +187,18 @@ __device__ __forceinline__ void unit_tiles(const AttnP& p, const Rows& o, int& t
     per = max((tile1 - tile0 + 2 * p.splits - 1) / (2 * p.splits), kWarps) * 2;  // of a split, whole pairs
 }
 
-// One warp's query rows, running sums and the work on one tile.
-template <int NB, int MODE, typename T>
+// One warp's query rows, running sums and the work on one tile.  MT operand
+// tiles of rows: one, its query operands in registers, or two, theirs in shared
+// memory (`as`: [MT][NB][2][32 lanes]).
+template <int NB, int MODE, typename T, int MT>
 struct Warp {
-    static constexpr int R = MODE == kOne16 ? 16 : 8;
-    static constexpr int H = MODE == kOne16 ? 2 : 1;  // rows a lane
-    uint32_t aq[NB][2][4];
+    static constexpr int R1 = MODE == kOne16 ? 16 : 8, R = R1 * MT;
+    static constexpr int HH = MODE == kOne16 ? 2 : 1, H = HH * MT;  // rows a lane: of an operand tile, in all
+    uint32_t aq[MT == 1 ? NB : 1][2][4];
+    uint4* as;
     float qs[H];      // back from the normalised row, times the softmax scale
     int rpos[H];      // position of the row's query; -1: no row
-    float oacc[NB][4][4];
+    float oacc[MT][NB][4][4];
     float m[H], l[H];
     float E;
     float bound;      // 2^E
@@ -202,10 +206,14 @@ struct Warp {
     int full0, full1;      // tiles that every row sees whole
     int seen;              // positions that any row sees end here
 
+    // row of lane group g's h-th
+    static __device__ __forceinline__ int row_of(int g, int h) { return (h / HH) * R1 + g + 8 * (h % HH); }
+
     __device__ __forceinline__ void init(const AttnP& p, const Rows& o, int r0, int g, int t) {
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            const int r = r0 + g + 8 * h;
+            const int mt = h / HH, hh = h % HH;
+            const int r = r0 + row_of(g, h);
             const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
             const int64_t tok = (int64_t)o.q0 + i;
             const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
@@ -239,23 +247,29 @@ struct Warp {
                     for (int j = 0; j < 2; j++) {  // elements 4 s + 2 j, + 1: operand half j of step s
                         const float f0 = x[b][4 * s + 2 * j] * down, f1 = x[b][4 * s + 2 * j + 1] * down;
                         const uint32_t hi = pack(f0, f1);
-                        if (MODE == kOne16) {
-                            aq[b][s][2 * j + h] = hi;
+                        const float2 back = unpack(hi);
+                        const uint32_t lo = MODE == kOne16 ? 0u : pack(f0 - back.x, f1 - back.y);
+                        if constexpr (MT > 1) {
+                            uint32_t* at = reinterpret_cast<uint32_t*>(as + ((mt * NB + b) * 2 + s) * 32 + 4 * g + t);
+                            at[2 * j + hh] = hi;
+                            if (MODE != kOne16) at[2 * j + 1] = lo;
                         } else {
-                            const float2 back = unpack(hi);
-                            aq[b][s][2 * j] = hi;
-                            aq[b][s][2 * j + 1] = pack(f0 - back.x, f1 - back.y);
+                            aq[b][s][2 * j + hh] = hi;
+                            if (MODE != kOne16) aq[b][s][2 * j + 1] = lo;
                         }
                     }
             m[h] = -INFINITY;
             l[h] = 0.0f;
         }
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int n = 0; n < 4; n++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) oacc[b][n][i] = 0.0f;
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) oacc[mt][b][n][i] = 0.0f;
+        __syncwarp();  // the operands in shared memory are there
         set_scale(-15);
         const int i0 = r0 / p.group, i1 = min(o.n_q - 1, (r0 + R - 1) / p.group);
         full1 = max(0, min(o.held, o.pos0 + i0 + 1)) / kKv4Tile;
@@ -269,17 +283,19 @@ struct Warp {
         inv = __float2half2_rn(__int_as_float((127 - e) << 23));
     }
     __device__ __forceinline__ void scale_rows(const float (&f)[H]) {
-        // rows g and g + 8 of the accumulators: in the 8-row modes both
-        // halves belong to row g
+        // rows g and g + 8 of an accumulator: in the 8-row mode both halves
+        // belong to row g
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                oacc[b][n][0] *= f[0];
-                oacc[b][n][1] *= f[0];
-                oacc[b][n][2] *= f[H - 1];
-                oacc[b][n][3] *= f[H - 1];
-            }
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    oacc[mt][b][n][0] *= f[mt * HH];
+                    oacc[mt][b][n][1] *= f[mt * HH];
+                    oacc[mt][b][n][2] *= f[mt * HH + HH - 1];
+                    oacc[mt][b][n][3] *= f[mt * HH + HH - 1];
+                }
     }
 
     // NT tiles at tile_at, + 1 that the operand source `src` holds:
@@ -293,32 +309,79 @@ struct Warp {
     __device__ __forceinline__ void tiles(const AttnP& p, int tile_at, int t, Src& src) {
         float2 sc[NT][2][H];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            src.k(i);
+        for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
+            for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int h = 0; h < H; h++) sc[i][n][h] = make_float2(0.0f, 0.0f);
-                float c[NB][4];  // all blocks' first steps, then the second ones: no product waits for the one before
-                uint4 w[NB];
+        auto add = [&](float2 (&to)[H], int mt, const float (&c)[4], float2 d) {
+            const float2 lo = make_float2(c[0], c[1]), hi = make_float2(c[2], c[3]);
+            if (MODE == kOne16) {
+                to[mt * HH] = fma2(lo, d, to[mt * HH]);
+                to[mt * HH + HH - 1] = fma2(hi, d, to[mt * HH + HH - 1]);
+            } else {
+                to[mt] = fma2(add2(lo, hi), d, to[mt]);
+            }
+        };
+        if constexpr (MT == 1) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    w[b] = src.kop(i, n, b);
-                    mma16816_0(c[b], aq[b][0], w[b].x, w[b].y);
-                }
+            for (int i = 0; i < NT; i++) {
+                src.k(i);
 #pragma unroll
-                for (int b = 0; b < NB; b++) mma16816(c[b], aq[b][1], w[b].z, w[b].w);
+                for (int n = 0; n < 2; n++) {
+                    float c[NB][4];  // all blocks' first steps, then the second ones: no product waits for the one before
+                    uint4 w[NB];
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const float2 d = unpack(src.ksc(i, n, b));
-                    const float2 lo = make_float2(c[b][0], c[b][1]), hi = make_float2(c[b][2], c[b][3]);
-                    if (MODE == kOne16) {
-                        sc[i][n][0] = fma2(lo, d, sc[i][n][0]);
-                        sc[i][n][H - 1] = fma2(hi, d, sc[i][n][H - 1]);
-                    } else {
-                        sc[i][n][0] = fma2(add2(lo, hi), d, sc[i][n][0]);
+                    for (int b = 0; b < NB; b++) {
+                        w[b] = src.kop(i, n, b);
+                        mma16816_0(c[b], aq[b][0], w[b].x, w[b].y);
                     }
+#pragma unroll
+                    for (int b = 0; b < NB; b++) mma16816(c[b], aq[b][1], w[b].z, w[b].w);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) add(sc[i][n], 0, c[b], unpack(src.ksc(i, n, b)));
                 }
+            }
+        } else {
+            // block by block, so that its query operands are fetched once for
+            // all tiles
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t a[MT][2][4];
+                float c[MT][NT][2][4];
+                uint4 w[NT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const uint4 v = as[((mt * NB + b) * 2 + s) * 32 + (threadIdx.x & 31)];
+                        a[mt][s][0] = v.x;
+                        a[mt][s][1] = v.y;
+                        a[mt][s][2] = v.z;
+                        a[mt][s][3] = v.w;
+                    }
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        w[i][n] = src.kop(i, n, b);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) mma16816_0(c[mt][i][n], a[mt][0], w[i][n].x, w[i][n].y);
+                    }
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) mma16816(c[mt][i][n], a[mt][1], w[i][n].z, w[i][n].w);
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float2 d = unpack(src.ksc(i, n, b));
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) add(sc[i][n], mt, c[mt][i][n], d);
+                    }
             }
         }
         uint2 vs[NT][NB];
@@ -414,7 +477,7 @@ struct Warp {
         }
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            uint32_t ph[H][2], pl[2], nh[2];
+            uint32_t ph[H][2], pl[MT][2], nh[MT][2];
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 const float base = m[h] == -INFINITY ? 0.0f : m[h];
@@ -426,8 +489,8 @@ struct Warp {
                     ph[h][x] = pack(pr[i][h][2 * x], pr[i][h][2 * x + 1]);
                     if (MODE == kSplit8) {
                         const float2 back = unpack(ph[h][x]);
-                        pl[x] = pack(back.x - pr[i][h][2 * x], back.y - pr[i][h][2 * x + 1]);  // -pl
-                        nh[x] = ph[h][x] ^ 0x80008000u;
+                        pl[h / HH][x] = pack(back.x - pr[i][h][2 * x], back.y - pr[i][h][2 * x + 1]);  // -pl
+                        nh[h / HH][x] = ph[h][x] ^ 0x80008000u;
                     }
                 }
             }
@@ -435,37 +498,35 @@ struct Warp {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const __half2 d01 = __hmul2(as_h2(vs[i][b].x), inv), d23 = __hmul2(as_h2(vs[i][b].y), inv);
-                uint32_t a[4];
+                uint32_t a[MT][4];
 #pragma unroll
                 for (int h = 0; h < H; h++) {
+                    const int mt = h / HH, hh = h % HH;
                     const __half2 x = __hmul2(as_h2(ph[h][0]), d01), y = __hmul2(as_h2(ph[h][1]), d23);
-                    if (MODE == kOne16) {
-                        a[h] = as_u32(x);
-                        a[2 + h] = as_u32(y);
-                    } else {
-                        a[0] = as_u32(x);
-                        a[2] = as_u32(y);
+                    a[mt][hh] = as_u32(x);
+                    a[mt][2 + hh] = as_u32(y);
+                    if (MODE == kSplit8) {
                         // minus the low part, which spares the negations: value() subtracts
-                        a[1] = as_u32(__hfma2(as_h2(pl[0]), d01, __hfma2(as_h2(nh[0]), d01, x)));
-                        a[3] = as_u32(__hfma2(as_h2(pl[1]), d23, __hfma2(as_h2(nh[1]), d23, y)));
+                        a[mt][1] = as_u32(__hfma2(as_h2(pl[mt][0]), d01, __hfma2(as_h2(nh[mt][0]), d01, x)));
+                        a[mt][3] = as_u32(__hfma2(as_h2(pl[mt][1]), d23, __hfma2(as_h2(nh[mt][1]), d23, y)));
                     }
                     if constexpr (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
-                        if (MODE == kOne16) {
-                            a[h] &= see[i][h][0];
-                            a[2 + h] &= see[i][h][1];
-                        } else {
-                            a[0] &= see[i][h][0];
-                            a[1] &= see[i][h][0];
-                            a[2] &= see[i][h][1];
-                            a[3] &= see[i][h][1];
+                        a[mt][hh] &= see[i][h][0];
+                        a[mt][2 + hh] &= see[i][h][1];
+                        if (MODE == kSplit8) {
+                            a[mt][1] &= see[i][h][0];
+                            a[mt][3] &= see[i][h][1];
                         }
                     }
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const uint4 w = src.vop(i, b, half);
-                    mma16816(oacc[b][2 * half], a, w.x, w.y);
-                    mma16816(oacc[b][2 * half + 1], a, w.z, w.w);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma16816(oacc[mt][b][2 * half], a[mt], w.x, w.y);
+                        mma16816(oacc[mt][b][2 * half + 1], a[mt], w.z, w.w);
+                    }
                 }
             }
         }
@@ -496,10 +557,11 @@ struct Warp {
     }
     // elements 32 b + 8 n + 2 t, + 1 of row h
     __device__ __forceinline__ float2 value(int b, int n, int h) const {
-        float2 v = h ? make_float2(oacc[b][n][2], oacc[b][n][3]) : make_float2(oacc[b][n][0], oacc[b][n][1]);
+        const float(&o)[4] = oacc[h / HH][b][n];
+        float2 v = h % HH ? make_float2(o[2], o[3]) : make_float2(o[0], o[1]);
         if (MODE == kSplit8) {
-            v.x -= oacc[b][n][2];
-            v.y -= oacc[b][n][3];
+            v.x -= o[2];
+            v.y -= o[3];
         }
         return make_float2(v.x * bound, v.y * bound);
     }
@@ -769,7 +831,7 @@ struct Line {
 template <int NB, int MODE, typename T>
 __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using W = Warp<NB, MODE, T>;
+    using W = Warp<NB, MODE, T, 1>;
     constexpr int R = W::R, H = W::H, HD = 32 * NB, kThreads = kWarps * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
@@ -910,9 +972,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
 // stream.  Two warps share a stream: one unpacks its K, the other its V into
 // f16 operands that all four use.
 template <int NB, int MODE, typename T>
-__global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
+__global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using W = Warp<NB, MODE, T>;
+    using W = Warp<NB, MODE, T, 2>;
     constexpr int R = W::R, H = W::H, HD = 32 * NB, kLists = kWarps / 2;
     constexpr int kOps = SharedSrc<NB>::kOps;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -935,6 +997,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __g
     in.begin(o.b, o.kvh, t0 + 2 * list, t1);
     const int steps = t1 > t0 ? (t1 - t0 + kWarps - 1) / kWarps : 0;
     W w;
+    w.as = reinterpret_cast<uint4*>(scl + kWarps * 64 * NB + kLists * kStagesRows * 2 * Rec::kBytes) + warp * (2 * NB * 2 * 32);
     const int r0 = o.r0 + warp * R;
     w.init(p, o, r0, g, t);
     // tiles that this warp's rows see
@@ -992,7 +1055,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv4_attn_rows_kernel(const __g
     w.finish();
 #pragma unroll
     for (int h = 0; h < H; h++) {
-        const int r = r0 + g + 8 * h;
+        const int r = r0 + W::row_of(g, h);
         const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
         const int64_t tok = (int64_t)o.q0 + i;
         if (r >= o.rows || tok < 0 || tok >= p.n_tokens) continue;
@@ -1109,7 +1172,7 @@ Fns fns_of(bool rows) {
     constexpr int R = MODE == kOne16 ? 16 : 8;
     if constexpr (sizeof(T) == 4 || MODE == kOne16)  // 16-bit queries have no form of many rows in tiles of eight
         if (rows)
-            return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, R * kWarps, T>};
+            return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
     return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
 }
 template <int NB, typename T>
@@ -1188,12 +1251,12 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
         pl.pieces = pl.ctas > 1 ? 2 * pl.ctas * pl.R : 0;
         return pl;
     }
-    pl.R *= kWarps;
+    pl.R *= 2 * kWarps;
     pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
     const int64_t units = a->batch * c->n_kv * pl.row_tiles;
-    // splits of the long axis where the units leave the device's places (three
+    // splits of the long axis where the units leave the device's places (two
     // CTAs an SM) empty, none shorter than two steps
-    const int64_t want = sms * 3 / std::max<int64_t>(units, 1);
+    const int64_t want = sms * 2 / std::max<int64_t>(units, 1);
     pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / (2 * kWarps)));
     pl.ctas = units * pl.splits;
     pl.pieces = pl.splits > 1 ? a->n_tokens * a->n_heads * pl.splits : 0;
@@ -1254,7 +1317,7 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.magic = Magic{kEven, kOdd};
     p.err = err;
     const int nb = c->head_dim / 32;
-    const size_t smem = pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb)
+    const size_t smem = pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb + 2048 * nb)
                                 : (size_t)kWarps * (kStages * 2 * 576 * nb + pl.R * 32 * nb * 4);
     const Fns fn = fns_of(a->dtype, nb, pl.mode, pl.rows);
     if (smem > 48 * 1024) {
