@@ -97,6 +97,10 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// What sums kept relative to maximum m count relative to M, the largest: where
+// no position was seen m and M are -inf and the sums are zeros -- or not numbers,
+// if all scores were none, which have to stay so.
+__device__ __forceinline__ float weight(float m, float M) { return M > -INFINITY ? ex2(m - M) : 1.0f; }
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -190,11 +194,11 @@ __device__ __forceinline__ void unit_tiles(const AttnP& p, const Rows& o, int& t
 // One warp's query rows, running sums and the work on one tile.  MT operand
 // tiles of rows: one, its query operands in registers, or two, theirs in shared
 // memory (`as`: [MT][NB][2][32 lanes]).
-template <int NB, int MODE, typename T, int MT>
+template <int NB, int MODE, typename T, int MT, bool AS>
 struct Warp {
     static constexpr int R1 = MODE == kOne16 ? 16 : 8, R = R1 * MT;
     static constexpr int HH = MODE == kOne16 ? 2 : 1, H = HH * MT;  // rows a lane: of an operand tile, in all
-    uint32_t aq[MT == 1 ? NB : 1][2][4];
+    uint32_t aq[AS ? 1 : NB][2][4];
     uint4* as;
     float qs[H];      // back from the normalised row, times the softmax scale
     int rpos[H];      // position of the row's query; -1: no row
@@ -249,7 +253,7 @@ struct Warp {
                         const uint32_t hi = pack(f0, f1);
                         const float2 back = unpack(hi);
                         const uint32_t lo = MODE == kOne16 ? 0u : pack(f0 - back.x, f1 - back.y);
-                        if constexpr (MT > 1) {
+                        if constexpr (AS) {
                             uint32_t* at = reinterpret_cast<uint32_t*>(as + ((mt * NB + b) * 2 + s) * 32 + 4 * g + t);
                             at[2 * j + hh] = hi;
                             if (MODE != kOne16) at[2 * j + 1] = lo;
@@ -323,7 +327,7 @@ struct Warp {
                 to[mt] = fma2(add2(lo, hi), d, to[mt]);
             }
         };
-        if constexpr (MT == 1) {
+        if constexpr (!AS) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 src.k(i);
@@ -350,6 +354,7 @@ struct Warp {
                 uint32_t a[MT][2][4];
                 float c[MT][NT][2][4];
                 uint4 w[NT][2];
+                src.template kblock<NT>(b);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -649,16 +654,35 @@ struct Stream {
 };
 
 // Operands built in registers from the records of a pair
-template <int NB>
+template <int NB, bool kAS>
 struct RecordSrc {
     const uint8_t* rec;
     Magic magic;
     int lane, t, first = 0;
     uint32_t w[2 * NB];
+    uint32_t kb[2][4];  // K words of blocks b (even) and b + 1 of both tiles
+    template <int NT>
+    __device__ __forceinline__ void kblock(int b) {
+        if (b & 1) return;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            if (b + 1 < NB) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at(i) + (b >> 1) * 512 + lane * 16);
+                kb[i][0] = v.x;
+                kb[i][1] = v.y;
+                kb[i][2] = v.z;
+                kb[i][3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(at(i) + (b >> 1) * 512 + lane * 8);
+                kb[i][0] = v.x;
+                kb[i][1] = v.y;
+            }
+        }
+    }
     __device__ __forceinline__ const uint8_t* at(int i) const { return rec + (first + i) * Kv4Rec<NB>::kBytes; }
     __device__ __forceinline__ void k(int i) { load_words<NB>(at(i), lane, w); }
     __device__ __forceinline__ void v(int i) { load_words<NB>(at(i) + Kv4Rec<NB>::kV, lane, w); }
-    __device__ __forceinline__ uint4 kop(int, int n, int b) const { return k_operands(w[2 * b + n], magic); }
+    __device__ __forceinline__ uint4 kop(int i, int n, int b) const { return k_operands(kAS ? kb[i][2 * (b & 1) + n] : w[2 * b + n], magic); }
     __device__ __forceinline__ uint32_t ksc(int i, int n, int b) const {
         return *reinterpret_cast<const uint32_t*>(at(i) + Kv4Rec<NB>::kKs + t * 8 * NB + 8 * b + 4 * n);
     }
@@ -677,6 +701,8 @@ struct SharedSrc {
     int lane, t, first = 0;
     __device__ __forceinline__ void k(int) {}
     __device__ __forceinline__ void v(int) {}
+    template <int NT>
+    __device__ __forceinline__ void kblock(int) {}
     __device__ __forceinline__ uint4 kop(int i, int n, int b) const {
         return reinterpret_cast<const uint4*>(ops + (first + i) * kOps)[(2 * b + n) * 32 + lane];
     }
@@ -706,6 +732,8 @@ __device__ __forceinline__ void store2(T* p, bool pair, float a, float b) {
 // CTAs of an SM: what 168 (head_dim 96, 128) or 128 registers a thread allow
 template <int NB>
 constexpr int kPerSm = NB > 2 ? 3 : 4;
+template <int NB>
+constexpr bool kInShared = NB > 2;
 
 // Few rows.  The work is the line of all units' pairs of tiles (units in the
 // order of sequence, kv head, row tile), each unit headed by kHead empty places
@@ -831,7 +859,8 @@ struct Line {
 template <int NB, int MODE, typename T>
 __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using W = Warp<NB, MODE, T, 1>;
+    constexpr bool kAs = kInShared<NB>;
+    using W = Warp<NB, MODE, T, 1, kAs>;
     constexpr int R = W::R, H = W::H, HD = 32 * NB, kThreads = kWarps * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
@@ -870,7 +899,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
     }
     const uint8_t* ring = smem + warp * kStages * 2 * Rec::kBytes;
     Stream<kStages, Rec::kBytes, kWarps> in(p, smem_u32(ring), smem_u32(&bars[warp][0]), lane);
-    RecordSrc<NB> src;
+    RecordSrc<NB, kAs> src;
     src.lane = lane;
     src.t = t;
     src.magic = p.magic;
@@ -883,6 +912,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
         if (warp == 0) line.next(p, line.piece[turn ^ 1]);
         const Rows o(p, cur.b, cur.kvh, cur.r0);
         W w;
+        w.as = reinterpret_cast<uint4*>(joint + warp * (R * HD));  // this warp's part, free until the join
         w.init(p, o, o.r0, g, t);
         const int t0 = cur.t0;
         int s = 0;
@@ -903,7 +933,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
         }
         w.finish();
         // ---- join the warps: each one's m, l and row sums through shared
-        // memory, while the next piece's first copies are under way
+        // memory (where the query operands were), while the next piece's first
+        // copies are under way
+        if (kAs) __syncwarp();
         float* so = joint + warp * (R * HD);
 #pragma unroll
         for (int h = 0; h < H; h++) {
@@ -931,11 +963,11 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
             for (int x = 0; x < kWarps; x++) M = fmaxf(M, s_m[x][row]);
 #pragma unroll
             for (int x = 0; x < kWarps; x++) {
-                f[x] = M > -INFINITY ? ex2(s_m[x][row] - M) : 0.0f;
-                if (M > -INFINITY) L = fmaf(f[x], s_l[x][row], L);
+                f[x] = weight(s_m[x][row], M);
+                L = fmaf(f[x], s_l[x][row], L);
             }
             const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
-            const float scale = cur.whole && M > -INFINITY ? 1.0f / L : 1.0f;
+            const float scale = cur.whole && L != 0.0f ? 1.0f / L : 1.0f;
 #pragma unroll
             for (int x = 0; x < kWarps; x++) s_f[row][x] = f[x] * scale;
             s_at[row] = !ok ? -1 : cur.whole ? tok * p.ot + head * p.oh : ((int64_t)cur.slot * R + row) * HD;
@@ -974,7 +1006,7 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
 template <int NB, int MODE, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using W = Warp<NB, MODE, T, 2>;
+    using W = Warp<NB, MODE, T, 2, true>;
     constexpr int R = W::R, H = W::H, HD = 32 * NB, kLists = kWarps / 2;
     constexpr int kOps = SharedSrc<NB>::kOps;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1062,8 +1094,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
         if (p.splits == 1) {
             T* dst = static_cast<T*>(p.out) + tok * p.ot + head * p.oh + 2 * t;
             const bool two = ((uintptr_t)dst & 7) == 0;
-            const bool any = w.m[h] > -INFINITY;
-            const float f = any ? 1.0f / w.l[h] : 0.0f;
+            const bool any = w.l[h] != 0.0f;  // (not a number counts)
+            const float f = 1.0f / w.l[h];
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -1105,19 +1137,17 @@ __device__ __forceinline__ void join_row(const AttnP& p, int64_t dst, int used, 
     float L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (grp < groups) {
-        if (M > -INFINITY) {
 #pragma unroll 4
-            for (int s = grp; s < used; s += groups) {
-                const int64_t at = slot(s);
-                const float2 v = p.ml[at];
-                const float4 x = reinterpret_cast<const float4*>(p.part + at * (32 * NB))[e];
-                const float f = ex2(v.x - M);
-                L = fmaf(f, v.y, L);
-                acc.x = fmaf(f, x.x, acc.x);
-                acc.y = fmaf(f, x.y, acc.y);
-                acc.z = fmaf(f, x.z, acc.z);
-                acc.w = fmaf(f, x.w, acc.w);
-            }
+        for (int s = grp; s < used; s += groups) {
+            const int64_t at = slot(s);
+            const float2 v = p.ml[at];
+            const float4 x = reinterpret_cast<const float4*>(p.part + at * (32 * NB))[e];
+            const float f = weight(v.x, M);
+            L = fmaf(f, v.y, L);
+            acc.x = fmaf(f, x.x, acc.x);
+            acc.y = fmaf(f, x.y, acc.y);
+            acc.z = fmaf(f, x.z, acc.z);
+            acc.w = fmaf(f, x.w, acc.w);
         }
         s_o[grp][e] = acc;
         if (e == 0) s_l[grp] = L;
@@ -1130,7 +1160,7 @@ __device__ __forceinline__ void join_row(const AttnP& p, int64_t dst, int used, 
             l += s_l[i];
             sum += reinterpret_cast<const float*>(s_o[i])[tid];
         }
-        static_cast<T*>(p.out)[dst + tid] = from_f32<T>(M > -INFINITY ? sum / l : 0.0f);
+        static_cast<T*>(p.out)[dst + tid] = from_f32<T>(l != 0.0f ? sum / l : 0.0f);
     }
 }
 // Few rows: CTA i R + row joins row `row` of the unit that starts in CTA i.

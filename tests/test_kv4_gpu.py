@@ -198,7 +198,7 @@ def test_attention_matches_the_formula(gen, kind, H, kv, hd, page, lens, qs, win
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("qn", [1, 4])
+@pytest.mark.parametrize("qn", [1, 4, 40])
 def test_long_sequence_is_split_and_joined(gen, kind, qn):
     from rustyllm_b200.kv4 import KV4Cache
     cache = KV4Cache(320, 32, 2, 64)
@@ -232,6 +232,119 @@ def test_hidden_positions_do_not_enter(gen):
     want = attention_ref(q.double().cpu().numpy(), kval, vval, table.cpu().numpy(), 16, lens, cu, 0.125, 0, 8)
     close(out[[0, 1, 3]], want, [0, 1, 3], "f32")
     assert out[2].isnan().all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("B,most_q,most", [(300, 1, 90), (150, 3, 40), (129, 1, 700)])
+def test_batches_of_many_sequences(gen, kind, B, most_q, most):
+    """More sequences than a CTA looks up at a time, of all lengths, some of
+    them empty and some without queries; the pieces of the line begin and end
+    anywhere."""
+    from rustyllm_b200.kv4 import KV4Cache
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, most + 1, B)
+    lens[rng.random(B) < 0.2] = 0
+    lens[5] = 10 * most
+    qs = np.ones(B, int) if most_q == 1 else rng.integers(0, most_q + 1, B)
+    width = (10 * most + 15) // 16
+    cache = KV4Cache(width + 40, 16, 2, 32)
+    kval, vval = fill(cache, gen, kind)
+    table = torch.randint(0, cache.n_pages, (B, width), generator=gen, device="cuda").to(torch.int32)
+    cu = np.concatenate([[0], np.cumsum(qs)]).astype(np.int32)
+    q = torch.randn(int(cu[-1]), 8, 32, generator=gen, device="cuda").to(TYPES[kind])
+    want = attention_ref(q.double().cpu().numpy(), kval, vval, table.cpu().numpy(), 16, lens, cu, 32 ** -0.5, 0, cache.n_pages)
+    got = cache.attention(q, table, torch.from_numpy(lens.astype(np.int32)).cuda(),
+                          cu_q=None if most_q == 1 else torch.from_numpy(cu).cuda(), max_q=most_q)
+    close(got, want, slice(None), kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_prompts_over_missing_pages_and_odd_rows(gen, kind):
+    """The many-rows form: pages outside the cache, not-a-number blocks that
+    only later queries see, a query row that is not a number, and rows behind
+    n_tokens."""
+    from rustyllm_b200.kv4 import KV4Cache
+    cache = KV4Cache(40, 16, 2, 64)
+    kval, vval = fill(cache, gen, kind)
+    cache.append(torch.full((1, 2, 64), math.nan, device="cuda"), torch.full((1, 2, 64), math.nan, device="cuda"),
+                 torch.tensor([7 * 16 + 5], dtype=torch.int32, device="cuda"))
+    table = torch.arange(1, 17, dtype=torch.int32, device="cuda")[None].repeat(2, 1)
+    table[0, 3], table[0, 9], table[1, 0] = -1, 40, 2 ** 31 - 1
+    at = 6 * 16 + 5  # page 7 is the table's entry 6: position 101
+    lens, qs = [130, 75], [70, 75]
+    cu = np.array([0, 70, 145], np.int32)
+    q = torch.randn(145, 8, 64, generator=gen, device="cuda").to(TYPES[kind])
+    q[80, 3] = math.nan   # position 10, on the absent page: sees nothing
+    q[100, 3] = math.nan  # position 30
+    want = attention_ref(q.double().cpu().numpy(), kval, vval, table.cpu().numpy(), 16, lens, cu, 0.125, 0, 40)
+    out = torch.full_like(q, 5.0)
+    cache.attention(q[:140], table, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu_q=torch.from_numpy(cu).cuda(),
+                    max_q=75, out=out[:140])
+    clean = [r for r in range(140) if not (r < 70 and lens[0] - 70 + r >= at) and r != 100]
+    close(out[clean], want, clean, kind)
+    assert out[[r for r in range(70) if lens[0] - 70 + r >= at]].isnan().all()
+    assert not out[80].any() and out[100, 3].isnan().all() and not out[100, [0, 1, 2, 4, 5, 6, 7]].isnan().any()
+    # and for single tokens
+    one = cache.attention(q[100:101], table[1:], torch.tensor([31], dtype=torch.int32, device="cuda"))
+    assert one[0, 3].isnan().all() and not one[0, [0, 1, 2, 4, 5, 6, 7]].isnan().any()
+    assert (out[140:] == 5).all()
+
+
+def test_slots_past_four_gigabytes(gen):
+    from rustyllm_b200.kv4 import KV4Cache
+    cache = KV4Cache(70000, 64, 8, 128)  # 5.2 GB
+    assert cache.device_bytes() > 2 ** 32
+    k, v = make(gen, 64, 8, 128, "f32")
+    page = 69999
+    slots = torch.arange(page * 64, page * 64 + 64, dtype=torch.int32, device="cuda")
+    cache.append(k, v, slots)
+    rk, rv = cache.read(slots)
+    assert np.array_equal(rk.double().cpu().numpy(), quantize_ref(k.cpu().numpy()))
+    low, _ = cache.read(torch.arange(0, 4096, dtype=torch.int32, device="cuda"))
+    assert not low.any()
+    q = torch.randn(1, 8, 128, generator=gen, device="cuda")
+    table = torch.tensor([[page]], dtype=torch.int32, device="cuda")
+    got = cache.attention(q, table, torch.tensor([64], dtype=torch.int32, device="cuda"))
+    p = torch.softmax(torch.einsum("hd,jhd->hj", q[0].double(), rk.double()) / 128 ** 0.5, -1)
+    want = torch.einsum("hj,jhd->hd", p, rv.double())
+    assert ((got[0].double() - want).abs() <= 2e-5 * want.abs().amax(-1, keepdim=True)).all()
+
+
+def test_calls_on_two_streams_and_in_two_graphs_do_not_meet(gen):
+    """The same cache read by two streams at once, and by two captured graphs
+    replayed at once: every call has its own workspace."""
+    from rustyllm_b200.kv4 import KV4Cache
+    cache = KV4Cache(600, 16, 2, 64)
+    fill(cache, gen)
+    lens = torch.tensor([9600], dtype=torch.int32, device="cuda")
+    table = torch.randperm(600, generator=gen, device="cuda").to(torch.int32)[None].contiguous()
+    qs = [torch.randn(1, 16, 64, generator=gen, device="cuda") for _ in range(2)]
+    want = [cache.attention(q, table, lens) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(20):
+        got = []
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                got.append(cache.attention(q, table, lens))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for q, s in zip(qs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(cache.attention(q, table, lens))
+        graphs.append(g)
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    del graphs
 
 
 @pytest.mark.parametrize("scale_v", [2.0 ** -12, 1.0, 2.0 ** 10])
