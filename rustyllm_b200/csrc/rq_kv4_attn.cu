@@ -35,6 +35,7 @@
 
 #include "rq_async.cuh"
 #include "rq_kv4.cuh"
+#include "rq_tcgen05.cuh"
 
 namespace rq {
 namespace {
@@ -1115,6 +1116,431 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
     }
 }
 
+// Many rows of 16-bit queries: 128 rows and steps of 64 positions on tcgen05.
+//
+// The K scales differ by block of 32 elements, so the scores of a block are an
+// accumulator of their own (S_b = Q_b C_b^T, 128 x 64 in TMEM) and the softmax
+// threads add them up with the scales; the V scales make P differ by block, so
+// P_b = p d_b lies in TMEM NB times as the A operand and O's columns of block b
+// take P_b C_b.  64 NB columns of S, 32 NB of P, 32 NB of O: all 512 at head_dim
+// 128, one CTA an SM.  Roles (13 warps):
+//   0 - 7   softmax: warp w holds rows 32 (w % 4) + lane and positions 32 (w / 4)
+//           .. + 31 of a step; the two warps of a row agree on its maximum
+//           through shared memory
+//   8       issues the products: S of the next step while this one's softmax
+//           runs, O once its P is there
+//   9 - 12  unpack: two warps a stream of records, one K, one V, into the
+//           128-byte-swizzled operands of the next step (two buffers)
+// What bounds it: per step and sub-core about 620 softmax and 250 unpacking
+// instructions, 512 cycles of ex2 beside them; the products take 500.
+constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 13;
+
+template <int NB>
+struct TcSmem {  // dynamic shared memory from a 1024-byte border
+    static constexpr int kAtoms = (NB + 1) / 2;  // 64 elements = 128 bytes of a row
+    static constexpr int kQ = 0, kK = kAtoms * 16384, kV = kK + 2 * kAtoms * 8192, kRing = kV + 2 * NB * 4096;
+    static constexpr int kKs = kRing + 2 * 2 * 2 * 576 * NB, kVs = kKs + 2 * NB * kTcStep * 4;
+    static constexpr int kBytes = kVs + 2 * NB * kTcStep * 2;
+    static constexpr int kCols = NB == 1 ? 128 : NB == 2 ? 256 : 512;
+};
+// byte of 16-byte chunk c of row r in a 128-byte-swizzled operand
+__device__ __forceinline__ int sw128(int r, int c) { return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4); }
+
+template <int NB, typename T>
+__global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __grid_constant__ AttnP p) {
+    using Rec = Kv4Rec<NB>;
+    using S = TcSmem<NB>;
+    constexpr int HD = 32 * NB, kSCol = 0, kPCol = 64 * NB, kOCol = 96 * NB;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2][2], b_ops_full[2], b_ops_empty[2], b_s_full, b_s_empty, b_p_full, b_pv_done;
+    __shared__ float s_mx[2][2][kTcRows], s_qs[kTcRows], s_lg[2], s_dm[2][2], s_l[2][kTcRows];
+    __shared__ int s_E[2], s_there[2][2];
+    __shared__ uint32_t s_tmem;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int unit = (int)(blockIdx.x / p.splits), split = (int)blockIdx.x - unit * p.splits;
+    const Rows o = unit_rows<kTcRows>(p, unit);
+    if (o.r0 >= o.rows) return;
+    int tile0, tile1, per;
+    unit_tiles<kTcRows>(p, o, tile0, tile1, per);
+    const int t0 = tile0 + split * per, t1 = min(t0 + per, tile1);
+    if (p.splits > 1 && t0 >= t1) return;  // the join does not read this split
+    const int steps = t1 > t0 ? (t1 - t0 + 3) / 4 : 0;
+    const int i0 = o.r0 / p.group, i1 = min(o.n_q - 1, (o.r0 + kTcRows - 1) / p.group);
+    const int seen = max(0, min(o.held, o.pos0 + i1 + 1));  // positions that any row sees end here
+    uint8_t* const sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sm32 = smem_u32(sm);
+
+    // ---- set-up: barriers, TMEM, the query operand
+    const int pw = warp - 9, list = pw >> 1, is_v = pw & 1;
+    Stream<2, Rec::kBytes, 2> in(p, sm32 + S::kRing + (warp >= 9 ? list : 0) * 2 * 2 * Rec::kBytes,
+                                 smem_u32(&bars[warp >= 9 ? list : 0][0]), lane, warp >= 9 && !is_v);
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; i++) {
+                mbar_init(smem_u32(&b_ops_full[i]), 4);
+                mbar_init(smem_u32(&b_ops_empty[i]), 1);
+            }
+            mbar_init(smem_u32(&b_s_full), 1);
+            mbar_init(smem_u32(&b_s_empty), 8);
+            mbar_init(smem_u32(&b_p_full), 8);
+            mbar_init(smem_u32(&b_pv_done), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                     "r"((uint32_t)S::kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (warp < 4) {
+        // a thread a row: normalised by a power of two to f16, which is exact
+        // for f16 and (but for elements below 2^-14 of the largest) bf16
+        const int row = threadIdx.x, r = o.r0 + row;
+        const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+        const int64_t tok = (int64_t)o.q0 + i;
+        const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
+        const T* q = static_cast<const T*>(p.q) + tok * p.qt + head * p.qh;
+        float mx = 0.0f;
+        if (ok)
+            for (int c = 0; c < HD / 8; c++) {
+                float x[8];
+                load8(q + 8 * c, p.wide, x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
+            }
+        int e2 = 0;
+        if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e2);
+        e2 = max(-120, min(120, e2));
+        const float down = __int_as_float((127 - e2) << 23);
+        s_qs[row] = __int_as_float((127 + e2) << 23) * p.scale;
+        for (int c = 0; c < HD / 8; c++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = 0.0f;
+            if (ok) load8(q + 8 * c, p.wide, x);
+            *reinterpret_cast<uint4*>(sm + S::kQ + (c >> 3) * 16384 + sw128(row, c & 7)) =
+                make_uint4(pack(x[0] * down, x[1] * down), pack(x[2] * down, x[3] * down), pack(x[4] * down, x[5] * down),
+                           pack(x[6] * down, x[7] * down));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc::tmem_fence_before();
+    __syncthreads();
+    tc::tmem_fence_after();
+    const uint32_t tmem = s_tmem;
+    bool ok = true;
+
+    if (warp >= 9) {
+        // ---------------------------------------------------------- unpack
+        in.begin(o.b, o.kvh, t0 + 2 * list, t1);
+        int E = -15;
+        const Magic magic = p.magic;
+        for (int k = 0; k < steps; k++) {
+            const int st = k & 1, s = k & 1;
+            if (ok && k >= 2 && !mbar_wait(smem_u32(&b_ops_empty[st]), ((k >> 1) - 1) & 1)) ok = false;
+            uint32_t there = k < in.n ? in.there(s) : 0;
+            if (ok && there && !in.wait(s)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) there = 0;
+            const uint8_t* rec = sm + S::kRing + (list * 2 + s) * 2 * Rec::kBytes;
+            const int g = lane >> 2, t = lane & 3;
+            uint2 sc[2];  // this lane's (token group, block) scales of both tiles
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int tile = 2 * list + i;  // of the step
+                const uint8_t* r = rec + i * Rec::kBytes;
+                uint32_t x[2 * NB];
+                sc[i] = make_uint2(0u, 0u);
+                if ((there >> i) & 1u) {
+                    load_words<NB>(r + is_v * Rec::kV, lane, x);
+                    if (lane < 4 * NB) {
+                        sc[i] = *reinterpret_cast<const uint2*>(r + Rec::kKs + is_v * 32 * NB + lane * 8);
+                        // positions that nobody sees count for nothing, whatever lies there
+                        const int left = seen - ((t0 + 4 * k + tile) * kKv4Tile + 4 * (lane / NB));
+                        if (left < 4) {
+                            sc[i].y &= left > 2 ? 0x0000FFFFu : 0u;
+                            sc[i].x &= left > 1 ? 0xFFFFFFFFu : left > 0 ? 0x0000FFFFu : 0u;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2 * NB; b++) x[b] = 0x88888888u;  // zeros
+                }
+                if (is_v) {
+                    uint8_t* dst = sm + S::kV + st * NB * 4096;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint4 v = v_operands(x[2 * b] >> (8 * h), x[2 * b + 1] >> (8 * h), magic);
+                            // rows (elements) 32 b + 16 h + g and + 8, positions 4 t .. + 3 of the tile
+                            const int e = 32 * b + 16 * h + g, c = tile * 2 + (t >> 1);
+                            *reinterpret_cast<uint2*>(dst + sw128(e, c) + 8 * (t & 1)) = make_uint2(v.x, v.y);
+                            *reinterpret_cast<uint2*>(dst + sw128(e + 8, c) + 8 * (t & 1)) = make_uint2(v.z, v.w);
+                        }
+                } else {
+                    uint8_t* dst = sm + S::kK + st * S::kAtoms * 8192;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++) {
+                            const int row = tile * kKv4Tile + 4 * (g >> 1) + (g & 1) + 2 * n;
+                            *reinterpret_cast<uint4*>(dst + (b >> 1) * 8192 + sw128(row, (b & 1) * 4 + t)) =
+                                k_operands(x[2 * b + n], magic);
+                        }
+                }
+            }
+            if (is_v) {
+                // E follows the largest scale; the two V warps agree on it
+                __half2 big = __half2half2(__ushort_as_half(0));
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    big = __hmax2(big, __hmax2(__habs2(as_h2(sc[i].x)), __habs2(as_h2(sc[i].y))));
+                float dm = fmaxf(__half2float(__low2half(big)), __half2float(__high2half(big)));
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, i));
+                if (lane == 0) s_dm[st][list] = dm;
+                named_bar_sync(7, 64);
+                dm = fmaxf(s_dm[st][0], s_dm[st][1]);
+                if (dm > __int_as_float((127 + E) << 23)) {
+                    int e;
+                    frexpf(dm, &e);
+                    E = e;
+                }
+                if (list == 0 && lane == 0) {
+                    s_E[st] = E;
+                    s_lg[st] = fmaxf(lg2(dm) - (float)E, -7.0f);
+                }
+                const __half2 inv = __float2half2_rn(__int_as_float((127 - E) << 23));
+                if (lane < 4 * NB)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        *reinterpret_cast<uint2*>(sm + S::kVs + ((st * NB + lane % NB) * kTcStep + (2 * list + i) * 16 + 4 * (lane / NB)) * 2) =
+                            make_uint2(as_u32(__hmul2(as_h2(sc[i].x), inv)), as_u32(__hmul2(as_h2(sc[i].y), inv)));
+            } else if (lane < 4 * NB) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float2 u = unpack(sc[i].x), v = unpack(sc[i].y);
+                    *reinterpret_cast<float4*>(sm + S::kKs + ((st * NB + lane % NB) * kTcStep + (2 * list + i) * 16 + 4 * (lane / NB)) * 4) =
+                        make_float4(u.x, u.y, v.x, v.y);
+                }
+            }
+            if (!is_v && lane == 0) s_there[st][list] = (int)there;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&b_ops_full[st]));
+            named_bar_sync(5 + list, 64);  // both warps have read the records
+            if (ok && k + 2 < in.n) in.issue(k + 2, s);
+        }
+        if (!ok) in.abandon(0);
+    } else if (warp == 8) {
+        // -------------------------------------------------------- products
+        constexpr uint32_t kIdS = (1u << 4) | ((uint32_t)(kTcStep >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t kIdO = (1u << 4) | ((uint32_t)(32 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        for (int k = -1; k < steps; k++) {
+            if (k + 1 < steps) {  // S of the next step
+                const int st = (k + 1) & 1;
+                if (ok && !mbar_wait(smem_u32(&b_ops_full[st]), ((k + 1) >> 1) & 1)) ok = false;
+                if (ok && k >= 0 && !mbar_wait(smem_u32(&b_s_empty), k & 1)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                tc::tmem_fence_after();
+                if (tc::elect_one()) {
+                    if (ok) {
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                const uint32_t off = (uint32_t)(64 * (b & 1) + 32 * x);
+                                tc::umma_f16(tmem + kSCol + 64 * b, tc::desc_sw128(sm32 + S::kQ + (b >> 1) * 16384 + off),
+                                             tc::desc_sw128(sm32 + S::kK + (st * S::kAtoms + (b >> 1)) * 8192 + off), kIdS,
+                                             x ? 1u : 0u);
+                            }
+                    }
+                    tc::umma_commit(smem_u32(&b_s_full));
+                }
+                __syncwarp();
+            }
+            if (k >= 0) {  // O of this one
+                const int st = k & 1;
+                if (ok && !mbar_wait(smem_u32(&b_p_full), k & 1)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                tc::tmem_fence_after();
+                if (tc::elect_one()) {
+                    if (ok) {
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+                                tc::umma_f16_ts(tmem + kOCol + 32 * b, tmem + kPCol + 32 * b + 8 * x,
+                                                tc::desc_sw128(sm32 + S::kV + (st * NB + b) * 4096 + 32 * x), kIdO,
+                                                k > 0 || x > 0 ? 1u : 0u);
+                    }
+                    tc::umma_commit(smem_u32(&b_pv_done));
+                    tc::umma_commit(smem_u32(&b_ops_empty[st]));
+                }
+                __syncwarp();
+            }
+        }
+        // the last commit's arrival, which nobody else waits for, may not find
+        // the CTA gone
+        if (ok && steps > 0 && !mbar_wait(smem_u32(&b_ops_empty[(steps - 1) & 1]), ((steps - 1) >> 1) & 1)) ok = false;
+        if (!ok && lane == 0) atomicExch(p.err, 1);
+    } else {
+        // --------------------------------------------------------- softmax
+        const int q = warp & 3, h = warp >> 2, row = 32 * q + lane;
+        const int r = o.r0 + row, i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+        const int64_t tok = (int64_t)o.q0 + i;
+        const bool live = r < o.rows && tok >= 0 && tok < p.n_tokens;
+        const int rpos = live ? o.pos0 + i : -1;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+        const float qs = s_qs[row];
+        float m = -INFINITY, l = 0.0f;
+        int E = 0;
+        for (int k = 0; k < steps; k++) {
+            const int st = k & 1;
+            if (ok && !mbar_wait(smem_u32(&b_ops_full[st]), (k >> 1) & 1)) ok = false;
+            if (ok && !mbar_wait(smem_u32(&b_s_full), k & 1)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            tc::tmem_fence_after();
+            // ---- scores of positions j0 .. j0 + 31
+            const int j0 = (t0 + 4 * k) * kKv4Tile + 32 * h;
+            float2 sc[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) sc[j] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t a[32];
+                tc::tmem_ld32(lanes + kSCol + 64 * b + 32 * h, a);
+                tc::tmem_wait_ld();
+                const float4* d = reinterpret_cast<const float4*>(sm + S::kKs + ((st * NB + b) * kTcStep + 32 * h) * 4);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 v = d[j];
+                    sc[2 * j] = fma2(make_float2(__uint_as_float(a[4 * j]), __uint_as_float(a[4 * j + 1])), make_float2(v.x, v.y), sc[2 * j]);
+                    sc[2 * j + 1] = fma2(make_float2(__uint_as_float(a[4 * j + 2]), __uint_as_float(a[4 * j + 3])), make_float2(v.z, v.w), sc[2 * j + 1]);
+                }
+            }
+            tc::tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&b_s_empty));
+            // ---- which of them the row sees
+            const uint32_t there = (uint32_t)s_there[st][h];
+            const int hi = min(min(rpos + 1, o.held) - j0, 32), lo = p.window > 0 ? max(rpos - p.window + 1 - j0, 0) : 0;
+            uint32_t sees = (hi >= 32 ? 0xFFFFFFFFu : hi > 0 ? (1u << hi) - 1u : 0u) & (lo >= 32 ? 0u : 0xFFFFFFFFu << lo);
+            sees &= (there & 1u ? 0xFFFFu : 0u) | (there & 2u ? 0xFFFF0000u : 0u);
+            const bool full = __all_sync(0xffffffffu, sees == 0xFFFFFFFFu);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                sc[j] = mul2(sc[j], make_float2(qs, qs));
+                if (!full) {
+                    if (!((sees >> (2 * j)) & 1u)) sc[j].x = -INFINITY;
+                    if (!((sees >> (2 * j + 1)) & 1u)) sc[j].y = -INFINITY;
+                }
+                mx = fmaxf(mx, fmaxf(sc[j].x, sc[j].y));
+            }
+            s_mx[st][h][row] = mx;
+            named_bar_sync(1 + q, 64);
+            mx = fmaxf(mx, s_mx[st][h ^ 1][row]) + s_lg[st];
+            // ---- move the row's reference or the scales' power where they grew
+            const int e = s_E[st];
+            float al = k > 0 ? __int_as_float((127 + max(E - e, -126)) << 23) : 1.0f;
+            E = e;
+            if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
+                const float f = m == -INFINITY ? 0.0f : ex2(m - mx);
+                al *= f;
+                l *= f;
+                m = mx;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            uint32_t ph[16];
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float2 x = add2(sc[j], make_float2(-base, -base));
+                const float2 y = make_float2(ex2(x.x), ex2(x.y));
+                sum = add2(sum, y);
+                ph[j] = pack(y.x, y.y);
+            }
+            l += sum.x + sum.y;
+            // ---- O and P are free once the products of the step before are done
+            if (ok && k > 0 && !mbar_wait(smem_u32(&b_pv_done), (k - 1) & 1)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            tc::tmem_fence_after();
+            if (k > 0 && __any_sync(0xffffffffu, al != 1.0f)) {
+#pragma unroll
+                for (int c = 0; c < NB; c++) {  // this warp's half of the columns
+                    uint32_t a[16];
+                    const uint32_t at = lanes + kOCol + 16 * (h * NB + c);
+                    tc::tmem_ld16(at, a);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 16; x++) a[x] = __float_as_uint(__uint_as_float(a[x]) * al);
+                    tc::tmem_st16u(at, a);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint4* d = reinterpret_cast<const uint4*>(sm + S::kVs + ((st * NB + b) * kTcStep + 32 * h) * 2);
+                uint32_t a[16];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint4 v = d[j];
+                    a[4 * j] = as_u32(__hmul2(as_h2(ph[4 * j]), as_h2(v.x)));
+                    a[4 * j + 1] = as_u32(__hmul2(as_h2(ph[4 * j + 1]), as_h2(v.y)));
+                    a[4 * j + 2] = as_u32(__hmul2(as_h2(ph[4 * j + 2]), as_h2(v.z)));
+                    a[4 * j + 3] = as_u32(__hmul2(as_h2(ph[4 * j + 3]), as_h2(v.w)));
+                }
+                if (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        a[j] &= ((sees >> (2 * j)) & 1u ? 0xFFFFu : 0u) | ((sees >> (2 * j + 1)) & 1u ? 0xFFFF0000u : 0u);
+                }
+                tc::tmem_st16u(lanes + kPCol + 32 * b + 16 * h, a);
+            }
+            tc::tmem_wait_st();
+            tc::tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&b_p_full));
+        }
+        if (ok && steps > 0 && !mbar_wait(smem_u32(&b_pv_done), (steps - 1) & 1)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok && lane == 0) atomicExch(p.err, 1);
+        tc::tmem_fence_after();
+        s_l[h][row] = l;
+        named_bar_sync(1 + q, 64);
+        l += s_l[h ^ 1][row];
+        // ---- columns 16 NB h .. of the row
+        const bool any = l != 0.0f;  // (not a number counts)
+        const float bound = __int_as_float((127 + E) << 23), f = p.splits == 1 ? bound / l : bound;
+        const int64_t at = (tok * p.n_heads + head) * p.splits + split;
+        T* out = static_cast<T*>(p.out) + tok * p.ot + head * p.oh;
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            uint32_t a[16];
+            const int col = 16 * (h * NB + c);
+            if (steps > 0) {
+                tc::tmem_ld16(lanes + kOCol + col, a);
+                tc::tmem_wait_ld();
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                const float v = any ? __uint_as_float(a[x]) * f : 0.0f;
+                if (p.splits == 1) out[col + x] = from_f32<T>(v);
+                else p.part[at * HD + col + x] = v;
+            }
+        }
+        if (p.splits > 1 && live && h == 0) p.ml[at] = make_float2(m, l);
+    }
+    // every product and copy has been waited for (or its wait gave up)
+    tc::tmem_fence_before();
+    __syncthreads();
+    tc::tmem_fence_after();
+    if (warp == 8)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)S::kCols));
+}
+
 // Joins the pieces of a row, a CTA a row: groups of 8 NB threads (four elements
 // each) take every kJoin / (8 NB)-th piece, and add up in group order.  slot(s):
 // where piece s lies.
@@ -1200,9 +1626,12 @@ struct Fns {
 template <int NB, int MODE, typename T>
 Fns fns_of(bool rows) {
     constexpr int R = MODE == kOne16 ? 16 : 8;
-    if constexpr (sizeof(T) == 4 || MODE == kOne16)  // 16-bit queries have no form of many rows in tiles of eight
+    if constexpr (sizeof(T) == 4) {
         if (rows)
             return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
+    } else if constexpr (MODE == kOne16) {
+        if (rows) return Fns{(const void*)kv4_attn_tc_kernel<NB, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
+    }
     return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
 }
 template <int NB, typename T>
@@ -1228,7 +1657,7 @@ Fns fns_of(int dtype, int nb, int mode, bool rows) {
 
 struct Plan {
     int mode, R;       // R: rows of a CTA
-    bool rows;         // the many-rows form
+    bool rows, tc;     // a many-rows form; the one on tcgen05
     int64_t ctas;      // of the main launch
     int row_tiles, splits;  // many rows
     int64_t pieces;    // row sums kept for the join: 0, no join
@@ -1281,12 +1710,13 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
         pl.pieces = pl.ctas > 1 ? 2 * pl.ctas * pl.R : 0;
         return pl;
     }
-    pl.R *= 2 * kWarps;
+    pl.tc = a->dtype != RQ_F32;
+    pl.R = pl.tc ? kTcRows : 2 * kWarps * pl.R;
     pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
     const int64_t units = a->batch * c->n_kv * pl.row_tiles;
     // splits of the long axis where the units leave the device's places (two
     // CTAs an SM) empty, none shorter than two steps
-    const int64_t want = sms * 2 / std::max<int64_t>(units, 1);
+    const int64_t want = sms * (pl.tc ? 1 : 2) / std::max<int64_t>(units, 1);
     pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / (2 * kWarps)));
     pl.ctas = units * pl.splits;
     pl.pieces = pl.splits > 1 ? a->n_tokens * a->n_heads * pl.splits : 0;
@@ -1347,16 +1777,18 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.magic = Magic{kEven, kOdd};
     p.err = err;
     const int nb = c->head_dim / 32;
-    const size_t smem = pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb + 2048 * nb)
+    constexpr int tc_smem[4] = {TcSmem<1>::kBytes, TcSmem<2>::kBytes, TcSmem<3>::kBytes, TcSmem<4>::kBytes};
+    const size_t smem = pl.tc     ? (size_t)tc_smem[nb - 1] + 1024
+                        : pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb + 2048 * nb)
                                 : (size_t)kWarps * (kStages * 2 * 576 * nb + pl.R * 32 * nb * 4);
     const Fns fn = fns_of(a->dtype, nb, pl.mode, pl.rows);
-    if (smem > 48 * 1024) {
+    if (smem > 32 * 1024) {  // (48 KB without asking, the kernels' static part included)
         const int rc = cuda_error(cudaFuncSetAttribute(fn.main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                                   "kv4 attention kernel");
         if (rc) return rc;
     }
     void* args[] = {&p};
-    const int rc = launch_pdl(fn.main, (unsigned)pl.ctas, kWarps * 32, smem, st, args, "kv4 attention kernel");
+    const int rc = launch_pdl(fn.main, (unsigned)pl.ctas, (pl.tc ? kTcWarps : kWarps) * 32, smem, st, args, "kv4 attention kernel");
     if (rc || !pl.pieces) return rc;
     const int64_t joins = pl.rows ? a->batch * c->n_kv * pl.row_tiles * pl.R : pl.ctas * pl.R;
     return launch_pdl(fn.join, (unsigned)joins, kJoin, 0, st, args, "kv4 join kernel");
