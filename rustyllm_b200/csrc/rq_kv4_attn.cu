@@ -4,9 +4,24 @@
 // For a query row q and the positions j it sees, with K = (c - 8) d per block
 // of 32 elements:
 //   s_j = scale * sum_b dK_jb (q_b . (cK_jb - 8)),  o = sum_j softmax(s)_j V_j.
-// The codes c - 8 are exact in f16, so both products run on mma.m16n8k16
-// without rounding the cache: q is scaled by a power of two to [-1, 1] and
-// split into f16 hi + lo (f32 input; 16-bit inputs need hi alone), the K
+// The codes c - 8 are exact in f16.
+//
+// Three forms, chosen by make_plan:
+//  - few rows (decode, drafted tokens), on mma.m16n8k16: every warp of a CTA
+//    walks its own tiles of 16 positions for the same rows, so one row tile uses
+//    all lanes of the GPU; its operands are built in registers from the record
+//    that one bulk copy brought to shared memory.  The warps join through shared
+//    memory, the pieces of a unit that went to several CTAs through a second
+//    launch.
+//  - many rows of f32 queries (prompts), on mma.m16n8k16: the warps hold
+//    different rows, two operand tiles each; the records are turned into f16
+//    operands in shared memory once for all four, and an operand read from there
+//    serves two tiles of rows (with one tile a warp, reading them took as long as
+//    the products).
+//  - many rows of 16-bit queries, on tcgen05: see there.
+//
+// The first two do not round the cache: q is scaled by a power of two to [-1, 1]
+// and split into f16 hi + lo (f32 input; 16-bit inputs need hi alone), the K
 // scales multiply the f32 block sums, and the V scales multiply the
 // probabilities, P_jb = p_j dV_jb.  For f32 the hi and lo parts are the two row
 // halves of one m16 operand: eight query rows a tile, no extra instructions.
@@ -14,23 +29,12 @@
 // P enters as f16: for f32, p = ph + pl (22 bits) and ph d = h + r exactly (h
 // the rounded product, r = fma(ph, d, -h)), so P = h + (r + pl d) costs three
 // packed operations a pair of tokens; 16-bit outputs take h alone (two
-// roundings of 2^-12, below the output's own).  f16's range is kept whatever
-// the scale of V: the scales are divided by a power of two 2^E that follows
-// the largest one seen, and the running maximum m is taken over s_j + log2 of
-// the lane's largest scale (not below 2^-7), so that |P| <= 2^8 with the
+// roundings of 2^-11, an eighth of bf16's own and as much as f16's).  f16's range
+// is kept whatever the scale of V: the scales are divided by a power of two 2^E
+// that follows the largest one seen, and the running maximum m is taken over s_j
+// + log2 of the lane's largest scale (not below 2^-7), so that |P| <= 2^8 with the
 // largest near 1, and p <= 2^15.  m and E move lazily, when P would pass 2^8
 // or a scale 2^E.  Sums stay in f32 throughout.
-//
-// Two forms of one kernel:
-//  - few rows (decode): every warp of a CTA walks its own tiles of 16
-//    positions for the same rows, so one row tile uses all lanes of the GPU;
-//    its operands are built in registers from the record that one bulk copy
-//    brought to shared memory.  The warps join through shared memory, the
-//    pieces of a unit that went to several CTAs through a second launch.
-//  - many rows (prompts): the warps hold different rows, two operand tiles each;
-//    the records are turned into f16 operands in shared memory once for all
-//    four, and an operand read from there serves two tiles of rows (with one
-//    tile a warp, reading them took as long as the products).
 #include <algorithm>
 
 #include "rq_async.cuh"
@@ -44,7 +48,6 @@ constexpr int kWarps = 4;       // warps of a CTA
 constexpr int kStages = 3;      // pairs of tiles in flight per warp (few rows)
 constexpr int kStagesRows = 2;  // (many rows)
 constexpr float kLazy = 8.0f;   // log2 of the largest |P|
-constexpr float kFloor = 0.0078125f;  // 2^-7
 
 enum Mode { kSplit8, kOne16 };  // 8 rows of hi + lo parts, 16 rows of one part
 
@@ -60,7 +63,7 @@ struct AttnP {
     int64_t qt, qh;
     void* out;
     int64_t ot, oh;
-    bool wide;
+    bool wide, wide_out;  // rows of q, of out on 16-byte borders
     int64_t n_tokens;
     int n_heads, group, batch, max_q, row_tiles, splits;
     const int32_t* cu_q;
@@ -180,7 +183,7 @@ struct Rows : Seq {
     __device__ __forceinline__ Rows(const AttnP& p, int b, int kvh, int r0)
         : Seq(p, b), b(b), kvh(kvh), r0(r0), rows(n_q * p.group) {}
 };
-// Unit `unit` of the many-rows form, row tiles of R; false: no such rows
+// Unit `unit` of the many-rows forms, row tiles of R; its r0 may lie behind the rows
 template <int R>
 __device__ __forceinline__ Rows unit_rows(const AttnP& p, int unit) {
     const int bk = unit / p.row_tiles, b = bk / p.n_kv;
@@ -1118,47 +1121,74 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 
 // Many rows of 16-bit queries: 128 rows and steps of 64 positions on tcgen05.
 //
-// The K scales differ by block of 32 elements, so the scores of a block are an
-// accumulator of their own (S_b = Q_b C_b^T, 128 x 64 in TMEM) and the softmax
-// threads add them up with the scales; the V scales make P differ by block, so
-// P_b = p d_b lies in TMEM NB times as the A operand and O's columns of block b
-// take P_b C_b.  64 NB columns of S, 32 NB of P, 32 NB of O: all 512 at head_dim
-// 128, one CTA an SM.  Roles (13 warps):
-//   0 - 7   softmax: warp w holds rows 32 (w % 4) + lane and positions 32 (w / 4)
-//           .. + 31 of a step; the two warps of a row agree on its maximum
-//           through shared memory
-//   8       issues the products: S of the next step while this one's softmax
-//           runs, O once its P is there
-//   9 - 12  unpack: two warps a stream of records, one K, one V, into the
-//           128-byte-swizzled operands of the next step (two buffers)
-// What bounds it: per step and sub-core about 620 softmax and 250 unpacking
-// instructions, 512 cycles of ex2 beside them; the products take 500.
-constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 13;
+// K and V enter as f16 values (c - 8) d / 2^E, one rounding of 2^-11 of each:
+// as much as the queries' own type gives them, and for V as P's.  (Kept exact --
+// a product a block, scaled in the softmax, P times each block's scales -- S and
+// P crossed TMEM head_dim / 32 times, for 1.3 times the softmax's time.)  E is
+// the step's: zero scales apart, the largest one comes to [2^11, 2^12) -- so
+// that 8 d still is an f16 -- or stays below it with the power at its floor, and
+// only scales 2^26 times smaller than that lose bits.  A row keeps its own
+// largest power of V in sight and weighs the step by 2^(E - that).  A value that
+// is not a number cannot lie in an operand that rows share which do not see it:
+// it enters as zero, and the rows that do see it are marked and get it at the
+// end.
+//
+// TMEM, for even steps and for odd ones: S (64 columns), P as the A operand
+// (32) and O (32 NB).
+// Roles (17 warps):
+//   0 - 7   softmax: even steps the first four, odd ones the others, a thread a
+//           row; the two groups keep their own maxima and sums, joined at the
+//           end (as one group with half the positions a warp, which agreed on
+//           every step's maximum: 318 us where two took 279)
+//   8       issues the products: S two steps ahead of P V
+//   9 - 16  unpack, even steps the first four, odd ones the others: two warps a
+//           half of the step, one K, one V, into the 128-byte-swizzled operands
+//           (four buffers: with two, and one group, unpacking a step waited for
+//           the products two steps before, 3400 cycles a step where this takes
+//           2000)
+//
+// 270 us at three prompts of 256 - 512 tokens on up to 4500 positions, 64 query
+// heads on 8, head_dim 128 (280 TFLOP/s): the issue of some 5700 warp
+// instructions a step bounds it, two thirds of them the unpacking's and the
+// exponentials', at 2.2 a cycle; the tensor pipe is busy for a fifth of the time.
+constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 17, kTcOps = 4;
+constexpr int kTcTop = 12, kTcLow = -8;  // see E
+constexpr float kTcUp = 7.0f;  // the largest P lies in [2^7, 2^15], so that f16 has it to 2^-11 down to 2^-21 of that
 
 template <int NB>
 struct TcSmem {  // dynamic shared memory from a 1024-byte border
     static constexpr int kAtoms = (NB + 1) / 2;  // 64 elements = 128 bytes of a row
-    static constexpr int kQ = 0, kK = kAtoms * 16384, kV = kK + 2 * kAtoms * 8192, kRing = kV + 2 * NB * 4096;
-    static constexpr int kKs = kRing + 2 * 2 * 2 * 576 * NB, kVs = kKs + 2 * NB * kTcStep * 4;
-    static constexpr int kBytes = kVs + 2 * NB * kTcStep * 2;
-    static constexpr int kCols = NB == 1 ? 128 : NB == 2 ? 256 : 512;
+    static constexpr int kQ = 0, kK = kAtoms * 16384, kV = kK + kTcOps * kAtoms * 8192,
+                         kRing = kV + kTcOps * NB * 4096;
+    static constexpr int kScl = kRing + 4 * 2 * 2 * 576 * NB;  // [8 unpacking warps][2 tiles][32 NB]
+    static constexpr int kBytes = kScl + 8 * 2 * 32 * NB;
+    static constexpr int kCols = NB == 1 ? 256 : 512;
 };
 // byte of 16-byte chunk c of row r in a 128-byte-swizzled operand
 __device__ __forceinline__ int sw128(int r, int c) { return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) { return as_u32(__hmul2(as_h2(a), as_h2(b))); }
+// halves of all ones where w's f16 is not a number
+__device__ __forceinline__ uint32_t nan_halves(uint32_t w) {
+    return __hne2_mask(as_h2(w), as_h2(w));
+}
 
 template <int NB, typename T>
 __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
     using S = TcSmem<NB>;
-    constexpr int HD = 32 * NB, kSCol = 0, kPCol = 64 * NB, kOCol = 96 * NB;
+    constexpr int HD = 32 * NB, kPCol = 128, kOCol = 192;  // TMEM: S, P, O of even and odd steps
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2][2], b_ops_full[2], b_ops_empty[2], b_s_full, b_s_empty, b_p_full, b_pv_done;
-    __shared__ float s_mx[2][2][kTcRows], s_qs[kTcRows], s_lg[2], s_dm[2][2], s_l[2][kTcRows];
-    __shared__ int s_E[2], s_there[2][2];
+    __shared__ __align__(8) uint64_t bars[4][2], b_ops_full[kTcOps], b_ops_empty[kTcOps], b_s_full[2], b_s_empty[2],
+        b_p_full[2], b_pv_done[2];
+    __shared__ float s_qs[kTcRows], s_dm[kTcOps][2][2], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows], s_kf[kTcOps];
+    __shared__ int s_E[kTcOps], s_there[kTcOps][2], s_any_nan[kTcOps][2];
+    __shared__ uint32_t s_nan[kTcOps][2][NB], s_bad[2][kTcRows];  // positions that are not numbers: of a step's half, by block
     __shared__ uint32_t s_tmem;
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int unit = (int)(blockIdx.x / p.splits), split = (int)blockIdx.x - unit * p.splits;
+    // a sequence's last rows, which see the most, first
+    const int at0 = (int)(blockIdx.x / p.splits), split = (int)blockIdx.x - at0 * p.splits;
+    const int unit = (int)(gridDim.x / p.splits) - 1 - at0;
     const Rows o = unit_rows<kTcRows>(p, unit);
     if (o.r0 >= o.rows) return;
     int tile0, tile1, per;
@@ -1166,25 +1196,29 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
     const int t0 = tile0 + split * per, t1 = min(t0 + per, tile1);
     if (p.splits > 1 && t0 >= t1) return;  // the join does not read this split
     const int steps = t1 > t0 ? (t1 - t0 + 3) / 4 : 0;
-    const int i0 = o.r0 / p.group, i1 = min(o.n_q - 1, (o.r0 + kTcRows - 1) / p.group);
+    const int i1 = min(o.n_q - 1, (o.r0 + kTcRows - 1) / p.group);
     const int seen = max(0, min(o.held, o.pos0 + i1 + 1));  // positions that any row sees end here
     uint8_t* const sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sm32 = smem_u32(sm);
 
-    // ---- set-up: barriers, TMEM, the query operand
+    // ---- set-up: barriers, TMEM, the query operand, the first records
     const int pw = warp - 9, list = pw >> 1, is_v = pw & 1;
-    Stream<2, Rec::kBytes, 2> in(p, sm32 + S::kRing + (warp >= 9 ? list : 0) * 2 * 2 * Rec::kBytes,
+    Stream<2, Rec::kBytes, 4> in(p, sm32 + S::kRing + (warp >= 9 ? list : 0) * 2 * 2 * Rec::kBytes,
                                  smem_u32(&bars[warp >= 9 ? list : 0][0]), lane, warp >= 9 && !is_v);
-    if (warp == 8) {
+    if (warp >= 9) {
+        in.begin(o.b, o.kvh, t0 + 2 * list, t1);
+    } else if (warp == 8) {
         if (lane == 0) {
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < kTcOps; i++) {
                 mbar_init(smem_u32(&b_ops_full[i]), 4);
                 mbar_init(smem_u32(&b_ops_empty[i]), 1);
             }
-            mbar_init(smem_u32(&b_s_full), 1);
-            mbar_init(smem_u32(&b_s_empty), 8);
-            mbar_init(smem_u32(&b_p_full), 8);
-            mbar_init(smem_u32(&b_pv_done), 1);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(smem_u32(&b_s_full[i]), 1);
+                mbar_init(smem_u32(&b_s_empty[i]), 4);
+                mbar_init(smem_u32(&b_p_full[i]), 4);
+                mbar_init(smem_u32(&b_pv_done[i]), 1);
+            }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -1192,35 +1226,39 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                      "r"((uint32_t)S::kCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else if (warp < 4) {
-        // a thread a row: normalised by a power of two to f16, which is exact
+    } else {
+        // two lanes a row: normalised by a power of two to f16, which is exact
         // for f16 and (but for elements below 2^-14 of the largest) bf16
-        const int row = threadIdx.x, r = o.r0 + row;
+        const int row = threadIdx.x >> 1, r = o.r0 + row;
         const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
         const int64_t tok = (int64_t)o.q0 + i;
         const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
         const T* q = static_cast<const T*>(p.q) + tok * p.qt + head * p.qh;
+        float x[2 * NB][8];  // chunks 2 c + (lane & 1)
         float mx = 0.0f;
-        if (ok)
-            for (int c = 0; c < HD / 8; c++) {
-                float x[8];
-                load8(q + 8 * c, p.wide, x);
 #pragma unroll
-                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
-            }
+        for (int c = 0; c < 2 * NB; c++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[c][e] = 0.0f;
+            if (ok) load8(q + 8 * (2 * c + (lane & 1)), p.wide, x[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         int e2 = 0;
         if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e2);
-        e2 = max(-120, min(120, e2));
-        const float down = __int_as_float((127 - e2) << 23);
-        s_qs[row] = __int_as_float((127 + e2) << 23) * p.scale;
-        for (int c = 0; c < HD / 8; c++) {
-            float x[8];
+        e2 = max(-110, min(110, e2));
+        // the scale's sign is the operand's, so that scores grow with their sums
+        const float down = p.scale == 0.0f ? 0.0f : copysignf(__int_as_float((127 - e2) << 23), p.scale);
+        if ((lane & 1) == 0) s_qs[row] = p.scale == 0.0f ? 1.0f : __int_as_float((127 + e2) << 23) * fabsf(p.scale);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = 0.0f;
-            if (ok) load8(q + 8 * c, p.wide, x);
-            *reinterpret_cast<uint4*>(sm + S::kQ + (c >> 3) * 16384 + sw128(row, c & 7)) =
-                make_uint4(pack(x[0] * down, x[1] * down), pack(x[2] * down, x[3] * down), pack(x[4] * down, x[5] * down),
-                           pack(x[6] * down, x[7] * down));
+        for (int c = 0; c < 2 * NB; c++) {
+            const int at = 2 * c + (lane & 1);
+            *reinterpret_cast<uint4*>(sm + S::kQ + (at >> 3) * 16384 + sw128(row, at & 7)) =
+                make_uint4(pack(x[c][0] * down, x[c][1] * down), pack(x[c][2] * down, x[c][3] * down),
+                           pack(x[c][4] * down, x[c][5] * down), pack(x[c][6] * down, x[c][7] * down));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -1232,36 +1270,77 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
 
     if (warp >= 9) {
         // ---------------------------------------------------------- unpack
-        in.begin(o.b, o.kvh, t0 + 2 * list, t1);
-        int E = -15;
+        const int g = lane >> 2, t = lane & 3, half = list & 1;
         const Magic magic = p.magic;
-        for (int k = 0; k < steps; k++) {
-            const int st = k & 1, s = k & 1;
-            if (ok && k >= 2 && !mbar_wait(smem_u32(&b_ops_empty[st]), ((k >> 1) - 1) & 1)) ok = false;
-            uint32_t there = k < in.n ? in.there(s) : 0;
+        uint8_t* const scl = sm + S::kScl + pw * 2 * 32 * NB;
+        for (int j = 0; 2 * j + (list >> 1) < steps; j++) {
+            const int k = 2 * j + (list >> 1), st = k % kTcOps, s = j & 1;
+            if (ok && k >= kTcOps && !mbar_wait(smem_u32(&b_ops_empty[st]), ((k / kTcOps) - 1) & 1)) ok = false;
+            uint32_t there = j < in.n ? in.there(s) : 0;
             if (ok && there && !in.wait(s)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) there = 0;
             const uint8_t* rec = sm + S::kRing + (list * 2 + s) * 2 * Rec::kBytes;
-            const int g = lane >> 2, t = lane & 3;
-            uint2 sc[2];  // this lane's (token group, block) scales of both tiles
+            // ---- scales: lane u holds those of token group u / NB, block u % NB
+            // (four tokens) of both tiles; positions that nobody sees count
+            // for nothing, whatever lies there
+            uint2 sc[2];
+            uint32_t bad[2] = {0u, 0u};  // tokens (bits 0 - 3) whose value is not a number
+            __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int tile = 2 * list + i;  // of the step
-                const uint8_t* r = rec + i * Rec::kBytes;
-                uint32_t x[2 * NB];
                 sc[i] = make_uint2(0u, 0u);
-                if ((there >> i) & 1u) {
-                    load_words<NB>(r + is_v * Rec::kV, lane, x);
-                    if (lane < 4 * NB) {
-                        sc[i] = *reinterpret_cast<const uint2*>(r + Rec::kKs + is_v * 32 * NB + lane * 8);
-                        // positions that nobody sees count for nothing, whatever lies there
-                        const int left = seen - ((t0 + 4 * k + tile) * kKv4Tile + 4 * (lane / NB));
-                        if (left < 4) {
-                            sc[i].y &= left > 2 ? 0x0000FFFFu : 0u;
-                            sc[i].x &= left > 1 ? 0xFFFFFFFFu : left > 0 ? 0x0000FFFFu : 0u;
-                        }
+                if (((there >> i) & 1u) && lane < 4 * NB) {
+                    sc[i] = *reinterpret_cast<const uint2*>(rec + i * Rec::kBytes + Rec::kKs + is_v * 32 * NB + lane * 8);
+                    const int left = seen - ((t0 + 4 * k + 2 * half + i) * kKv4Tile + 4 * (lane / NB));
+                    if (left < 4) {
+                        sc[i].y &= left > 2 ? 0x0000FFFFu : 0u;
+                        sc[i].x &= left > 1 ? 0xFFFFFFFFu : left > 0 ? 0x0000FFFFu : 0u;
                     }
+                    if (is_v) {
+                        const uint32_t nx = nan_halves(sc[i].x), ny = nan_halves(sc[i].y);
+                        bad[i] = (nx & 1u) | ((nx >> 15) & 2u) | ((ny & 1u) << 2) | ((ny >> 13) & 8u);
+                        sc[i].x &= ~nx;
+                        sc[i].y &= ~ny;
+                    }
+                }
+                big = __hmax2(big, __hmax2(__habs2(as_h2(sc[i].x)), __habs2(as_h2(sc[i].y))));
+            }
+            float dm = fmaxf(__half2float(__low2half(big)), __half2float(__high2half(big)));
+#pragma unroll
+            for (int i = 16; i > 0; i >>= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, i));
+            if (lane == 0) s_dm[st][is_v][half] = dm;
+            if (is_v) {
+                const bool none = !__any_sync(0xffffffffu, bad[0] | bad[1]);
+                if (lane < NB) s_nan[st][half][lane] = 0u;
+                if (lane == 0) s_any_nan[st][half] = !none;
+            }
+            named_bar_sync(9 + 2 * (list >> 1) + is_v, 64);  // the step's two K, or V warps
+            dm = fmaxf(s_dm[st][is_v][0], s_dm[st][is_v][1]);
+            int E = kTcLow;
+            if (dm > __int_as_float((127 + kTcTop + kTcLow) << 23)) {
+                frexpf(dm, &E);
+                E -= kTcTop;
+            }
+            if (half == 0 && lane == 0) {
+                if (is_v) s_E[st] = E;
+                else s_kf[st] = __int_as_float((127 + E) << 23);
+            }
+            const uint32_t inv = as_u32(__float2half2_rn(__int_as_float((127 - E) << 23)));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (lane < 4 * NB)
+                    *reinterpret_cast<uint2*>(scl + i * 32 * NB + lane * 8) = make_uint2(times(sc[i].x, inv), times(sc[i].y, inv));
+                if (bad[i]) atomicOr(&s_nan[st][half][lane % NB], bad[i] << (16 * i + 4 * (lane / NB)));
+            }
+            __syncwarp();
+            // ---- values
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int tile = 2 * half + i;  // of the step
+                uint32_t x[2 * NB];
+                if ((there >> i) & 1u) {
+                    load_words<NB>(rec + i * Rec::kBytes + is_v * Rec::kV, lane, x);
                 } else {
 #pragma unroll
                     for (int b = 0; b < 2 * NB; b++) x[b] = 0x88888888u;  // zeros
@@ -1269,121 +1348,86 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                 if (is_v) {
                     uint8_t* dst = sm + S::kV + st * NB * 4096;
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
+                    for (int b = 0; b < NB; b++) {
+                        const uint2 d = *reinterpret_cast<const uint2*>(scl + i * 32 * NB + (t * NB + b) * 8);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const uint4 v = v_operands(x[2 * b] >> (8 * h), x[2 * b + 1] >> (8 * h), magic);
                             // rows (elements) 32 b + 16 h + g and + 8, positions 4 t .. + 3 of the tile
                             const int e = 32 * b + 16 * h + g, c = tile * 2 + (t >> 1);
-                            *reinterpret_cast<uint2*>(dst + sw128(e, c) + 8 * (t & 1)) = make_uint2(v.x, v.y);
-                            *reinterpret_cast<uint2*>(dst + sw128(e + 8, c) + 8 * (t & 1)) = make_uint2(v.z, v.w);
+                            *reinterpret_cast<uint2*>(dst + sw128(e, c) + 8 * (t & 1)) = make_uint2(times(v.x, d.x), times(v.y, d.y));
+                            *reinterpret_cast<uint2*>(dst + sw128(e + 8, c) + 8 * (t & 1)) = make_uint2(times(v.z, d.x), times(v.w, d.y));
                         }
+                    }
                 } else {
                     uint8_t* dst = sm + S::kK + st * S::kAtoms * 8192;
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
+                    for (int b = 0; b < NB; b++) {
+                        const uint2 d = *reinterpret_cast<const uint2*>(scl + i * 32 * NB + ((g >> 1) * NB + b) * 8);
 #pragma unroll
                         for (int n = 0; n < 2; n++) {
+                            const uint32_t dd = __byte_perm(n ? d.y : d.x, 0u, g & 1 ? 0x3232u : 0x1010u);
                             const int row = tile * kKv4Tile + 4 * (g >> 1) + (g & 1) + 2 * n;
+                            const uint4 v = k_operands(x[2 * b + n], magic);
                             *reinterpret_cast<uint4*>(dst + (b >> 1) * 8192 + sw128(row, (b & 1) * 4 + t)) =
-                                k_operands(x[2 * b + n], magic);
+                                make_uint4(times(v.x, dd), times(v.y, dd), times(v.z, dd), times(v.w, dd));
                         }
+                    }
                 }
             }
-            if (is_v) {
-                // E follows the largest scale; the two V warps agree on it
-                __half2 big = __half2half2(__ushort_as_half(0));
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    big = __hmax2(big, __hmax2(__habs2(as_h2(sc[i].x)), __habs2(as_h2(sc[i].y))));
-                float dm = fmaxf(__half2float(__low2half(big)), __half2float(__high2half(big)));
-#pragma unroll
-                for (int i = 16; i > 0; i >>= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, i));
-                if (lane == 0) s_dm[st][list] = dm;
-                named_bar_sync(7, 64);
-                dm = fmaxf(s_dm[st][0], s_dm[st][1]);
-                if (dm > __int_as_float((127 + E) << 23)) {
-                    int e;
-                    frexpf(dm, &e);
-                    E = e;
-                }
-                if (list == 0 && lane == 0) {
-                    s_E[st] = E;
-                    s_lg[st] = fmaxf(lg2(dm) - (float)E, -7.0f);
-                }
-                const __half2 inv = __float2half2_rn(__int_as_float((127 - E) << 23));
-                if (lane < 4 * NB)
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        *reinterpret_cast<uint2*>(sm + S::kVs + ((st * NB + lane % NB) * kTcStep + (2 * list + i) * 16 + 4 * (lane / NB)) * 2) =
-                            make_uint2(as_u32(__hmul2(as_h2(sc[i].x), inv)), as_u32(__hmul2(as_h2(sc[i].y), inv)));
-            } else if (lane < 4 * NB) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float2 u = unpack(sc[i].x), v = unpack(sc[i].y);
-                    *reinterpret_cast<float4*>(sm + S::kKs + ((st * NB + lane % NB) * kTcStep + (2 * list + i) * 16 + 4 * (lane / NB)) * 4) =
-                        make_float4(u.x, u.y, v.x, v.y);
-                }
-            }
-            if (!is_v && lane == 0) s_there[st][list] = (int)there;
+            if (!is_v && lane == 0) s_there[st][half] = (int)there;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&b_ops_full[st]));
             named_bar_sync(5 + list, 64);  // both warps have read the records
-            if (ok && k + 2 < in.n) in.issue(k + 2, s);
+            if (ok && j + 2 < in.n) in.issue(j + 2, s);
         }
         if (!ok) in.abandon(0);
     } else if (warp == 8) {
         // -------------------------------------------------------- products
         constexpr uint32_t kIdS = (1u << 4) | ((uint32_t)(kTcStep >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        constexpr uint32_t kIdO = (1u << 4) | ((uint32_t)(32 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        for (int k = -1; k < steps; k++) {
-            if (k + 1 < steps) {  // S of the next step
-                const int st = (k + 1) & 1;
-                if (ok && !mbar_wait(smem_u32(&b_ops_full[st]), ((k + 1) >> 1) & 1)) ok = false;
-                if (ok && k >= 0 && !mbar_wait(smem_u32(&b_s_empty), k & 1)) ok = false;
+        constexpr uint32_t kIdO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        for (int k = -2; k < steps; k++) {
+            if (k + 2 < steps) {  // S of the step after the next
+                const int j = k + 2, st = j & 1, os = j % kTcOps;
+                if (ok && !mbar_wait(smem_u32(&b_ops_full[os]), (j / kTcOps) & 1)) ok = false;
+                if (ok && j >= 2 && !mbar_wait(smem_u32(&b_s_empty[st]), ((j >> 1) - 1) & 1)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 tc::tmem_fence_after();
                 if (tc::elect_one()) {
                     if (ok) {
 #pragma unroll
-                        for (int b = 0; b < NB; b++)
-#pragma unroll
-                            for (int x = 0; x < 2; x++) {
-                                const uint32_t off = (uint32_t)(64 * (b & 1) + 32 * x);
-                                tc::umma_f16(tmem + kSCol + 64 * b, tc::desc_sw128(sm32 + S::kQ + (b >> 1) * 16384 + off),
-                                             tc::desc_sw128(sm32 + S::kK + (st * S::kAtoms + (b >> 1)) * 8192 + off), kIdS,
-                                             x ? 1u : 0u);
-                            }
+                        for (int x = 0; x < 2 * NB; x++)
+                            tc::umma_f16(tmem + 64 * st, tc::desc_sw128(sm32 + S::kQ + (x >> 2) * 16384 + 32 * (x & 3)),
+                                         tc::desc_sw128(sm32 + S::kK + (os * S::kAtoms + (x >> 2)) * 8192 + 32 * (x & 3)), kIdS,
+                                         x ? 1u : 0u);
                     }
-                    tc::umma_commit(smem_u32(&b_s_full));
+                    tc::umma_commit(smem_u32(&b_s_full[st]));
                 }
                 __syncwarp();
             }
             if (k >= 0) {  // O of this one
-                const int st = k & 1;
-                if (ok && !mbar_wait(smem_u32(&b_p_full), k & 1)) ok = false;
+                const int st = k & 1, os = k % kTcOps;
+                if (ok && !mbar_wait(smem_u32(&b_p_full[st]), (k >> 1) & 1)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 tc::tmem_fence_after();
                 if (tc::elect_one()) {
                     if (ok) {
 #pragma unroll
-                        for (int b = 0; b < NB; b++)
-#pragma unroll
-                            for (int x = 0; x < 4; x++)
-                                tc::umma_f16_ts(tmem + kOCol + 32 * b, tmem + kPCol + 32 * b + 8 * x,
-                                                tc::desc_sw128(sm32 + S::kV + (st * NB + b) * 4096 + 32 * x), kIdO,
-                                                k > 0 || x > 0 ? 1u : 0u);
+                        for (int x = 0; x < 4; x++)
+                            tc::umma_f16_ts(tmem + kOCol + st * HD, tmem + kPCol + 32 * st + 8 * x,
+                                            tc::desc_sw128(sm32 + S::kV + os * NB * 4096 + 32 * x), kIdO, k > 1 || x > 0 ? 1u : 0u);
                     }
-                    tc::umma_commit(smem_u32(&b_pv_done));
-                    tc::umma_commit(smem_u32(&b_ops_empty[st]));
+                    tc::umma_commit(smem_u32(&b_pv_done[st]));
+                    tc::umma_commit(smem_u32(&b_ops_empty[os]));
                 }
                 __syncwarp();
             }
         }
-        // the last commit's arrival, which nobody else waits for, may not find
-        // the CTA gone
-        if (ok && steps > 0 && !mbar_wait(smem_u32(&b_ops_empty[(steps - 1) & 1]), ((steps - 1) >> 1) & 1)) ok = false;
+        // the last commits' arrivals, which nobody else may wait for, may not
+        // find the CTA gone
+        for (int k = max(0, steps - kTcOps); k < steps; k++)
+            if (ok && !mbar_wait(smem_u32(&b_ops_empty[k % kTcOps]), (k / kTcOps) & 1)) ok = false;
         if (!ok && lane == 0) atomicExch(p.err, 1);
     } else {
         // --------------------------------------------------------- softmax
@@ -1394,141 +1438,138 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         const int rpos = live ? o.pos0 + i : -1;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
         const float qs = s_qs[row];
+        const uint32_t s_at = lanes + 64 * h, p_at = lanes + kPCol + 32 * h, o_at = lanes + kOCol + HD * h;
         float m = -INFINITY, l = 0.0f;
-        int E = 0;
-        for (int k = 0; k < steps; k++) {
-            const int st = k & 1;
-            if (ok && !mbar_wait(smem_u32(&b_ops_full[st]), (k >> 1) & 1)) ok = false;
-            if (ok && !mbar_wait(smem_u32(&b_s_full), k & 1)) ok = false;
+        uint32_t bad = 0;  // blocks of O that a value which is not a number reaches
+        int E = kTcLow;
+        for (int k = h; k < steps; k += 2) {
+            const int ph = (k >> 1) & 1, os = k % kTcOps;
+            if (ok && !mbar_wait(smem_u32(&b_ops_full[os]), (k / kTcOps) & 1)) ok = false;
+            if (ok && !mbar_wait(smem_u32(&b_s_full[h]), ph)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             tc::tmem_fence_after();
-            // ---- scores of positions j0 .. j0 + 31
-            const int j0 = (t0 + 4 * k) * kKv4Tile + 32 * h;
-            float2 sc[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) sc[j] = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                uint32_t a[32];
-                tc::tmem_ld32(lanes + kSCol + 64 * b + 32 * h, a);
-                tc::tmem_wait_ld();
-                const float4* d = reinterpret_cast<const float4*>(sm + S::kKs + ((st * NB + b) * kTcStep + 32 * h) * 4);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float4 v = d[j];
-                    sc[2 * j] = fma2(make_float2(__uint_as_float(a[4 * j]), __uint_as_float(a[4 * j + 1])), make_float2(v.x, v.y), sc[2 * j]);
-                    sc[2 * j + 1] = fma2(make_float2(__uint_as_float(a[4 * j + 2]), __uint_as_float(a[4 * j + 3])), make_float2(v.z, v.w), sc[2 * j + 1]);
-                }
-            }
+            // ---- scores of positions j0 .. j0 + 63
+            const int j0 = (t0 + 4 * k) * kKv4Tile;
+            uint32_t a[2][32];
+            tc::tmem_ld32(s_at, a[0]);
+            tc::tmem_ld32(s_at + 32, a[1]);
+            tc::tmem_wait_ld();
             tc::tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&b_s_empty));
+            if (lane == 0) mbar_arrive(smem_u32(&b_s_empty[h]));
+            const float f = fmaxf(qs * s_kf[os], 1.2e-38f);  // (times -inf of a masked place)
+            const int e = s_E[os];
             // ---- which of them the row sees
-            const uint32_t there = (uint32_t)s_there[st][h];
-            const int hi = min(min(rpos + 1, o.held) - j0, 32), lo = p.window > 0 ? max(rpos - p.window + 1 - j0, 0) : 0;
-            uint32_t sees = (hi >= 32 ? 0xFFFFFFFFu : hi > 0 ? (1u << hi) - 1u : 0u) & (lo >= 32 ? 0u : 0xFFFFFFFFu << lo);
-            sees &= (there & 1u ? 0xFFFFu : 0u) | (there & 2u ? 0xFFFF0000u : 0u);
-            const bool full = __all_sync(0xffffffffu, sees == 0xFFFFFFFFu);
+            uint32_t sees[2];
             float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                sc[j] = mul2(sc[j], make_float2(qs, qs));
-                if (!full) {
-                    if (!((sees >> (2 * j)) & 1u)) sc[j].x = -INFINITY;
-                    if (!((sees >> (2 * j + 1)) & 1u)) sc[j].y = -INFINITY;
+            for (int i = 0; i < 2; i++) {
+                const uint32_t there = (uint32_t)s_there[os][i];
+                const int at = j0 + 32 * i;
+                const int hi = min(min(rpos + 1, o.held) - at, 32), lo = p.window > 0 ? max(rpos - p.window + 1 - at, 0) : 0;
+                sees[i] = (hi >= 32 ? 0xFFFFFFFFu : hi > 0 ? (1u << hi) - 1u : 0u) & (lo >= 32 ? 0u : 0xFFFFFFFFu << lo);
+                sees[i] &= (there & 1u ? 0xFFFFu : 0u) | (there & 2u ? 0xFFFF0000u : 0u);
+                if (__any_sync(0xffffffffu, sees[i] != 0xFFFFFFFFu)) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (!((sees[i] >> j) & 1u)) a[i][j] = 0xFF800000u;  // -inf
                 }
-                mx = fmaxf(mx, fmaxf(sc[j].x, sc[j].y));
+#pragma unroll
+                for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(a[i][j]));
             }
-            s_mx[st][h][row] = mx;
-            named_bar_sync(1 + q, 64);
-            mx = fmaxf(mx, s_mx[st][h ^ 1][row]) + s_lg[st];
-            // ---- move the row's reference or the scales' power where they grew
-            const int e = s_E[st];
-            float al = k > 0 ? __int_as_float((127 + max(E - e, -126)) << 23) : 1.0f;
-            E = e;
+            if (s_any_nan[os][0] | s_any_nan[os][1]) {
+                for (int b = 0; b < NB; b++)
+                    if ((s_nan[os][0][b] & sees[0]) | (s_nan[os][1][b] & sees[1])) bad |= 1u << b;
+            }
+            mx *= f;
+            // ---- move the row's power of V or its reference where they grew
+            float al = 1.0f;
+            if (mx > -INFINITY && e > E) {
+                al = __int_as_float((127 + E - e) << 23);
+                E = e;
+            }
             if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
-                const float f = m == -INFINITY ? 0.0f : ex2(m - mx);
-                al *= f;
-                l *= f;
+                const float d = m == -INFINITY ? 0.0f : ex2(m - mx);
+                al *= d;
+                l *= d;
                 m = mx;
             }
-            const float base = m == -INFINITY ? 0.0f : m;
-            uint32_t ph[16];
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float2 x = add2(sc[j], make_float2(-base, -base));
-                const float2 y = make_float2(ex2(x.x), ex2(x.y));
-                sum = add2(sum, y);
-                ph[j] = pack(y.x, y.y);
-            }
-            l += sum.x + sum.y;
-            // ---- O and P are free once the products of the step before are done
-            if (ok && k > 0 && !mbar_wait(smem_u32(&b_pv_done), (k - 1) & 1)) ok = false;
+            const float base = (m == -INFINITY ? 0.0f : m) + (float)(E - e) - kTcUp;
+            // ---- P and O are free once the group's last products are done
+            if (ok && k >= 2 && !mbar_wait(smem_u32(&b_pv_done[h]), ph ^ 1)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             tc::tmem_fence_after();
-            if (k > 0 && __any_sync(0xffffffffu, al != 1.0f)) {
-#pragma unroll
-                for (int c = 0; c < NB; c++) {  // this warp's half of the columns
-                    uint32_t a[16];
-                    const uint32_t at = lanes + kOCol + 16 * (h * NB + c);
-                    tc::tmem_ld16(at, a);
+            if (k >= 2 && __any_sync(0xffffffffu, al != 1.0f)) {
+#pragma unroll 1
+                for (int c = 0; c < 2 * NB; c++) {
+                    uint32_t v[16];
+                    tc::tmem_ld16(o_at + 16 * c, v);
                     tc::tmem_wait_ld();
 #pragma unroll
-                    for (int x = 0; x < 16; x++) a[x] = __float_as_uint(__uint_as_float(a[x]) * al);
-                    tc::tmem_st16u(at, a);
+                    for (int x = 0; x < 16; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * al);
+                    tc::tmem_st16u(o_at + 16 * c, v);
                 }
             }
+            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const uint4* d = reinterpret_cast<const uint4*>(sm + S::kVs + ((st * NB + b) * kTcStep + 32 * h) * 2);
-                uint32_t a[16];
+            for (int i = 0; i < 2; i++) {
+                uint32_t pk[16];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint4 v = d[j];
-                    a[4 * j] = as_u32(__hmul2(as_h2(ph[4 * j]), as_h2(v.x)));
-                    a[4 * j + 1] = as_u32(__hmul2(as_h2(ph[4 * j + 1]), as_h2(v.y)));
-                    a[4 * j + 2] = as_u32(__hmul2(as_h2(ph[4 * j + 2]), as_h2(v.z)));
-                    a[4 * j + 3] = as_u32(__hmul2(as_h2(ph[4 * j + 3]), as_h2(v.w)));
+                for (int j = 0; j < 16; j++) {
+                    const float2 x = fma2(make_float2(__uint_as_float(a[i][2 * j]), __uint_as_float(a[i][2 * j + 1])), make_float2(f, f), make_float2(-base, -base));
+                    const float2 y = make_float2(ex2(x.x), ex2(x.y));
+                    sum = add2(sum, y);
+                    pk[j] = pack(y.x, y.y);
                 }
-                if (!full) {  // whatever a hidden position holds (a NaN scale too) does not enter
-#pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        a[j] &= ((sees >> (2 * j)) & 1u ? 0xFFFFu : 0u) | ((sees >> (2 * j + 1)) & 1u ? 0xFFFF0000u : 0u);
-                }
-                tc::tmem_st16u(lanes + kPCol + 32 * b + 16 * h, a);
+                tc::tmem_st16u(p_at + 16 * i, pk);
             }
+            l = fmaf(sum.x + sum.y, __int_as_float((127 + E - e) << 23), l);
             tc::tmem_wait_st();
             tc::tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&b_p_full));
+            if (lane == 0) mbar_arrive(smem_u32(&b_p_full[h]));
         }
-        if (ok && steps > 0 && !mbar_wait(smem_u32(&b_pv_done), (steps - 1) & 1)) ok = false;
+        const int last = steps - 1 - ((steps - 1 - h) & 1);  // of the group
+        if (ok && last >= 0 && !mbar_wait(smem_u32(&b_pv_done[h]), (last >> 1) & 1)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok && lane == 0) atomicExch(p.err, 1);
-        tc::tmem_fence_after();
+        // ---- the row's even and odd steps together
+        s_m[h][row] = m;
         s_l[h][row] = l;
+        s_bound[h][row] = __int_as_float((127 + E) << 23);
+        s_bad[h][row] = bad;
+        tc::tmem_fence_before();
         named_bar_sync(1 + q, 64);
-        l += s_l[h ^ 1][row];
+        tc::tmem_fence_after();
+        m = fmaxf(s_m[0][row], s_m[1][row]);
+        const float w0 = weight(s_m[0][row], m), w1 = weight(s_m[1][row], m);
+        l = s_l[0][row] * w0 + s_l[1][row] * w1;
+        bad = s_bad[0][row] | s_bad[1][row];
         // ---- columns 16 NB h .. of the row
         const bool any = l != 0.0f;  // (not a number counts)
-        const float bound = __int_as_float((127 + E) << 23), f = p.splits == 1 ? bound / l : bound;
+        const float f = p.splits == 1 ? 1.0f / l : 1.0f, f0 = s_bound[0][row] * w0 * f, f1 = s_bound[1][row] * w1 * f;
         const int64_t at = (tok * p.n_heads + head) * p.splits + split;
         T* out = static_cast<T*>(p.out) + tok * p.ot + head * p.oh;
 #pragma unroll
         for (int c = 0; c < NB; c++) {
-            uint32_t a[16];
+            uint32_t a0[16], a1[16];
             const int col = 16 * (h * NB + c);
-            if (steps > 0) {
-                tc::tmem_ld16(lanes + kOCol + col, a);
-                tc::tmem_wait_ld();
-            }
+            if (steps > 0) tc::tmem_ld16(lanes + kOCol + col, a0);
+            if (steps > 1) tc::tmem_ld16(lanes + kOCol + HD + col, a1);
+            tc::tmem_wait_ld();
             if (!live) continue;
+            const bool not_number = (bad >> (col >> 5)) & 1u;
 #pragma unroll
-            for (int x = 0; x < 16; x++) {
-                const float v = any ? __uint_as_float(a[x]) * f : 0.0f;
-                if (p.splits == 1) out[col + x] = from_f32<T>(v);
-                else p.part[at * HD + col + x] = v;
+            for (int x = 0; x < 16; x += 8) {
+                float v[8];
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    v[y] = any ? __uint_as_float(a0[x + y]) * f0 : 0.0f;
+                    if (any && steps > 1) v[y] = fmaf(__uint_as_float(a1[x + y]), f1, v[y]);
+                    if (not_number) v[y] = __int_as_float(0x7fffffff);
+                }
+                if (p.splits == 1) store8(out + col + x, p.wide_out, v);
+                else store8(p.part + at * HD + col + x, true, v);
             }
         }
         if (p.splits > 1 && live && h == 0) p.ml[at] = make_float2(m, l);
@@ -1693,7 +1734,13 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
     // since the other half of the operand would be empty
     pl.mode = a->dtype == RQ_F32 || rows <= 8 ? kSplit8 : kOne16;
     pl.R = pl.mode == kOne16 ? 16 : 8;
-    pl.rows = rows > 2 * pl.R;
+    // Where the many-rows forms win, few rows -> many rows (us, 8 heads a kv head of
+    // 8, head_dim 128): 16 bits at 16 rows, 16 x 2048 keys 44 -> 42, 64 x 1024
+    // 77 -> 99, 1 x 40000 46 -> 50; at 24 rows 42 -> 42, 117 -> 100, 66 -> 51; at
+    // 128 rows 183 -> 43, 384 -> 105, 206 -> 55.  f32 at 32 rows 64 -> 94,
+    // 118 -> 152, 67 -> 86; at 48 rows 86 -> 101, 166 -> 156, 89 -> 88; at 64 rows
+    // 108 -> 107, 215 -> 161, 126 -> 90.
+    pl.rows = rows > (a->dtype == RQ_F32 ? 48 : 16);
     const int64_t tiles_of_row = (rows + pl.R - 1) / pl.R;
     int64_t len = a->table_width * c->page_size;
     if (a->max_len > 0) len = std::min(len, a->max_len);
@@ -1752,6 +1799,7 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.ot = a->out_stride[0];
     p.oh = a->out_stride[1];
     p.wide = (((uintptr_t)a->q | (uintptr_t)(p.qt * (int64_t)size) | (uintptr_t)(p.qh * (int64_t)size)) & 15) == 0;
+    p.wide_out = (((uintptr_t)a->out | (uintptr_t)(p.ot * (int64_t)size) | (uintptr_t)(p.oh * (int64_t)size)) & 15) == 0;
     p.n_tokens = a->n_tokens;
     p.n_heads = (int)a->n_heads;
     p.group = (int)(a->n_heads / c->n_kv);

@@ -4,8 +4,8 @@ together, against plain implementations in 64 bits.
 
 Tolerances.  The cache's values are exact (a code is the nearest multiple of
 an f16 scale, decided without rounding), so append / read compare for equality
-in f32 and to one rounding (2^-9 bf16, 2^-12 f16 relative, at most half a step
-of the type) else.  Attention with f32 queries: queries and probabilities
+in f32 and to one rounding (half a step of the type: 2^-8 bf16, 2^-11 f16
+relative) else.  Attention with f32 queries: queries and probabilities
 enter the products as f16 hi + lo (22 bits), sums are f32; scores of the size
 used here (|s| <= 32) carry at most 32 * 2^-23 absolute error from the f32 sum,
 i.e. 4e-6 relative in a probability, so 2e-5 of the row's largest value holds
@@ -15,7 +15,11 @@ probabilities are rounded to f16 and multiplied by the value's scale in f16:
 two roundings of 2^-11, so the sum of p_j v_j is off by at most (2 * 2^-11 +
 2^-22) sum p_j |v_j|, to which the output's own rounding adds half a step of its
 type times |o|, and the f32 parts above 2e-5 of sum p_j |v_j|; the tests take
-the sum of p_j |v_j| from the reference ("reach")."""
+the sum of p_j |v_j| from the reference ("reach").  More than 16 rows of 16-bit
+queries a kv head take the form with rounded operands: there the second rounding
+of 2^-11 is the value's, and the keys are rounded to f16 as well, which moves a
+score by at most D = 2^-11 scale sum_d |q_d k_d| and so, since every weight and
+their sum move by at most exp(+-D), the output by (exp(2 D) - 1) sum p_j |v_j|."""
 import math
 
 import numpy as np
@@ -113,11 +117,12 @@ def test_not_a_number_stays_in_its_block_and_infinities_saturate(gen):
 
 def attention_ref(q, kval, vval, table, page, kv_lens, cu, scale, window, n_pages):
     """float64, row by row; kval, vval [slots, kv, hd] float64.  Returns the
-    outputs and, for the tolerance, sum p |v| of each."""
+    outputs and, for the tolerance, sum p |v| of each and what rounded keys move."""
     n, H, hd = q.shape
     kv = kval.shape[1]
     out = np.full((n, H, hd), np.nan)
-    reach = out.copy()
+    reach, moved = out.copy(), np.zeros((n, H, 1))
+    many = H // kv * int(np.diff(cu).max()) > 16
     for b in range(table.shape[0]):
         L, nq = max(int(kv_lens[b]), 0), int(cu[b + 1] - cu[b])
         for i in range(nq):
@@ -136,7 +141,10 @@ def attention_ref(q, kval, vval, table, page, kv_lens, cu, scale, window, n_page
                 p = np.exp(s - s.max())
                 out[cu[b] + i, h] = (p / p.sum()) @ vval[slots, h // (H // kv)]
                 reach[cu[b] + i, h] = (p / p.sum()) @ np.abs(vval[slots, h // (H // kv)])
-    return out, reach
+                if many:
+                    d = 2.0 ** -11 * abs(scale) * (np.abs(kval[slots, h // (H // kv)]) @ np.abs(q[cu[b] + i, h]))
+                    moved[cu[b] + i, h] = np.expm1(min(2 * d.max(), 100))
+    return out, reach, moved
 
 
 def fill(cache, gen, kind="f32"):
@@ -150,12 +158,12 @@ def fill(cache, gen, kind="f32"):
 
 def close(got, ref, rows, kind):
     """The rows (a slice or list) of the reference against got, row for row."""
-    want, reach = ref[0][rows], ref[1][rows]
+    want, reach, moved = ref[0][rows], ref[1][rows], ref[2][rows]
     got = got.double().cpu().numpy()
     if kind == "f32":
         tol = 2e-5 * np.abs(want).max(-1, keepdims=True) + 1e-30
     else:
-        tol = (2 * 2.0 ** -11 + 2.0 ** -22 + 2e-5) * reach + HALF_STEP[kind] * np.abs(want) + 2.0 ** -24
+        tol = (2 * 2.0 ** -11 + 2.0 ** -22 + 2e-5 + moved) * reach + HALF_STEP[kind] * np.abs(want) + 2.0 ** -24
     bad = np.abs(got - want) > tol
     assert not bad.any(), (np.abs(got - want) / tol).max()
 
@@ -288,6 +296,42 @@ def test_prompts_over_missing_pages_and_odd_rows(gen, kind):
     one = cache.attention(q[100:101], table[1:], torch.tensor([31], dtype=torch.int32, device="cuda"))
     assert one[0, 3].isnan().all() and not one[0, [0, 1, 2, 4, 5, 6, 7]].isnan().any()
     assert (out[140:] == 5).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.05, -0.05, 0.0])
+@pytest.mark.parametrize("falls", [False, True])
+def test_prompts_over_values_of_every_size(gen, kind, scale, falls):
+    """The form with rounded operands: values that grow or fall by 10^6 over
+    the sequence, and at its last position, which the last query alone sees,
+    the cache's largest keys and values, 2^24 times their neighbours'.  (The
+    scores stay within e^-4.4 of one another, so that no weight comes near the
+    end of f16's range.)  Values that are not numbers in the last one's place
+    leave the other queries within the same bounds."""
+    from rustyllm_b200.kv4 import KV4Cache
+    n, nq, kv, hd = 203, 101, 2, 96
+    cache = KV4Cache(16, 16, kv, hd)
+    k, v = make(gen, n, kv, hd, kind)
+    k = (k.float() / k.float().abs().amax() * 4).to(TYPES[kind])
+    size = torch.logspace(-2, 4, n, device="cuda")
+    v = (v.float() / v.float().abs().amax(-1, keepdim=True) * (size.flip(0) if falls else size)[:, None, None]).to(TYPES[kind])
+    k[-1] = v[-1] = 6e4 if kind == "f16" else 5e5
+    slots = torch.arange(n, dtype=torch.int32, device="cuda") + 16
+    cache.append(k, v, slots)
+    every = torch.arange(256, dtype=torch.int32, device="cuda")
+    rk, rv = cache.read(every)
+    table = torch.arange(1, 16, dtype=torch.int32, device="cuda")[None]
+    cu = np.array([0, nq], np.int32)
+    q = torch.randn(nq, 8, hd, generator=gen, device="cuda").clamp(-4, 4).to(TYPES[kind])
+    want = attention_ref(q.double().cpu().numpy(), rk.double().cpu().numpy(), rv.double().cpu().numpy(), table.cpu().numpy(),
+                         16, [n], cu, scale, 0, 16)
+    lens, cu = torch.tensor([n], dtype=torch.int32, device="cuda"), torch.from_numpy(cu).cuda()
+    got = cache.attention(q, table, lens, cu_q=cu, max_q=nq, scale=scale)
+    close(got[:-1], want, slice(0, nq - 1), kind)
+    v[-1] = math.nan
+    cache.append(k, v, slots)
+    again = cache.attention(q, table, lens, cu_q=cu, max_q=nq, scale=scale)
+    close(again[:-1], want, slice(0, nq - 1), kind)
 
 
 def test_slots_past_four_gigabytes(gen):
