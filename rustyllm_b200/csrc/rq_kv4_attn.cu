@@ -13,23 +13,24 @@
 //    that one bulk copy brought to shared memory.  The warps join through shared
 //    memory, the pieces of a unit that went to several CTAs through a second
 //    launch.
-//  - many rows of f32 queries (prompts), on mma.m16n8k16: the warps hold
+//  - many rows of f32 and f16 queries (prompts), on mma.m16n8k16: the warps hold
 //    different rows, two operand tiles each; the records are turned into f16
 //    operands in shared memory once for all four, and an operand read from there
 //    serves two tiles of rows (with one tile a warp, reading them took as long as
 //    the products).
-//  - many rows of 16-bit queries, on tcgen05: see there.
+//  - many rows of bf16 queries, on tcgen05: see there.
 //
 // The first two do not round the cache: q is scaled by a power of two to [-1, 1]
-// and split into f16 hi + lo (f32 input; 16-bit inputs need hi alone), the K
+// and split into f16 hi + lo (16-bit inputs need hi alone), the K
 // scales multiply the f32 block sums, and the V scales multiply the
-// probabilities, P_jb = p_j dV_jb.  For f32 the hi and lo parts are the two row
-// halves of one m16 operand: eight query rows a tile, no extra instructions.
+// probabilities, P_jb = p_j dV_jb.  The hi and lo parts are the two row halves of
+// one m16 operand: eight query rows a tile, no extra instructions.  (Nine to
+// sixteen bf16 rows take both halves for one part.)
 //
-// P enters as f16: for f32, p = ph + pl (22 bits) and ph d = h + r exactly (h
+// P enters as f16: in two parts, p = ph + pl (22 bits) and ph d = h + r exactly (h
 // the rounded product, r = fma(ph, d, -h)), so P = h + (r + pl d) costs three
-// packed operations a pair of tokens; 16-bit outputs take h alone (two
-// roundings of 2^-11, an eighth of bf16's own and as much as f16's).  f16's range
+// packed operations a pair of tokens; one part takes h alone (two roundings of
+// 2^-11, an eighth of bf16's own).  f16's range
 // is kept whatever the scale of V: the scales are divided by a power of two 2^E
 // that follows the largest one seen, and the running maximum m is taken over s_j
 // + log2 of the lane's largest scale (not below 2^-7), so that |P| <= 2^8 with the
@@ -206,7 +207,13 @@ struct Warp {
     uint4* as;
     float qs[H];      // back from the normalised row, times the softmax scale
     int rpos[H];      // position of the row's query; -1: no row
-    float oacc[MT][NB][4][4];
+    // The tensor cores cut their sums off rather than round them: over the tiles
+    // of a long walk that grows to 1.3e-5 of the output (60000 positions), nothing
+    // to 16-bit outputs, but for f32 a tile's products are summed alone and added
+    // here (7e-7; 1 to 5 % slower).
+    static constexpr bool kAlone = sizeof(T) == 4;
+    static constexpr int kAcc = kAlone ? 2 : 4;  // kAlone: hi and lo rows together
+    float oacc[MT][NB][4][kAcc];
     float m[H], l[H];
     float E;
     float bound;      // 2^E
@@ -276,7 +283,7 @@ struct Warp {
 #pragma unroll
                 for (int n = 0; n < 4; n++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) oacc[mt][b][n][i] = 0.0f;
+                    for (int i = 0; i < kAcc; i++) oacc[mt][b][n][i] = 0.0f;
         __syncwarp();  // the operands in shared memory are there
         set_scale(-15);
         const int i0 = r0 / p.group, i1 = min(o.n_q - 1, (r0 + R - 1) / p.group);
@@ -290,6 +297,18 @@ struct Warp {
         bound = __int_as_float((127 + e) << 23);
         inv = __float2half2_rn(__int_as_float((127 - e) << 23));
     }
+    static __device__ __forceinline__ void add_products(float (&o)[kAcc], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        if constexpr (kAlone) {
+            float c[4];
+            mma16816_0(c, a, b0, b1);
+            const float2 d = add2(make_float2(c[0], c[1]), make_float2(-c[2], -c[3]));
+            const float2 s = add2(make_float2(o[0], o[1]), d);
+            o[0] = s.x;
+            o[1] = s.y;
+        } else {
+            mma16816(o, a, b0, b1);
+        }
+    }
     __device__ __forceinline__ void scale_rows(const float (&f)[H]) {
         // rows g and g + 8 of an accumulator: in the 8-row mode both halves
         // belong to row g
@@ -299,10 +318,8 @@ struct Warp {
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
-                    oacc[mt][b][n][0] *= f[mt * HH];
-                    oacc[mt][b][n][1] *= f[mt * HH];
-                    oacc[mt][b][n][2] *= f[mt * HH + HH - 1];
-                    oacc[mt][b][n][3] *= f[mt * HH + HH - 1];
+#pragma unroll
+                    for (int i = 0; i < kAcc; i++) oacc[mt][b][n][i] *= f[mt * HH + (i < 2 ? 0 : HH - 1)];
                 }
     }
 
@@ -533,8 +550,8 @@ struct Warp {
                     const uint4 w = src.vop(i, b, half);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        mma16816(oacc[mt][b][2 * half], a[mt], w.x, w.y);
-                        mma16816(oacc[mt][b][2 * half + 1], a[mt], w.z, w.w);
+                        add_products(oacc[mt][b][2 * half], a[mt], w.x, w.y);
+                        add_products(oacc[mt][b][2 * half + 1], a[mt], w.z, w.w);
                     }
                 }
             }
@@ -566,11 +583,14 @@ struct Warp {
     }
     // elements 32 b + 8 n + 2 t, + 1 of row h
     __device__ __forceinline__ float2 value(int b, int n, int h) const {
-        const float(&o)[4] = oacc[h / HH][b][n];
-        float2 v = h % HH ? make_float2(o[2], o[3]) : make_float2(o[0], o[1]);
-        if (MODE == kSplit8) {
-            v.x -= o[2];
-            v.y -= o[3];
+        const float(&o)[kAcc] = oacc[h / HH][b][n];
+        float2 v = make_float2(o[0], o[1]);
+        if constexpr (!kAlone) {
+            if (h % HH) v = make_float2(o[2], o[3]);
+            if (MODE == kSplit8) {
+                v.x -= o[2];
+                v.y -= o[3];
+            }
         }
         return make_float2(v.x * bound, v.y * bound);
     }
@@ -1119,10 +1139,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
     }
 }
 
-// Many rows of 16-bit queries: 128 rows and steps of 64 positions on tcgen05.
+// Many rows of bf16 queries: 128 rows and steps of 64 positions on tcgen05.
 //
-// K and V enter as f16 values (c - 8) d / 2^E, one rounding of 2^-11 of each:
-// as much as the queries' own type gives them, and for V as P's.  (Kept exact --
+// K and V enter as f16 values (c - 8) d / 2^E, one rounding of 2^-11 of each, and
+// P as f16: an eighth each of the rounding that bf16 gives the output.  (Kept exact --
 // a product a block, scaled in the softmax, P times each block's scales -- S and
 // P crossed TMEM head_dim / 32 times, for 1.3 times the softmax's time.)  E is
 // the step's: zero scales apart, the largest one comes to [2^11, 2^12) -- so
@@ -1667,19 +1687,22 @@ struct Fns {
 template <int NB, int MODE, typename T>
 Fns fns_of(bool rows) {
     constexpr int R = MODE == kOne16 ? 16 : 8;
-    if constexpr (sizeof(T) == 4) {
-        if (rows)
+    if (rows) {
+        if constexpr (MODE == kOne16)
+            return Fns{(const void*)kv4_attn_tc_kernel<NB, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
+        else
             return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
-    } else if constexpr (MODE == kOne16) {
-        if (rows) return Fns{(const void*)kv4_attn_tc_kernel<NB, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
     }
     return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
 }
 template <int NB, typename T>
 Fns fns_of(int mode, bool rows) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
         if (mode == kOne16) return fns_of<NB, kOne16, T>(rows);
-    return fns_of<NB, kSplit8, T>(rows);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        return Fns{(const void*)kv4_attn_kernel<NB, kSplit8, T>, (const void*)kv4_join_kernel<NB, 8, T>};
+    else
+        return fns_of<NB, kSplit8, T>(rows);
 }
 template <typename T>
 Fns fns_of(int nb, int mode, bool rows) {
@@ -1730,17 +1753,19 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
     Plan pl{};
     const int64_t group = a->n_heads / c->n_kv;
     const int64_t rows = group * (a->cu_q ? a->max_q : 1);
-    // f32 queries need the two parts; up to eight 16-bit rows take them too,
-    // since the other half of the operand would be empty
-    pl.mode = a->dtype == RQ_F32 || rows <= 8 ? kSplit8 : kOne16;
+    // f32 needs the two parts, and f16 does too: its own output rounding is no
+    // larger than the roundings of one part (errors of 1.4 to 1.8 of the output
+    // rounding's alone, where two parts leave 1.0; bf16: 1.02).  Up to eight bf16
+    // rows take them as well, since the other half of the operand would be empty.
+    pl.mode = a->dtype != RQ_BF16 || rows <= 8 ? kSplit8 : kOne16;
     pl.R = pl.mode == kOne16 ? 16 : 8;
     // Where the many-rows forms win, few rows -> many rows (us, 8 heads a kv head of
-    // 8, head_dim 128): 16 bits at 16 rows, 16 x 2048 keys 44 -> 42, 64 x 1024
+    // 8, head_dim 128): bf16 at 16 rows, 16 x 2048 keys 44 -> 42, 64 x 1024
     // 77 -> 99, 1 x 40000 46 -> 50; at 24 rows 42 -> 42, 117 -> 100, 66 -> 51; at
     // 128 rows 183 -> 43, 384 -> 105, 206 -> 55.  f32 at 32 rows 64 -> 94,
     // 118 -> 152, 67 -> 86; at 48 rows 86 -> 101, 166 -> 156, 89 -> 88; at 64 rows
     // 108 -> 107, 215 -> 161, 126 -> 90.
-    pl.rows = rows > (a->dtype == RQ_F32 ? 48 : 16);
+    pl.rows = rows > (a->dtype == RQ_BF16 ? 16 : 48);
     const int64_t tiles_of_row = (rows + pl.R - 1) / pl.R;
     int64_t len = a->table_width * c->page_size;
     if (a->max_len > 0) len = std::min(len, a->max_len);
@@ -1757,7 +1782,7 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
         pl.pieces = pl.ctas > 1 ? 2 * pl.ctas * pl.R : 0;
         return pl;
     }
-    pl.tc = a->dtype != RQ_F32;
+    pl.tc = a->dtype == RQ_BF16;
     pl.R = pl.tc ? kTcRows : 2 * kWarps * pl.R;
     pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
     const int64_t units = a->batch * c->n_kv * pl.row_tiles;

@@ -10,13 +10,14 @@ enter the products as f16 hi + lo (22 bits), sums are f32; scores of the size
 used here (|s| <= 32) carry at most 32 * 2^-23 absolute error from the f32 sum,
 i.e. 4e-6 relative in a probability, so 2e-5 of the row's largest value holds
 for the output.  16-bit queries are exact in f16 (bf16 after the row's power of
-two; elements below 2^-14 of the row's largest lose at most 2^-25 of it).  Their
-probabilities are rounded to f16 and multiplied by the value's scale in f16:
+two; elements below 2^-14 of the row's largest lose at most 2^-25 of it).  f16
+takes the same two parts of a probability as f32.  More than eight bf16 rows a kv
+head take one part, for which the bound is made: their probabilities are rounded to f16 and multiplied by the value's scale in f16:
 two roundings of 2^-11, so the sum of p_j v_j is off by at most (2 * 2^-11 +
 2^-22) sum p_j |v_j|, to which the output's own rounding adds half a step of its
 type times |o|, and the f32 parts above 2e-5 of sum p_j |v_j|; the tests take
-the sum of p_j |v_j| from the reference ("reach").  More than 16 rows of 16-bit
-queries a kv head take the form with rounded operands: there the second rounding
+the sum of p_j |v_j| from the reference ("reach").  More than 16 bf16 rows
+a kv head take the form with rounded operands: there the second rounding
 of 2^-11 is the value's, and the keys are rounded to f16 as well, which moves a
 score by at most D = 2^-11 scale sum_d |q_d k_d| and so, since every weight and
 their sum move by at most exp(+-D), the output by (exp(2 D) - 1) sum p_j |v_j|."""
@@ -296,6 +297,34 @@ def test_prompts_over_missing_pages_and_odd_rows(gen, kind):
     one = cache.attention(q[100:101], table[1:], torch.tensor([31], dtype=torch.int32, device="cuda"))
     assert one[0, 3].isnan().all() and not one[0, [0, 1, 2, 4, 5, 6, 7]].isnan().any()
     assert (out[140:] == 5).all()
+
+
+@pytest.mark.parametrize("kind,qn,ratio", [("f32", 1, 0), ("f32", 13, 0), ("f16", 2, 1.5), ("f16", 13, 1.5), ("bf16", 2, 1.5),
+                                           ("bf16", 13, 1.5)])
+def test_error_does_not_grow_with_the_walk(gen, kind, qn, ratio):
+    """24000 positions of one kv head under 8 query heads.  f32: per tile of 16
+    the products' cut-off sums lose at most 16 * 2^-23 of sum p |v|, hi + lo
+    parts 2^-21, scores within 16 carry 16 * 2^-22 into the weights, and adding
+    1500 tiles in f32 walks sqrt(1500) * 2^-25: 7e-6 of the output if all signs
+    agreed, 2e-6 in the mean over rows and elements, whose signs are free.  16 bits:
+    no more than 1.5 times what rounding the output alone leaves (bf16: three
+    roundings of an eighth beside it, sqrt(1 + 3 / 64))."""
+    from rustyllm_b200.kv4 import KV4Cache
+    n = 24000
+    cache = KV4Cache(n // 16, 16, 1, 64)
+    k, v = make(gen, n, 1, 64, kind)
+    every = torch.arange(n, dtype=torch.int32, device="cuda")
+    cache.append(k, v, every)
+    rk, rv = (x[:, 0].double() for x in cache.read(every))
+    q = torch.randn(qn, 8, 64, generator=gen, device="cuda").to(TYPES[kind])
+    got = cache.attention(q, every[:n // 16][None], torch.tensor([n], dtype=torch.int32, device="cuda"),
+                          cu_q=torch.tensor([0, qn], dtype=torch.int32, device="cuda"), max_q=qn).double()
+    s = q.double() @ rk.T * 64 ** -0.5
+    s.masked_fill_(every > (n - qn + torch.arange(qn, device="cuda"))[:, None, None], -math.inf)
+    want = s.softmax(-1) @ rv
+    off = ((got - want).norm() / want.norm()).item()
+    alone = ((want.to(TYPES[kind]).double() - want).norm() / want.norm()).item()
+    assert off < (ratio * alone if ratio else 2e-6)
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
