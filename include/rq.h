@@ -389,7 +389,10 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * (n <= max_q; cu_q NULL: row b, n = 1), query i at position kv_lens[b] - n +
  * i; it sees the positions j <= its own and, with window > 0, j > its own -
  * window.  out row = softmax_j(scale * q . k_j) v over the seen positions, in
- * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  A query
+ * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  f32 and f16
+ * queries take the cache's values exactly; more than 16 bf16 rows (queries times
+ * heads) a kv head take them rounded to f16, where a value below 2^-26 of the
+ * largest of its 64 positions keeps fewer bits.  A query
  * that sees nothing gets zeros.  Positions behind table_width * page_size or
  * on a page outside the cache are not seen.  Rows of q and out that belong to
  * no sequence (or lie at or behind n_tokens) are left as they were.  out may

@@ -68,7 +68,9 @@ __device__ __forceinline__ int owner(const int64_t* v, int n, int64_t x) {
 // bisection in shared memory.  New entries of the table are written and old
 // ones read, never the same ones, so the CTAs need one barrier a chunk: before
 // kv_lens (which may be ctx_lens) and the state (which may be its own output)
-// are written.  Latency-bound.
+// are written.  Bound by latencies: 4 us for 16 sequences of one new token (the
+// lengths, two sums over the CTA, a barrier, the writes), 9.7 us for 200 of which
+// most take in a prompt (354 KB written; 14 us before a warp took runs of tokens).
 __global__ void __launch_bounds__(kThreads) pages_extend_kernel(const __grid_constant__ PagesP p) {
     pdl_wait();
     __shared__ int64_t tok[kThreads + 1], pg[kThreads + 1];

@@ -15,7 +15,10 @@
 // of kGroup consecutive elements (one warp a group, 2 x 16 whole lines in
 // flight), the CTAs exchange their sums through distributed shared memory, and
 // the one whose share holds the target re-reads one group (from L2), 16
-// elements a lane, and scans it.
+// elements a lane, and scans it.  8.4 us for one sequence of four drafts over
+// 32000 tokens (four dependent round trips to memory and two cluster barriers),
+// 17.4 us for 32 of seven over 128003 (1.9 TB/s of the f32 rows read: 5 us at the
+// copy's rate, the round trips before and behind it the rest).
 #include <algorithm>
 
 #include "rq_kv4.cuh"
