@@ -392,7 +392,7 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  f32 and f16
  * queries take the cache's values exactly; more than 16 bf16 rows (queries times
  * heads) a kv head take them rounded to f16, where a value below 2^-26 of the
- * largest of its 64 positions keeps fewer bits.  A query
+ * largest of its 32 positions keeps fewer bits.  A query
  * that sees nothing gets zeros.  Positions behind table_width * page_size or
  * on a page outside the cache are not seen.  Rows of q and out that belong to
  * no sequence (or lie at or behind n_tokens) are left as they were.  out may

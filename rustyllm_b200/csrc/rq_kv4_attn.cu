@@ -1155,10 +1155,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 // P as f16: an eighth each of the rounding that bf16 gives the output.  (Kept exact --
 // a product a block, scaled in the softmax, P times each block's scales -- S and
 // P crossed TMEM head_dim / 32 times, for 1.3 times the softmax's time.)  E is
-// the step's: zero scales apart, the largest one comes to [2^11, 2^12) -- so
-// that 8 d still is an f16 -- or stays below it with the power at its floor, and
-// only scales 2^26 times smaller than that lose bits.  A row keeps its own
-// largest power of V in sight and weighs the step by 2^(E - that).  A value that
+// that of 32 positions: their largest scale comes to [2^11, 2^12) -- so that 8 d
+// still is an f16 -- or stays below it with the power at its floor, and only scales
+// 2^26 times smaller than that lose bits.  A row keeps its own largest power of V
+// in sight and weighs the positions by 2^(E - that).  A value that
 // is not a number cannot lie in an operand that rows share which do not see it:
 // it enters as zero, and the rows that do see it are marked and get it at the
 // end.
@@ -1210,8 +1210,9 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4][2], b_ops_full[kTcOps], b_ops_empty[kTcOps], b_s_full[2], b_s_empty[2],
         b_p_full[2], b_pv_done[2];
-    __shared__ float s_qs[kTcRows], s_dm[kTcOps][2][2], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows], s_kf[kTcOps];
-    __shared__ int s_E[kTcOps], s_there[kTcOps][2], s_any_nan[kTcOps][2];
+    __shared__ float s_qs[kTcRows], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows];
+    __shared__ float s_kf[kTcOps][2];  // of a step's half: 2^E of K, E of V, tiles that are there
+    __shared__ int s_E[kTcOps][2], s_there[kTcOps][2], s_any_nan[kTcOps][2];
     __shared__ uint32_t s_nan[kTcOps][2][NB], s_bad[2][kTcRows];  // positions that are not numbers: of a step's half, by block
     __shared__ uint32_t s_tmem;
     pdl_wait();
@@ -1303,6 +1304,15 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         const int g = lane >> 2, t = lane & 3, half = list & 1;
         const Magic magic = p.magic;
         uint8_t* const scl = sm + S::kScl + pw * 2 * 32 * NB;
+        // where the lane's values go: V, elements g, + 8, .. and positions 4 t .. + 3
+        // of tile i; K, elements 8 t .. (chunk t, or t + 4 for odd blocks) of positions
+        // 4 (g / 2) + g % 2 + 2 n of the half's first tile
+        int at[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            at[i] = is_v ? sw128(g, 4 * half + 2 * i + (t >> 1)) + 8 * (t & 1)
+                         : half * 4096 + sw128(4 * (g >> 1) + (g & 1) + 2 * i, t);
+        const uint32_t pick = g & 1 ? 0x3232u : 0x1010u;
         for (int j = 0; 2 * j + (list >> 1) < steps; j++) {
             const int k = 2 * j + (list >> 1), st = k % kTcOps, s = j & 1;
             if (ok && k >= kTcOps && !mbar_wait(smem_u32(&b_ops_empty[st]), ((k / kTcOps) - 1) & 1)) ok = false;
@@ -1317,15 +1327,18 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             uint2 sc[2];
             uint32_t bad[2] = {0u, 0u};  // tokens (bits 0 - 3) whose value is not a number
             __half2 big = __half2half2(__ushort_as_half(0));
+            const bool ends = (t0 + 4 * k + 2 * half + 2) * kKv4Tile > seen;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 sc[i] = make_uint2(0u, 0u);
                 if (((there >> i) & 1u) && lane < 4 * NB) {
                     sc[i] = *reinterpret_cast<const uint2*>(rec + i * Rec::kBytes + Rec::kKs + is_v * 32 * NB + lane * 8);
-                    const int left = seen - ((t0 + 4 * k + 2 * half + i) * kKv4Tile + 4 * (lane / NB));
-                    if (left < 4) {
-                        sc[i].y &= left > 2 ? 0x0000FFFFu : 0u;
-                        sc[i].x &= left > 1 ? 0xFFFFFFFFu : left > 0 ? 0x0000FFFFu : 0u;
+                    if (ends) {
+                        const int left = seen - ((t0 + 4 * k + 2 * half + i) * kKv4Tile + 4 * (lane / NB));
+                        if (left < 4) {
+                            sc[i].y &= left > 2 ? 0x0000FFFFu : 0u;
+                            sc[i].x &= left > 1 ? 0xFFFFFFFFu : left > 0 ? 0x0000FFFFu : 0u;
+                        }
                     }
                     if (is_v) {
                         const uint32_t nx = nan_halves(sc[i].x), ny = nan_halves(sc[i].y);
@@ -1337,24 +1350,24 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                 big = __hmax2(big, __hmax2(__habs2(as_h2(sc[i].x)), __habs2(as_h2(sc[i].y))));
             }
             float dm = fmaxf(__half2float(__low2half(big)), __half2float(__high2half(big)));
-#pragma unroll
-            for (int i = 16; i > 0; i >>= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, i));
-            if (lane == 0) s_dm[st][is_v][half] = dm;
-            if (is_v) {
-                const bool none = !__any_sync(0xffffffffu, bad[0] | bad[1]);
-                if (lane < NB) s_nan[st][half][lane] = 0u;
-                if (lane == 0) s_any_nan[st][half] = !none;
-            }
-            named_bar_sync(9 + 2 * (list >> 1) + is_v, 64);  // the step's two K, or V warps
-            dm = fmaxf(s_dm[st][is_v][0], s_dm[st][is_v][1]);
             int E = kTcLow;
-            if (dm > __int_as_float((127 + kTcTop + kTcLow) << 23)) {
+            if (__any_sync(0xffffffffu, dm > __int_as_float((127 + kTcTop + kTcLow) << 23))) {
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, i));
                 frexpf(dm, &E);
                 E -= kTcTop;
             }
-            if (half == 0 && lane == 0) {
-                if (is_v) s_E[st] = E;
-                else s_kf[st] = __int_as_float((127 + E) << 23);
+            if (is_v) {
+                const bool some = __any_sync(0xffffffffu, bad[0] | bad[1]);
+                if (lane < NB) s_nan[st][half][lane] = 0u;
+                if (lane == 0) {
+                    s_any_nan[st][half] = some;
+                    s_E[st][half] = E;
+                }
+                __syncwarp();
+            } else if (lane == 0) {
+                s_kf[st][half] = __int_as_float((127 + E) << 23);
+                s_there[st][half] = (int)there;
             }
             const uint32_t inv = as_u32(__float2half2_rn(__int_as_float((127 - E) << 23)));
 #pragma unroll
@@ -1367,7 +1380,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             // ---- values
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int tile = 2 * half + i;  // of the step
                 uint32_t x[2 * NB];
                 if ((there >> i) & 1u) {
                     load_words<NB>(rec + i * Rec::kBytes + is_v * Rec::kV, lane, x);
@@ -1376,36 +1388,32 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                     for (int b = 0; b < 2 * NB; b++) x[b] = 0x88888888u;  // zeros
                 }
                 if (is_v) {
-                    uint8_t* dst = sm + S::kV + st * NB * 4096;
+                    uint8_t* dst = sm + S::kV + st * NB * 4096 + at[i];
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         const uint2 d = *reinterpret_cast<const uint2*>(scl + i * 32 * NB + (t * NB + b) * 8);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const uint4 v = v_operands(x[2 * b] >> (8 * h), x[2 * b + 1] >> (8 * h), magic);
-                            // rows (elements) 32 b + 16 h + g and + 8, positions 4 t .. + 3 of the tile
-                            const int e = 32 * b + 16 * h + g, c = tile * 2 + (t >> 1);
-                            *reinterpret_cast<uint2*>(dst + sw128(e, c) + 8 * (t & 1)) = make_uint2(times(v.x, d.x), times(v.y, d.y));
-                            *reinterpret_cast<uint2*>(dst + sw128(e + 8, c) + 8 * (t & 1)) = make_uint2(times(v.z, d.x), times(v.w, d.y));
+                            *reinterpret_cast<uint2*>(dst + b * 4096 + h * 2048) = make_uint2(times(v.x, d.x), times(v.y, d.y));
+                            *reinterpret_cast<uint2*>(dst + b * 4096 + h * 2048 + 1024) = make_uint2(times(v.z, d.x), times(v.w, d.y));
                         }
                     }
                 } else {
-                    uint8_t* dst = sm + S::kK + st * S::kAtoms * 8192;
+                    uint8_t* dst = sm + S::kK + st * S::kAtoms * 8192 + i * 2048;
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         const uint2 d = *reinterpret_cast<const uint2*>(scl + i * 32 * NB + ((g >> 1) * NB + b) * 8);
 #pragma unroll
                         for (int n = 0; n < 2; n++) {
-                            const uint32_t dd = __byte_perm(n ? d.y : d.x, 0u, g & 1 ? 0x3232u : 0x1010u);
-                            const int row = tile * kKv4Tile + 4 * (g >> 1) + (g & 1) + 2 * n;
+                            const uint32_t dd = __byte_perm(n ? d.y : d.x, 0u, pick);
                             const uint4 v = k_operands(x[2 * b + n], magic);
-                            *reinterpret_cast<uint4*>(dst + (b >> 1) * 8192 + sw128(row, (b & 1) * 4 + t)) =
+                            *reinterpret_cast<uint4*>(dst + (b >> 1) * 8192 + (b & 1 ? at[n] ^ 64 : at[n])) =
                                 make_uint4(times(v.x, dd), times(v.y, dd), times(v.z, dd), times(v.w, dd));
                         }
                     }
                 }
             }
-            if (!is_v && lane == 0) s_there[st][half] = (int)there;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&b_ops_full[st]));
@@ -1487,15 +1495,16 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             tc::tmem_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&b_s_empty[h]));
-            const float f = fmaxf(qs * s_kf[os], 1.2e-38f);  // (times -inf of a masked place)
-            const int e = s_E[os];
             // ---- which of them the row sees
             uint32_t sees[2];
-            float mx = -INFINITY;
+            float f[2], mx = -INFINITY;
+            int e[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const uint32_t there = (uint32_t)s_there[os][i];
                 const int at = j0 + 32 * i;
+                f[i] = fmaxf(qs * s_kf[os][i], 1.2e-38f);  // (times -inf of a masked place)
+                e[i] = s_E[os][i];
                 const int hi = min(min(rpos + 1, o.held) - at, 32), lo = p.window > 0 ? max(rpos - p.window + 1 - at, 0) : 0;
                 sees[i] = (hi >= 32 ? 0xFFFFFFFFu : hi > 0 ? (1u << hi) - 1u : 0u) & (lo >= 32 ? 0u : 0xFFFFFFFFu << lo);
                 sees[i] &= (there & 1u ? 0xFFFFu : 0u) | (there & 2u ? 0xFFFF0000u : 0u);
@@ -1504,19 +1513,21 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                     for (int j = 0; j < 32; j++)
                         if (!((sees[i] >> j) & 1u)) a[i][j] = 0xFF800000u;  // -inf
                 }
+                float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(a[i][j]));
+                for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(a[i][j]));
+                mx = fmaxf(mx, top * f[i]);
             }
             if (s_any_nan[os][0] | s_any_nan[os][1]) {
                 for (int b = 0; b < NB; b++)
                     if ((s_nan[os][0][b] & sees[0]) | (s_nan[os][1][b] & sees[1])) bad |= 1u << b;
             }
-            mx *= f;
+            const int e_top = max(e[0], e[1]);
             // ---- move the row's power of V or its reference where they grew
             float al = 1.0f;
-            if (mx > -INFINITY && e > E) {
-                al = __int_as_float((127 + E - e) << 23);
-                E = e;
+            if (mx > -INFINITY && e_top > E) {
+                al = __int_as_float((127 + E - e_top) << 23);
+                E = e_top;
             }
             if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
                 const float d = m == -INFINITY ? 0.0f : ex2(m - mx);
@@ -1524,7 +1535,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                 l *= d;
                 m = mx;
             }
-            const float base = (m == -INFINITY ? 0.0f : m) + (float)(E - e) - kTcUp;
             // ---- P and O are free once the group's last products are done
             if (ok && k >= 2 && !mbar_wait(smem_u32(&b_pv_done[h]), ph ^ 1)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
@@ -1540,20 +1550,22 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                     tc::tmem_st16u(o_at + 16 * c, v);
                 }
             }
-            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
+                const float base = (m == -INFINITY ? 0.0f : m) + (float)(E - e[i]) - kTcUp;
+                float2 sum = make_float2(0.0f, 0.0f);
                 uint32_t pk[16];
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const float2 x = fma2(make_float2(__uint_as_float(a[i][2 * j]), __uint_as_float(a[i][2 * j + 1])), make_float2(f, f), make_float2(-base, -base));
+                    const float2 x = fma2(make_float2(__uint_as_float(a[i][2 * j]), __uint_as_float(a[i][2 * j + 1])),
+                                          make_float2(f[i], f[i]), make_float2(-base, -base));
                     const float2 y = make_float2(ex2(x.x), ex2(x.y));
                     sum = add2(sum, y);
                     pk[j] = pack(y.x, y.y);
                 }
                 tc::tmem_st16u(p_at + 16 * i, pk);
+                l = fmaf(sum.x + sum.y, __int_as_float((127 + E - e[i]) << 23), l);
             }
-            l = fmaf(sum.x + sum.y, __int_as_float((127 + E - e) << 23), l);
             tc::tmem_wait_st();
             tc::tmem_fence_before();
             __syncwarp();
