@@ -1163,33 +1163,39 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 // it enters as zero, and the rows that do see it are marked and get it at the
 // end.
 //
-// TMEM, for even steps and for odd ones: S (64 columns), P as the A operand
-// (32) and O (32 NB).
+// Two groups of four warps do the softmax, a thread a row, each with its own S (64
+// columns of TMEM), P as the A operand (32) and O (32 NB): with PAIR of a tile of
+// 128 rows each, so that unpacking a step serves 256 rows; else of even and of odd
+// steps of one tile, with their own maxima and sums, joined at the end (one group
+// with half the positions a warp, which agreed on every step's maximum, took 318 us
+// where the two took 279).  PAIR from 129 rows: 192 rows of 8 heads a kv head of 8,
+// head_dim 128, 16 x 2048 positions 84 -> 66 us, 64 x 1024 182 -> 158, 1 x 40000
+// 94 -> 83; at 128 rows, where its second tile would be empty, the steps' latencies
+// are not hidden (41, 102, 54 us as it is).
+//
 // Roles (17 warps):
-//   0 - 7   softmax: even steps the first four, odd ones the others, a thread a
-//           row; the two groups keep their own maxima and sums, joined at the
-//           end (as one group with half the positions a warp, which agreed on
-//           every step's maximum: 318 us where two took 279)
-//   8       issues the products: S two steps ahead of P V
+//   0 - 7   softmax, group w / 4, rows 32 (w % 4) + lane of the tile
+//   8       issues the products: S ahead of P V by a step of the group
 //   9 - 16  unpack, even steps the first four, odd ones the others: two warps a
 //           half of the step, one K, one V, into the 128-byte-swizzled operands
-//           (four buffers: with two, and one group, unpacking a step waited for
-//           the products two steps before, 3400 cycles a step where this takes
-//           2000)
+//           (three or four buffers: with two, and one group, unpacking a step
+//           waited for the products two steps before, 3400 cycles a step where
+//           this takes 2000)
 //
-// 270 us at three prompts of 256 - 512 tokens on up to 4500 positions, 64 query
-// heads on 8, head_dim 128 (280 TFLOP/s): the issue of some 5700 warp
-// instructions a step bounds it, two thirds of them the unpacking's and the
-// exponentials', at 2.2 a cycle; the tensor pipe is busy for a fifth of the time.
-constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 17, kTcOps = 4;
+// 254 us at three prompts of 256 - 512 tokens on up to 4500 positions, 64 query
+// heads on 8, head_dim 128 (297 TFLOP/s): the instructions of the unpacking and
+// the exponentials bound it, some 2.2 a cycle and SM, and the last wave's length
+// (288 CTAs on 148 SMs); the tensor pipe is busy for a fifth of the time.
+constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 17;
 constexpr int kTcTop = 12, kTcLow = -8;  // see E
 constexpr float kTcUp = 7.0f;  // the largest P lies in [2^7, 2^15], so that f16 has it to 2^-11 down to 2^-21 of that
 
-template <int NB>
+template <int NB, bool PAIR>
 struct TcSmem {  // dynamic shared memory from a 1024-byte border
+    static constexpr int kOps = PAIR ? 3 : 4;    // operand buffers
     static constexpr int kAtoms = (NB + 1) / 2;  // 64 elements = 128 bytes of a row
-    static constexpr int kQ = 0, kK = kAtoms * 16384, kV = kK + kTcOps * kAtoms * 8192,
-                         kRing = kV + kTcOps * NB * 4096;
+    static constexpr int kQ = 0, kK = (PAIR ? 2 : 1) * kAtoms * 16384, kV = kK + kOps * kAtoms * 8192,
+                         kRing = kV + kOps * NB * 4096;
     static constexpr int kScl = kRing + 4 * 2 * 2 * 576 * NB;  // [8 unpacking warps][2 tiles][32 NB]
     static constexpr int kBytes = kScl + 8 * 2 * 32 * NB;
     static constexpr int kCols = NB == 1 ? 256 : 512;
@@ -1202,15 +1208,16 @@ __device__ __forceinline__ uint32_t nan_halves(uint32_t w) {
     return __hne2_mask(as_h2(w), as_h2(w));
 }
 
-template <int NB, typename T>
+template <int NB, bool PAIR, typename T>
 __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using S = TcSmem<NB>;
-    constexpr int HD = 32 * NB, kPCol = 128, kOCol = 192;  // TMEM: S, P, O of even and odd steps
+    using S = TcSmem<NB, PAIR>;
+    constexpr int kTcOps = S::kOps, kAllRows = PAIR ? 2 * kTcRows : kTcRows;
+    constexpr int HD = 32 * NB, kPCol = 128, kOCol = 192;  // TMEM: the groups' S, P, O
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4][2], b_ops_full[kTcOps], b_ops_empty[kTcOps], b_s_full[2], b_s_empty[2],
         b_p_full[2], b_pv_done[2];
-    __shared__ float s_qs[kTcRows], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows];
+    __shared__ float s_qs[kAllRows], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows];
     __shared__ float s_kf[kTcOps][2];  // of a step's half: 2^E of K, E of V, tiles that are there
     __shared__ int s_E[kTcOps][2], s_there[kTcOps][2], s_any_nan[kTcOps][2];
     __shared__ uint32_t s_nan[kTcOps][2][NB], s_bad[2][kTcRows];  // positions that are not numbers: of a step's half, by block
@@ -1220,14 +1227,15 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
     // a sequence's last rows, which see the most, first
     const int at0 = (int)(blockIdx.x / p.splits), split = (int)blockIdx.x - at0 * p.splits;
     const int unit = (int)(gridDim.x / p.splits) - 1 - at0;
-    const Rows o = unit_rows<kTcRows>(p, unit);
+    const Rows o = unit_rows<kAllRows>(p, unit);
     if (o.r0 >= o.rows) return;
     int tile0, tile1, per;
-    unit_tiles<kTcRows>(p, o, tile0, tile1, per);
+    unit_tiles<kAllRows>(p, o, tile0, tile1, per);
     const int t0 = tile0 + split * per, t1 = min(t0 + per, tile1);
     if (p.splits > 1 && t0 >= t1) return;  // the join does not read this split
     const int steps = t1 > t0 ? (t1 - t0 + 3) / 4 : 0;
-    const int i1 = min(o.n_q - 1, (o.r0 + kTcRows - 1) / p.group);
+    const int i1 = min(o.n_q - 1, (o.r0 + kAllRows - 1) / p.group);
+    const int groups = PAIR && o.rows - o.r0 <= kTcRows ? 1 : 2;
     const int seen = max(0, min(o.held, o.pos0 + i1 + 1));  // positions that any row sees end here
     uint8_t* const sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sm32 = smem_u32(sm);
@@ -1260,36 +1268,39 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
     } else {
         // two lanes a row: normalised by a power of two to f16, which is exact
         // for f16 and (but for elements below 2^-14 of the largest) bf16
-        const int row = threadIdx.x >> 1, r = o.r0 + row;
-        const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
-        const int64_t tok = (int64_t)o.q0 + i;
-        const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
-        const T* q = static_cast<const T*>(p.q) + tok * p.qt + head * p.qh;
-        float x[2 * NB][8];  // chunks 2 c + (lane & 1)
-        float mx = 0.0f;
+#pragma unroll 1
+        for (int tile = 0; tile < (PAIR ? groups : 1); tile++) {
+            const int row = tile * kTcRows + (threadIdx.x >> 1), r = o.r0 + row;
+            const int i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+            const int64_t tok = (int64_t)o.q0 + i;
+            const bool ok = r < o.rows && tok >= 0 && tok < p.n_tokens;
+            const T* q = static_cast<const T*>(p.q) + tok * p.qt + head * p.qh;
+            float x[2 * NB][8];  // chunks 2 c + (lane & 1)
+            float mx = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 2 * NB; c++) {
+            for (int c = 0; c < 2 * NB; c++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[c][e] = 0.0f;
-            if (ok) load8(q + 8 * (2 * c + (lane & 1)), p.wide, x[c]);
-        }
+                for (int e = 0; e < 8; e++) x[c][e] = 0.0f;
+                if (ok) load8(q + 8 * (2 * c + (lane & 1)), p.wide, x[c]);
+            }
 #pragma unroll
-        for (int c = 0; c < 2 * NB; c++)
+            for (int c = 0; c < 2 * NB; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        int e2 = 0;
-        if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e2);
-        e2 = max(-110, min(110, e2));
-        // the scale's sign is the operand's, so that scores grow with their sums
-        const float down = p.scale == 0.0f ? 0.0f : copysignf(__int_as_float((127 - e2) << 23), p.scale);
-        if ((lane & 1) == 0) s_qs[row] = p.scale == 0.0f ? 1.0f : __int_as_float((127 + e2) << 23) * fabsf(p.scale);
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            int e2 = 0;
+            if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e2);
+            e2 = max(-110, min(110, e2));
+            // the scale's sign is the operand's, so that scores grow with their sums
+            const float down = p.scale == 0.0f ? 0.0f : copysignf(__int_as_float((127 - e2) << 23), p.scale);
+            if ((lane & 1) == 0) s_qs[row] = p.scale == 0.0f ? 1.0f : __int_as_float((127 + e2) << 23) * fabsf(p.scale);
 #pragma unroll
-        for (int c = 0; c < 2 * NB; c++) {
-            const int at = 2 * c + (lane & 1);
-            *reinterpret_cast<uint4*>(sm + S::kQ + (at >> 3) * 16384 + sw128(row, at & 7)) =
-                make_uint4(pack(x[c][0] * down, x[c][1] * down), pack(x[c][2] * down, x[c][3] * down),
-                           pack(x[c][4] * down, x[c][5] * down), pack(x[c][6] * down, x[c][7] * down));
+            for (int c = 0; c < 2 * NB; c++) {
+                const int at = 2 * c + (lane & 1);
+                *reinterpret_cast<uint4*>(sm + S::kQ + (tile * S::kAtoms + (at >> 3)) * 16384 + sw128(row & (kTcRows - 1), at & 7)) =
+                    make_uint4(pack(x[c][0] * down, x[c][1] * down), pack(x[c][2] * down, x[c][3] * down),
+                               pack(x[c][4] * down, x[c][5] * down), pack(x[c][6] * down, x[c][7] * down));
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -1425,41 +1436,49 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         // -------------------------------------------------------- products
         constexpr uint32_t kIdS = (1u << 4) | ((uint32_t)(kTcStep >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
         constexpr uint32_t kIdO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        for (int k = -2; k < steps; k++) {
-            if (k + 2 < steps) {  // S of the step after the next
-                const int j = k + 2, st = j & 1, os = j % kTcOps;
+        constexpr int kAhead = PAIR ? 1 : 2;  // steps from S to P V
+        for (int k = -kAhead; k < steps; k++) {
+            // (without PAIR a step belongs to one group, as its n-th)
+            if (const int j = k + kAhead; j < steps) {
+                const int os = j % kTcOps, n = PAIR ? j : j >> 1;
                 if (ok && !mbar_wait(smem_u32(&b_ops_full[os]), (j / kTcOps) & 1)) ok = false;
-                if (ok && j >= 2 && !mbar_wait(smem_u32(&b_s_empty[st]), ((j >> 1) - 1) & 1)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
-                tc::tmem_fence_after();
-                if (tc::elect_one()) {
-                    if (ok) {
+                for (int g = PAIR ? 0 : j & 1; g < (PAIR ? groups : (j & 1) + 1); g++) {
+                    if (ok && n > 0 && !mbar_wait(smem_u32(&b_s_empty[g]), (n - 1) & 1)) ok = false;
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc::tmem_fence_after();
+                    if (tc::elect_one()) {
+                        if (ok) {
+                            const uint32_t qa = sm32 + S::kQ + (PAIR ? g * S::kAtoms * 16384 : 0);
 #pragma unroll
-                        for (int x = 0; x < 2 * NB; x++)
-                            tc::umma_f16(tmem + 64 * st, tc::desc_sw128(sm32 + S::kQ + (x >> 2) * 16384 + 32 * (x & 3)),
-                                         tc::desc_sw128(sm32 + S::kK + (os * S::kAtoms + (x >> 2)) * 8192 + 32 * (x & 3)), kIdS,
-                                         x ? 1u : 0u);
+                            for (int x = 0; x < 2 * NB; x++)
+                                tc::umma_f16(tmem + 64 * g, tc::desc_sw128(qa + (x >> 2) * 16384 + 32 * (x & 3)),
+                                             tc::desc_sw128(sm32 + S::kK + (os * S::kAtoms + (x >> 2)) * 8192 + 32 * (x & 3)), kIdS,
+                                             x ? 1u : 0u);
+                        }
+                        tc::umma_commit(smem_u32(&b_s_full[g]));
                     }
-                    tc::umma_commit(smem_u32(&b_s_full[st]));
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-            if (k >= 0) {  // O of this one
-                const int st = k & 1, os = k % kTcOps;
-                if (ok && !mbar_wait(smem_u32(&b_p_full[st]), (k >> 1) & 1)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
-                tc::tmem_fence_after();
-                if (tc::elect_one()) {
-                    if (ok) {
+            if (k >= 0) {
+                const int os = k % kTcOps, n = PAIR ? k : k >> 1;
+                const int last = PAIR ? groups - 1 : k & 1;
+                for (int g = PAIR ? 0 : k & 1; g <= last; g++) {
+                    if (ok && !mbar_wait(smem_u32(&b_p_full[g]), n & 1)) ok = false;
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc::tmem_fence_after();
+                    if (tc::elect_one()) {
+                        if (ok) {
 #pragma unroll
-                        for (int x = 0; x < 4; x++)
-                            tc::umma_f16_ts(tmem + kOCol + st * HD, tmem + kPCol + 32 * st + 8 * x,
-                                            tc::desc_sw128(sm32 + S::kV + os * NB * 4096 + 32 * x), kIdO, k > 1 || x > 0 ? 1u : 0u);
+                            for (int x = 0; x < 4; x++)
+                                tc::umma_f16_ts(tmem + kOCol + g * HD, tmem + kPCol + 32 * g + 8 * x,
+                                                tc::desc_sw128(sm32 + S::kV + os * NB * 4096 + 32 * x), kIdO, n > 0 || x > 0 ? 1u : 0u);
+                        }
+                        tc::umma_commit(smem_u32(&b_pv_done[g]));
+                        if (g == last) tc::umma_commit(smem_u32(&b_ops_empty[os]));
                     }
-                    tc::umma_commit(smem_u32(&b_pv_done[st]));
-                    tc::umma_commit(smem_u32(&b_ops_empty[os]));
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
         // the last commits' arrivals, which nobody else may wait for, may not
@@ -1469,19 +1488,20 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         if (!ok && lane == 0) atomicExch(p.err, 1);
     } else {
         // --------------------------------------------------------- softmax
-        const int q = warp & 3, h = warp >> 2, row = 32 * q + lane;
-        const int r = o.r0 + row, i = r / p.group, head = o.kvh * p.group + r - i * p.group;
+        const int q = warp & 3, h = warp >> 2, row = 32 * q + lane, at_row = row + (PAIR ? h * kTcRows : 0);
+        const int r = o.r0 + at_row, i = r / p.group, head = o.kvh * p.group + r - i * p.group;
         const int64_t tok = (int64_t)o.q0 + i;
         const bool live = r < o.rows && tok >= 0 && tok < p.n_tokens;
         const int rpos = live ? o.pos0 + i : -1;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
-        const float qs = s_qs[row];
+        const float qs = s_qs[at_row];
         const uint32_t s_at = lanes + 64 * h, p_at = lanes + kPCol + 32 * h, o_at = lanes + kOCol + HD * h;
         float m = -INFINITY, l = 0.0f;
         uint32_t bad = 0;  // blocks of O that a value which is not a number reaches
         int E = kTcLow;
-        for (int k = h; k < steps; k += 2) {
-            const int ph = (k >> 1) & 1, os = k % kTcOps;
+        const int mine = h >= groups ? 0 : PAIR ? steps : (steps + 1 - h) / 2;
+        for (int n = 0; n < mine; n++) {
+            const int k = PAIR ? n : 2 * n + h, ph = n & 1, os = k % kTcOps;
             if (ok && !mbar_wait(smem_u32(&b_ops_full[os]), (k / kTcOps) & 1)) ok = false;
             if (ok && !mbar_wait(smem_u32(&b_s_full[h]), ph)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
@@ -1536,10 +1556,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                 m = mx;
             }
             // ---- P and O are free once the group's last products are done
-            if (ok && k >= 2 && !mbar_wait(smem_u32(&b_pv_done[h]), ph ^ 1)) ok = false;
+            if (ok && n > 0 && !mbar_wait(smem_u32(&b_pv_done[h]), ph ^ 1)) ok = false;
             ok = __all_sync(0xffffffffu, ok);
             tc::tmem_fence_after();
-            if (k >= 2 && __any_sync(0xffffffffu, al != 1.0f)) {
+            if (n > 0 && __any_sync(0xffffffffu, al != 1.0f)) {
 #pragma unroll 1
                 for (int c = 0; c < 2 * NB; c++) {
                     uint32_t v[16];
@@ -1571,33 +1591,40 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&b_p_full[h]));
         }
-        const int last = steps - 1 - ((steps - 1 - h) & 1);  // of the group
-        if (ok && last >= 0 && !mbar_wait(smem_u32(&b_pv_done[h]), (last >> 1) & 1)) ok = false;
+        if (ok && mine > 0 && !mbar_wait(smem_u32(&b_pv_done[h]), (mine - 1) & 1)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok && lane == 0) atomicExch(p.err, 1);
-        // ---- the row's even and odd steps together
-        s_m[h][row] = m;
-        s_l[h][row] = l;
-        s_bound[h][row] = __int_as_float((127 + E) << 23);
-        s_bad[h][row] = bad;
-        tc::tmem_fence_before();
-        named_bar_sync(1 + q, 64);
+        float f0 = __int_as_float((127 + E) << 23), f1 = 0.0f;  // what the groups' O counts
+        if constexpr (!PAIR) {  // the row's even and odd steps together
+            s_m[h][row] = m;
+            s_l[h][row] = l;
+            s_bound[h][row] = f0;
+            s_bad[h][row] = bad;
+            tc::tmem_fence_before();
+            named_bar_sync(1 + q, 64);
+            m = fmaxf(s_m[0][row], s_m[1][row]);
+            const float w0 = weight(s_m[0][row], m), w1 = weight(s_m[1][row], m);
+            l = s_l[0][row] * w0 + s_l[1][row] * w1;
+            bad = s_bad[0][row] | s_bad[1][row];
+            f0 = s_bound[0][row] * w0;
+            f1 = s_bound[1][row] * w1;
+        }
         tc::tmem_fence_after();
-        m = fmaxf(s_m[0][row], s_m[1][row]);
-        const float w0 = weight(s_m[0][row], m), w1 = weight(s_m[1][row], m);
-        l = s_l[0][row] * w0 + s_l[1][row] * w1;
-        bad = s_bad[0][row] | s_bad[1][row];
-        // ---- columns 16 NB h .. of the row
         const bool any = l != 0.0f;  // (not a number counts)
-        const float f = p.splits == 1 ? 1.0f / l : 1.0f, f0 = s_bound[0][row] * w0 * f, f1 = s_bound[1][row] * w1 * f;
+        if (p.splits == 1) {
+            const float f = 1.0f / l;
+            f0 *= f;
+            f1 *= f;
+        }
         const int64_t at = (tok * p.n_heads + head) * p.splits + split;
         T* out = static_cast<T*>(p.out) + tok * p.ot + head * p.oh;
+        // PAIR: all columns of the group's rows; else columns 16 NB h .. of the tile's
 #pragma unroll
-        for (int c = 0; c < NB; c++) {
+        for (int c = 0; c < (PAIR ? 2 * NB : NB); c++) {
             uint32_t a0[16], a1[16];
-            const int col = 16 * (h * NB + c);
-            if (steps > 0) tc::tmem_ld16(lanes + kOCol + col, a0);
-            if (steps > 1) tc::tmem_ld16(lanes + kOCol + HD + col, a1);
+            const int col = 16 * (PAIR ? c : h * NB + c);
+            if (mine > 0 || (!PAIR && steps > 0)) tc::tmem_ld16(lanes + kOCol + (PAIR ? HD * h : 0) + col, a0);
+            if (!PAIR && steps > 1) tc::tmem_ld16(lanes + kOCol + HD + col, a1);
             tc::tmem_wait_ld();
             if (!live) continue;
             const bool not_number = (bad >> (col >> 5)) & 1u;
@@ -1607,14 +1634,14 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
 #pragma unroll
                 for (int y = 0; y < 8; y++) {
                     v[y] = any ? __uint_as_float(a0[x + y]) * f0 : 0.0f;
-                    if (any && steps > 1) v[y] = fmaf(__uint_as_float(a1[x + y]), f1, v[y]);
+                    if (!PAIR && any && steps > 1) v[y] = fmaf(__uint_as_float(a1[x + y]), f1, v[y]);
                     if (not_number) v[y] = __int_as_float(0x7fffffff);
                 }
                 if (p.splits == 1) store8(out + col + x, p.wide_out, v);
                 else store8(p.part + at * HD + col + x, true, v);
             }
         }
-        if (p.splits > 1 && live && h == 0) p.ml[at] = make_float2(m, l);
+        if (p.splits > 1 && live && (PAIR || h == 0)) p.ml[at] = make_float2(m, l);
     }
     // every product and copy has been waited for (or its wait gave up)
     tc::tmem_fence_before();
@@ -1707,43 +1734,47 @@ struct Fns {
     const void *main, *join;
 };
 template <int NB, int MODE, typename T>
-Fns fns_of(bool rows) {
+Fns fns_of(bool rows, bool pair) {
     constexpr int R = MODE == kOne16 ? 16 : 8;
     if (rows) {
-        if constexpr (MODE == kOne16)
-            return Fns{(const void*)kv4_attn_tc_kernel<NB, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
-        else
+        if constexpr (MODE == kOne16) {
+            if (pair)
+                return Fns{(const void*)kv4_attn_tc_kernel<NB, true, T>, (const void*)kv4_join_rows_kernel<NB, 2 * kTcRows, T>};
+            return Fns{(const void*)kv4_attn_tc_kernel<NB, false, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
+        } else {
             return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
+        }
     }
     return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
 }
 template <int NB, typename T>
-Fns fns_of(int mode, bool rows) {
+Fns fns_of(int mode, bool rows, bool pair) {
     if constexpr (std::is_same_v<T, __nv_bfloat16>)
-        if (mode == kOne16) return fns_of<NB, kOne16, T>(rows);
+        if (mode == kOne16) return fns_of<NB, kOne16, T>(rows, pair);
     if constexpr (std::is_same_v<T, __nv_bfloat16>)
         return Fns{(const void*)kv4_attn_kernel<NB, kSplit8, T>, (const void*)kv4_join_kernel<NB, 8, T>};
     else
-        return fns_of<NB, kSplit8, T>(rows);
+        return fns_of<NB, kSplit8, T>(rows, pair);
 }
 template <typename T>
-Fns fns_of(int nb, int mode, bool rows) {
+Fns fns_of(int nb, int mode, bool rows, bool pair) {
     switch (nb) {
-    case 1: return fns_of<1, T>(mode, rows);
-    case 2: return fns_of<2, T>(mode, rows);
-    case 3: return fns_of<3, T>(mode, rows);
-    default: return fns_of<4, T>(mode, rows);
+    case 1: return fns_of<1, T>(mode, rows, pair);
+    case 2: return fns_of<2, T>(mode, rows, pair);
+    case 3: return fns_of<3, T>(mode, rows, pair);
+    default: return fns_of<4, T>(mode, rows, pair);
     }
 }
-Fns fns_of(int dtype, int nb, int mode, bool rows) {
-    return dtype == RQ_F32 ? fns_of<float>(nb, mode, rows)
-           : dtype == RQ_F16 ? fns_of<__half>(nb, mode, rows)
-                             : fns_of<__nv_bfloat16>(nb, mode, rows);
+Fns fns_of(int dtype, int nb, int mode, bool rows, bool pair) {
+    return dtype == RQ_F32 ? fns_of<float>(nb, mode, rows, pair)
+           : dtype == RQ_F16 ? fns_of<__half>(nb, mode, rows, pair)
+                             : fns_of<__nv_bfloat16>(nb, mode, rows, pair);
 }
 
 struct Plan {
     int mode, R;       // R: rows of a CTA
     bool rows, tc;     // a many-rows form; the one on tcgen05
+    bool pair;         // two tiles of rows a CTA there
     int64_t ctas;      // of the main launch
     int row_tiles, splits;  // many rows
     int64_t pieces;    // row sums kept for the join: 0, no join
@@ -1805,7 +1836,8 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
         return pl;
     }
     pl.tc = a->dtype == RQ_BF16;
-    pl.R = pl.tc ? kTcRows : 2 * kWarps * pl.R;
+    pl.pair = pl.tc && rows > kTcRows;  // (times: see the kernel)
+    pl.R = pl.tc ? (pl.pair ? 2 : 1) * kTcRows : 2 * kWarps * pl.R;
     pl.row_tiles = (int)((rows + pl.R - 1) / pl.R);
     const int64_t units = a->batch * c->n_kv * pl.row_tiles;
     // splits of the long axis where the units leave the device's places (two
@@ -1872,11 +1904,13 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.magic = Magic{kEven, kOdd};
     p.err = err;
     const int nb = c->head_dim / 32;
-    constexpr int tc_smem[4] = {TcSmem<1>::kBytes, TcSmem<2>::kBytes, TcSmem<3>::kBytes, TcSmem<4>::kBytes};
-    const size_t smem = pl.tc     ? (size_t)tc_smem[nb - 1] + 1024
+    constexpr int tc_smem[2][4] = {
+        {TcSmem<1, false>::kBytes, TcSmem<2, false>::kBytes, TcSmem<3, false>::kBytes, TcSmem<4, false>::kBytes},
+        {TcSmem<1, true>::kBytes, TcSmem<2, true>::kBytes, TcSmem<3, true>::kBytes, TcSmem<4, true>::kBytes}};
+    const size_t smem = pl.tc     ? (size_t)tc_smem[pl.pair][nb - 1] + 1024
                         : pl.rows ? (size_t)kWarps * (2048 * nb + 64 * nb + kStagesRows * 576 * nb + 2048 * nb)
                                 : (size_t)kWarps * (kStages * 2 * 576 * nb + pl.R * 32 * nb * 4);
-    const Fns fn = fns_of(a->dtype, nb, pl.mode, pl.rows);
+    const Fns fn = fns_of(a->dtype, nb, pl.mode, pl.rows, pl.pair);
     if (smem > 32 * 1024) {  // (48 KB without asking, the kernels' static part included)
         const int rc = cuda_error(cudaFuncSetAttribute(fn.main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                                   "kv4 attention kernel");
