@@ -397,7 +397,9 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * on a page outside the cache are not seen.  Rows of q and out that belong to
  * no sequence (or lie at or behind n_tokens) are left as they were.  out may
  * be q.  max_len (> 0): an upper bound of kv_lens that only guides how the
- * work is split (0: table_width * page_size).  `workspace` holds at least
+ * work is split (0: table_width * page_size).  One form serves the whole
+ * call, chosen by max_q: single tokens on long caches are faster in a call of
+ * their own than among prompts.  `workspace` holds at least
  * rq_kv4_attention_workspace bytes, used by this call alone until it is done
  * (two captured graphs that may run at once need one each). */
 typedef struct rq_kv4_query {

@@ -1183,9 +1183,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 //           this takes 2000)
 //
 // 254 us at three prompts of 256 - 512 tokens on up to 4500 positions, 64 query
-// heads on 8, head_dim 128 (297 TFLOP/s): the instructions of the unpacking and
-// the exponentials bound it, some 2.2 a cycle and SM, and the last wave's length
-// (288 CTAs on 148 SMs); the tensor pipe is busy for a fifth of the time.
+// heads on 8, head_dim 128 (297 TFLOP/s): the chains of the softmax (TMEM read,
+// maximum, exponentials, TMEM write) and of the unpacking bound it, at 1.8
+// instructions a cycle and SM, and the last wave's length (288 CTAs on 148 SMs); the
+// tensor pipe is busy for a quarter of the time.
 constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 17;
 constexpr int kTcTop = 12, kTcLow = -8;  // see E
 constexpr float kTcUp = 7.0f;  // the largest P lies in [2^7, 2^15], so that f16 has it to 2^-11 down to 2^-21 of that

@@ -62,12 +62,18 @@ void output(const Tensor& t, const Tensor& like, const char* name, int dev) {
     rows(t, name, like.size(1), like.size(2), dev);
     if (t.scalar_type() != like.scalar_type() || t.size(0) != like.size(0))
         refuse(std::string(name) + ": the shape and type of its input are wanted");
+    for (int i = 0; i < 2; i++)
+        if (t.size(i) > 1 && t.stride(i) == 0) refuse(std::string(name) + ": its rows lie on one another");
 }
 int table(const Tensor& t, int64_t batch, const char* name) {
     if (!t.is_cuda() || t.scalar_type() != at::kInt || t.dim() != 2 || (batch >= 0 && t.size(0) != batch) ||
         (t.size(1) > 1 && t.stride(1) != 1))
         refuse(std::string(name) + ": a CUDA int32 [batch, width] with contiguous rows is wanted");
     return t.device().index();
+}
+int small(int64_t n, const char* name) {
+    if (n != (int)n) refuse(std::string(name) + " " + std::to_string(n) + " is out of range");
+    return (int)n;
 }
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor new_ints(at::IntArrayRef shape, int dev) {
@@ -236,7 +242,7 @@ py::tuple pages_extend(uintptr_t ctx, const Tensor& ctx_lens, const Tensor& new_
     if (kv_lens_out) ints(kv, "kv_lens_out", dev, batch);
     int32_t* cu = buf.data_ptr<int32_t>() + 3 + batch;
     int32_t* pos = cu + batch + 1;
-    check(rq_pages_extend((rq_ctx*)ctx, batch, (int)page_size, c, f, tab.data_ptr<int32_t>(), tab.stride(0), tab.size(1), r,
+    check(rq_pages_extend((rq_ctx*)ctx, batch, small(page_size, "page_size"), c, f, tab.data_ptr<int32_t>(), tab.stride(0), tab.size(1), r,
                           ring.numel(), st, so.data_ptr<int32_t>(), kv.data_ptr<int32_t>(), cu, pos, pos + n_tokens, n_tokens,
                           stream_of(dev)));
     return py::make_tuple(std::move(so), std::move(kv), buf.narrow(0, 3 + batch, batch + 1),
@@ -251,7 +257,7 @@ void pages_release(uintptr_t ctx, const Tensor& held, const Tensor& keep, const 
     const int32_t* k = ints(keep, "keep_lens", dev, batch);
     int32_t* r = ints(ring, "ring", dev);
     int32_t* st = ints(state, "free", dev, 3);
-    check(rq_pages_release((rq_ctx*)ctx, batch, (int)page_size, h, k, tab.data_ptr<int32_t>(), tab.stride(0), tab.size(1), r,
+    check(rq_pages_release((rq_ctx*)ctx, batch, small(page_size, "page_size"), h, k, tab.data_ptr<int32_t>(), tab.stride(0), tab.size(1), r,
                            ring.numel(), st, stream_of(dev)));
 }
 

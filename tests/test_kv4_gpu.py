@@ -680,3 +680,23 @@ def test_refusals(gen):
     pair = (ctypes.c_int64 * 2)(128, 64)
     assert _lib.lib().rq_kv4_append(cache.handle, 0, host.ctypes.data, pair, k.data_ptr(), pair, slots.data_ptr(), 1, None) == 1
     assert "k must be device memory" in _lib.last_error()
+
+
+def test_refuses_outputs_whose_rows_lie_on_one_another_and_sizes_past_32_bits(gen):
+    from rustyllm_b200 import RqError
+    from rustyllm_b200.kv4 import KV4Cache
+    from rustyllm_b200.pages import pages_extend, pages_release
+    from rustyllm_b200.rope import qk_norm_rope, rope_tables
+    cache = KV4Cache(2, 16, 2, 64)
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    two = torch.ones(2, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 4, 64, device="cuda")
+    with pytest.raises(RqError, match="lie on one another"):
+        cache.attention(q, table, two, out=torch.zeros(1, 4, 64, device="cuda").expand(2, 4, 64))
+    with pytest.raises(RqError, match="lie on one another"):
+        qk_norm_rope(q, q, two, *rope_tables(4, 64), q_out=torch.zeros(2, 1, 64, device="cuda").expand(2, 4, 64))
+    ring, free = torch.arange(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 4, 0], dtype=torch.int32, device="cuda")
+    with pytest.raises(RqError, match="out of range"):
+        pages_extend(two, two, table, ring, free, 2 ** 32 + 16, 2)
+    with pytest.raises(RqError, match="out of range"):
+        pages_release(two, two, table, ring, free, 2 ** 32 + 16)
