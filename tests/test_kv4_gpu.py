@@ -327,6 +327,33 @@ def test_error_does_not_grow_with_the_walk(gen, kind, qn, ratio):
     assert off < (ratio * alone if ratio else 2e-6)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("H,kv,hd,page,lens,qs,window", [
+    (8, 1, 32, 16, [300, 40, 0, 17], [30, 17, 0, 17], 0),
+    (16, 2, 128, 64, [400, 257, 90], [40, 7, 16], 0),
+    (32, 2, 96, 32, [1000, 129], [9, 128], 50),
+    (16, 1, 128, 16, [2500], [20], 0),
+    (7, 1, 64, 16, [500, 64, 65], [64, 64, 37], 0),
+])
+def test_prompts_of_more_than_one_tile_of_rows(gen, kind, H, kv, hd, page, lens, qs, window):
+    """Row counts around one and two tiles of 128, steps that end inside a tile
+    of positions, sequences without queries, one that is split."""
+    from rustyllm_b200.kv4 import KV4Cache
+    B, width = len(lens), (max(lens) + page - 1) // page
+    cache = KV4Cache(B * width + 1, page, kv, hd)
+    kval, vval = fill(cache, gen, kind)
+    table = torch.randperm(B * width + 1, generator=gen, device="cuda")[:B * width].view(B, width).to(torch.int32)
+    cu = np.concatenate([[0], np.cumsum(qs)]).astype(np.int32)
+    q = torch.randn(int(cu[-1]) + 3, H, hd, generator=gen, device="cuda").to(TYPES[kind])
+    want = attention_ref(q.double().cpu().numpy(), kval, vval, table.cpu().numpy(), page, lens, cu, hd ** -0.5, window,
+                         cache.n_pages)
+    out = torch.full_like(q, 3.0)
+    cache.attention(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), cu_q=torch.from_numpy(cu).cuda(),
+                    max_q=max(qs), window=window, out=out)
+    close(out[:cu[-1]], want, slice(0, cu[-1]), kind)
+    assert (out[cu[-1]:] == 3).all()
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("scale", [0.05, -0.05, 0.0])
 @pytest.mark.parametrize("falls", [False, True])
