@@ -390,7 +390,9 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * i; it sees the positions j <= its own and, with window > 0, j > its own -
  * window.  out row = softmax_j(scale * q . k_j) v over the seen positions, in
  * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  f32 and f16
- * queries take the cache's values exactly; more than 16 bf16 rows (queries times
+ * queries take the cache's values exactly, whatever other positions hold (where a
+ * head's row has blocks whose scales differ by more than 2^14, the smaller ones
+ * to 2^-25 of the largest); more than 16 bf16 rows (queries times
  * heads) a kv head take them rounded to f16, where a value below 2^-26 of the
  * largest of its 32 positions keeps fewer bits.  A query
  * that sees nothing gets zeros.  Positions behind table_width * page_size or

@@ -30,12 +30,15 @@
 // P enters as f16: in two parts, p = ph + pl (22 bits) and ph d = h + r exactly (h
 // the rounded product, r = fma(ph, d, -h)), so P = h + (r + pl d) costs three
 // packed operations a pair of tokens; one part takes h alone (two roundings of
-// 2^-11, an eighth of bf16's own).  f16's range
-// is kept whatever the scale of V: the scales are divided by a power of two 2^E
-// that follows the largest one seen, and the running maximum m is taken over s_j
-// + log2 of the lane's largest scale (not below 2^-7), so that |P| <= 2^8 with the
-// largest near 1, and p <= 2^15.  m and E move lazily, when P would pass 2^8
-// or a scale 2^E.  Sums stay in f32 throughout.
+// 2^-11, an eighth of bf16's own).  f16's range is kept position by position: the
+// scales of position j are divided by their power 2^Dj (the smallest with all
+// |dV_jb| <= 2^Dj, within f16's normal numbers), p_j 2^Dj takes it, and the reference
+// m follows the largest s_j + Dj that the row sees: the products of the positions
+// that count most lie in [2^4, 2^14], and a huge value that a row does not see,
+// or sees with no weight, takes no bits from the others (a power that followed the
+// largest scale seen cost the f32 output up to 3 % behind one value of 5e5).  A
+// scale 2^14 below the largest of its own position keeps fewer bits, of its 2^-25.
+// m moves lazily, by 2^8.  Sums stay in f32 throughout.
 #include <algorithm>
 
 #include "rq_async.cuh"
@@ -48,7 +51,8 @@ namespace {
 constexpr int kWarps = 4;       // warps of a CTA
 constexpr int kStages = 3;      // pairs of tiles in flight per warp (few rows)
 constexpr int kStagesRows = 2;  // (many rows)
-constexpr float kLazy = 8.0f;   // log2 of the largest |P|
+constexpr float kLazy = 8.0f;   // log2 of how far P grows before the reference moves
+constexpr float kTop = 5.0f;    // log2 of the largest p 2^D where it has moved
 
 enum Mode { kSplit8, kOne16 };  // 8 rows of hi + lo parts, 16 rows of one part
 
@@ -113,6 +117,12 @@ __device__ __forceinline__ float lg2(float x) {
 }
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// For halves w >= 0: the smallest 2^D >= w with D in -14 .. 14 (above, 2^14: w is
+// 4 times that at most), 0 for 0.  2^-D has the exponent field 30 less this one's,
+// and for 0 some finite value.
+__device__ __forceinline__ uint32_t power(__half2 w) {
+    return as_u32(__hmin2(as_h2((as_u32(w) + 0x03FF03FFu) & 0x7C007C00u), __half2half2(__ushort_as_half(0x7400))));
+}
 // nibbles 0 and 4 (even) or 1 and 5 (odd) of w as f16 pairs c - 8: a nibble
 // placed in the mantissa of 1024 (or, four bits up, of 64) is that value + c.
 // The two constants come from the launch's parameters: known ones would be
@@ -215,9 +225,6 @@ struct Warp {
     static constexpr int kAcc = kAlone ? 2 : 4;  // kAlone: hi and lo rows together
     float oacc[MT][NB][4][kAcc];
     float m[H], l[H];
-    float E;
-    float bound;      // 2^E
-    __half2 inv;      // 2^-E
     int full0, full1;      // tiles that every row sees whole
     int seen;              // positions that any row sees end here
 
@@ -285,17 +292,11 @@ struct Warp {
 #pragma unroll
                     for (int i = 0; i < kAcc; i++) oacc[mt][b][n][i] = 0.0f;
         __syncwarp();  // the operands in shared memory are there
-        set_scale(-15);
         const int i0 = r0 / p.group, i1 = min(o.n_q - 1, (r0 + R - 1) / p.group);
         full1 = max(0, min(o.held, o.pos0 + i0 + 1)) / kKv4Tile;
         const int before = o.pos0 + i1 - p.window;  // positions up to here the last row no longer sees
         full0 = p.window > 0 && before >= 0 ? before / kKv4Tile + 1 : 0;
         seen = min(o.held, o.pos0 + i1 + 1);
-    }
-    __device__ __forceinline__ void set_scale(int e) {
-        E = (float)e;
-        bound = __int_as_float((127 + e) << 23);
-        inv = __float2half2_rn(__int_as_float((127 - e) << 23));
     }
     static __device__ __forceinline__ void add_products(float (&o)[kAcc], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         if constexpr (kAlone) {
@@ -412,6 +413,7 @@ struct Warp {
         }
         uint2 vs[NT][NB];
         uint32_t see[NT][H][2];  // halves of all ones: tokens that the row sees (used where !full)
+        uint32_t pw[NT][2];      // 2^D of the lane's tokens, f16; zero where all scales are
         float pr[NT][H][4], top[H];
         __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
@@ -427,21 +429,20 @@ struct Warp {
                 for (int x = 0; x < 4; x++) {
                     const int j = (tile_at + i) * kKv4Tile + 4 * t + x;
                     const uint32_t half = (x & 1) ? 0xFFFF0000u : 0x0000FFFFu;
-                    if (j >= seen) {  // nobody's: whatever scale lies there counts for nothing
-#pragma unroll
-                        for (int b = 0; b < NB; b++) {
-                            if (x < 2) vs[i][b].x &= ~half;
-                            else vs[i][b].y &= ~half;
-                        }
-                    }
 #pragma unroll
                     for (int h = 0; h < H; h++)
                         if (j >= seen || j > rpos[h] || (p.window > 0 && rpos[h] - j >= p.window)) see[i][h][x >> 1] &= ~half;
                 }
             }
-            // the largest V scale of this lane's tokens
+            // the power of each token's scales (a not-a-number one is passed over)
 #pragma unroll
-            for (int b = 0; b < NB; b++) big = __hmax2(big, __hmax2(__habs2(as_h2(vs[i][b].x)), __habs2(as_h2(vs[i][b].y))));
+            for (int x = 0; x < 2; x++) {
+                __half2 w = __habs2(as_h2(x ? vs[i][0].y : vs[i][0].x));
+#pragma unroll
+                for (int b = 1; b < NB; b++) w = __hmax2(w, __habs2(as_h2(x ? vs[i][b].y : vs[i][b].x)));
+                big = __hmax2(big, w);
+                pw[i][x] = power(w);
+            }
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 pr[i][h][0] = sc[i][0][h].x * qs[h];
@@ -458,43 +459,30 @@ struct Warp {
                 for (int x = 0; x < 4; x++) top[h] = fmaxf(top[h], pr[i][h][x]);
             }
         }
+        // No s + D of this lane passes its largest s plus its largest D: where that
+        // says that P stays in range the reference is not looked at
         const float2 big2 = __half22float2(big);
-        const float dmax = fmaxf(big2.x, big2.y);
-        float mx[H];
-        float lg = fmaxf(lg2(dmax) - E, -7.0f);
-        bool move = dmax > bound;
+        const float lg = kTop + kLazy - fmaxf(lg2(fmaxf(big2.x, big2.y)), -14.0f);
+        bool move = false;
 #pragma unroll
-        for (int h = 0; h < H; h++) {
-            mx[h] = top[h] + lg;
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            move |= mx[h] > m[h] + kLazy || (m[h] == -INFINITY && mx[h] > -INFINITY);
-        }
+        for (int h = 0; h < H; h++) move |= top[h] > m[h] + lg;  // (m -inf: anything that is seen)
         if (__any_sync(0xffffffffu, move)) {
-            if (__any_sync(0xffffffffu, dmax > bound)) {
-                float w = dmax;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-                int e;
-                frexpf(w, &e);  // w <= 2^e
-                const float down = __int_as_float((127 + (int)E - e) << 23);
-                float f[H];
-#pragma unroll
-                for (int h = 0; h < H; h++) f[h] = down;
-                scale_rows(f);
-                set_scale(e);
-                lg = fmaxf(lg2(dmax) - E, -7.0f);
-#pragma unroll
-                for (int h = 0; h < H; h++) {
-                    mx[h] = top[h] + lg;
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                }
-            }
             float al[H];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                const float mn = fmaxf(m[h], mx[h]);
+                float k = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        // no value at all counts for the sum of weights alone, which
+                        // holds 2^60 times the others' (and not infinity)
+                        const float2 u = unpack(pw[i][x]);
+                        k = fmaxf(k, fmaxf(pr[i][h][2 * x] + fmaxf(lg2(u.x), -60.0f), pr[i][h][2 * x + 1] + fmaxf(lg2(u.y), -60.0f)));
+                    }
+                k = fmaxf(k, __shfl_xor_sync(0xffffffffu, k, 1));
+                k = fmaxf(k, __shfl_xor_sync(0xffffffffu, k, 2));
+                const float mn = fmaxf(m[h], k - kTop);
                 al[h] = m[h] == -INFINITY ? 0.0f : ex2(m[h] - mn);
                 m[h] = mn;
                 l[h] *= al[h];
@@ -512,6 +500,9 @@ struct Warp {
                 l[h] += (pr[i][h][0] + pr[i][h][1]) + (pr[i][h][2] + pr[i][h][3]);
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
+                    const float2 u = unpack(pw[i][x]);
+                    pr[i][h][2 * x] *= u.x;
+                    pr[i][h][2 * x + 1] *= u.y;
                     ph[h][x] = pack(pr[i][h][2 * x], pr[i][h][2 * x + 1]);
                     if (MODE == kSplit8) {
                         const float2 back = unpack(ph[h][x]);
@@ -521,9 +512,10 @@ struct Warp {
                 }
             }
             src.v(i);
+            const uint32_t inv0 = 0x78007800u - pw[i][0], inv1 = 0x78007800u - pw[i][1];  // 2^-D
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const __half2 d01 = __hmul2(as_h2(vs[i][b].x), inv), d23 = __hmul2(as_h2(vs[i][b].y), inv);
+                const __half2 d01 = __hmul2(as_h2(vs[i][b].x), as_h2(inv0)), d23 = __hmul2(as_h2(vs[i][b].y), as_h2(inv1));
                 uint32_t a[MT][4];
 #pragma unroll
                 for (int h = 0; h < H; h++) {
@@ -573,7 +565,7 @@ struct Warp {
         src.first = 0;
     }
 
-    // Row sums complete, accumulators back at the values' scale.
+    // Row sums complete.
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int h = 0; h < H; h++) {
@@ -592,7 +584,7 @@ struct Warp {
                 v.y -= o[3];
             }
         }
-        return make_float2(v.x * bound, v.y * bound);
+        return v;
     }
 };
 

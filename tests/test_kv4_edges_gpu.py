@@ -1,0 +1,128 @@
+"""The paged operators where values, sizes and arguments are extreme, against
+the plain implementations (and the tolerances) of test_kv4_gpu.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_kv4_gpu import TYPES, attention_ref, close, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def gen(rq_ctx):
+    return torch.Generator(device="cuda").manual_seed(23)
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Setup:
+    """One sequence of n positions in pages of 16 that lie in random order,
+    and its last nq queries."""
+
+    def __init__(self, gen, kind, n, nq, kv, group, hd, k, v, q=None, scale=None, window=0):
+        from rustyllm_b200.kv4 import KV4Cache
+        self.n, self.nq, self.window, self.scale = n, nq, window, hd ** -0.5 if scale is None else scale
+        width = (n + 15) // 16
+        self.cache = KV4Cache(width + 1, 16, kv, hd)
+        self.table = torch.randperm(width + 1, generator=gen, device="cuda")[:width].to(torch.int32)[None].contiguous()
+        j = torch.arange(n, device="cuda")
+        self.slots = (self.table[0, j // 16] * 16 + j % 16).to(torch.int32)
+        self.cache.append(k, v, self.slots)
+        self.q = torch.randn(nq, kv * group, hd, generator=gen, device="cuda").to(TYPES[kind]) if q is None else q
+
+    def call(self):
+        return self.cache.attention(self.q, self.table, i32(self.n), cu_q=i32(0, self.nq), max_q=self.nq, scale=self.scale,
+                                    window=self.window)
+
+    def want(self):
+        every = torch.arange(self.cache.n_pages * 16, dtype=torch.int32, device="cuda")
+        rk, rv = (x.double().cpu().numpy() for x in self.cache.read(every))
+        return attention_ref(self.q.double().cpu().numpy(), rk, rv, self.table.cpu().numpy(), 16, [self.n], [0, self.nq],
+                             self.scale, self.window, self.cache.n_pages)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 3, 21])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_value_without_weight_costs_no_bits(gen, kind, nq, hd):
+    """The largest value that the cache can hold, at a position that every
+    query sees and none weighs (its score lies over 60 below the others'),
+    beside values of 0.05.  4 rows a kv head, 12 and 84: each form."""
+    n = 500
+    k, v = make(gen, n, 2, hd, kind)
+    v = (v.float() * 0.1).to(TYPES[kind])
+    q = torch.randn(nq, 8, hd, generator=gen, device="cuda").abs().to(TYPES[kind])
+    k[3] = -20
+    v[3] = 6e4 if kind == "f16" else 5.2e5
+    s = Setup(gen, kind, n, nq, 2, 4, hd, k, v, q)
+    close(s.call(), s.want(), slice(None), kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 21])
+@pytest.mark.parametrize("what", ["huge", "nan"])
+def test_values_before_the_window_do_not_enter(gen, kind, nq, what):
+    """The window of the first query starts inside a tile, behind a position
+    of huge or not-a-number keys and values."""
+    n, window = 300, 100
+    first = n - nq - window + 1  # the first position that any query sees
+    assert first % 16
+    k, v = make(gen, n, 2, 64, kind)
+    v = (v.float() * 0.1).to(TYPES[kind])
+    s = Setup(gen, kind, n, nq, 2, 4, 64, k, v, window=window)
+    want = s.want()
+    k[first - 1] = v[first - 1] = math.nan if what == "nan" else 6e4 if kind == "f16" else 5.2e5
+    s.cache.append(k, v, s.slots)
+    close(s.call(), want, slice(None), kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [2, 21])
+@pytest.mark.parametrize("what", ["huge", "nan"])
+def test_values_that_the_last_query_alone_sees_do_not_enter_others(gen, kind, nq, what):
+    n = 300
+    k, v = make(gen, n, 2, 64, kind)
+    v = (v.float() * 0.1).to(TYPES[kind])
+    s = Setup(gen, kind, n, nq, 2, 4, 64, k, v)
+    want = s.want()
+    k[-1] = v[-1] = math.nan if what == "nan" else 6e4 if kind == "f16" else 5.2e5
+    s.cache.append(k, v, s.slots)
+    close(s.call()[:-1], want, slice(0, nq - 1), kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("nq", [1, 21])
+@pytest.mark.parametrize("falls", [False, True])
+def test_values_that_grow_or_fall_over_the_sequence(gen, kind, nq, falls):
+    n = 400
+    k, v = make(gen, n, 2, 96, kind)
+    size = torch.logspace(-3.5, 3.5, n, device="cuda")
+    v = (v.float() * (size.flip(0) if falls else size)[:, None, None]).to(TYPES[kind])
+    s = Setup(gen, kind, n, nq, 2, 4, 96, k, v)
+    close(s.call(), s.want(), slice(None), kind)
+
+
+@pytest.mark.parametrize("nq", [1, 21])
+@pytest.mark.parametrize("size", [2.0 ** -19, 2.0 ** -16, 2.0 ** 14])
+def test_f32_accuracy_at_the_ends_of_the_scales(gen, nq, size):
+    """Scales down among f16's smallest numbers and up to its largest."""
+    k, v = make(gen, 200, 2, 64, "f32")
+    s = Setup(gen, "f32", 200, nq, 2, 4, 64, k, v * size)
+    got, want = s.call().double().cpu().numpy(), s.want()[0]
+    assert np.linalg.norm(got - want) / np.linalg.norm(want) < 2e-6
+
+
+def test_values_of_zero_next_to_others(gen):
+    """Positions without value still count in the sum of weights, however far
+    above the others their scores lie."""
+    k, v = make(gen, 100, 2, 64, "f32")
+    v[10:60] = 0
+    k[20] = 6
+    q = torch.randn(2, 8, 64, generator=gen, device="cuda").abs()
+    s = Setup(gen, "f32", 100, 2, 2, 4, 64, k, v, q)
+    close(s.call(), s.want(), slice(None), "f32")
