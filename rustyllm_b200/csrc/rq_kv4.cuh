@@ -192,15 +192,16 @@ __device__ __forceinline__ float kv4_quantize(const float (&x)[8], uint32_t (&c)
     // with the sign of d taken into x
     const uint32_t sign = __float_as_uint(d) & 0x80000000u;
     const float D = fabsf(d), inv = __frcp_rn(D), half = 0.5f * D;
+    constexpr int kMid = 0x4B400000;  // 12582912.0f
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float v = __uint_as_float(__float_as_uint(x[i]) ^ sign);
         const float z = fmaf(v, inv, 12582912.0f);  // 1.5 * 2^23: an integer in the low bits
         const float r = fmaf(12582912.0f - z, D, v);
-        int k = __float_as_int(z) - 0x4B400000 + 8;
+        int k = __float_as_int(z);  // kMid + the multiple, and in the order of z elsewhere (a negative z is a negative k)
         if (r >= half) k++;
         if (r < -half) k--;
-        c[i] = (uint32_t)min(max(k, 0), 15);
+        c[i] = (uint32_t)(min(max(k, kMid - 8), kMid + 7) - (kMid - 8));
     }
     return d;
 }

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv4_gpu import TYPES, attention_ref, close, make
+from test_kv4_gpu import TYPES, attention_ref, close, make, quantize_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -126,3 +126,28 @@ def test_values_of_zero_next_to_others(gen):
     q = torch.randn(2, 8, 64, generator=gen, device="cuda").abs()
     s = Setup(gen, "f32", 100, 2, 2, 4, 64, k, v, q)
     close(s.call(), s.want(), slice(None), "f32")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_finite_values_of_every_size_saturate_at_their_own_end(gen, kind):
+    """Elements from 5e5, where a block's scale reaches its end, to the largest
+    finite ones, of both signs, beside a larger one and a small one."""
+    from rustyllm_b200.kv4 import KV4Cache
+    from rustyllm_b200.rope import qk_norm_rope_append, rope_tables
+    sizes = torch.logspace(math.log10(5e5), 38.4, 600, dtype=torch.float64).float().to(TYPES[kind])
+    n = sizes.numel()
+    k = torch.randn(n, 2, 64, generator=gen, device="cuda").to(TYPES[kind])
+    sizes = sizes.cuda()
+    for head, sign in ((0, 1), (1, -1)):
+        k[:, head, 0], k[:, head, 33] = sign * sizes, sign * sizes
+        k[:, head, 7], k[:, head, 40] = -sign * sizes, sign * sizes * 0.75
+        k[1:, head, 9] = sign * sizes[:-1]
+    v = k.flip(0).contiguous()
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    every = KV4Cache(n // 16 + 1, 16, 2, 64), KV4Cache(n // 16 + 1, 16, 2, 64)
+    every[0].append(k, v, slots)
+    q = torch.zeros(n, 2, 64, device="cuda", dtype=TYPES[kind])
+    qk_norm_rope_append(every[1], q, k, v, slots % 4, slots, *rope_tables(4, 0))  # nothing is rotated
+    for cache in every:
+        for got, x in zip(cache.read(slots), (k, v)):
+            assert np.array_equal(got.cpu().numpy().astype(np.float64), quantize_ref(x.double().cpu().numpy()))
