@@ -386,7 +386,8 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * Sequence b holds kv_lens[b] positions, its newest tokens (already appended)
  * among them; position j lives in page block_table[b * table_stride + j /
  * page_size].  Its n queries are the rows cu_q[b] .. cu_q[b + 1] - 1 of q
- * (n <= max_q; cu_q NULL: row b, n = 1), query i at position kv_lens[b] - n +
+ * (n <= max_q; cu_q NULL: row b, n = 1; of more, the rows behind the first
+ * max_q are left as they were), query i at position kv_lens[b] - n +
  * i; it sees the positions j <= its own and, with window > 0, j > its own -
  * window.  out row = softmax_j(scale * q . k_j) v over the seen positions, in
  * f32 sums; query head h reads kv head h / (n_heads / n_kv_heads).  f32 and f16

@@ -51,6 +51,7 @@ namespace {
 constexpr int kWarps = 4;       // warps of a CTA
 constexpr int kStages = 3;      // pairs of tiles in flight per warp (few rows)
 constexpr int kStagesRows = 2;  // (many rows)
+constexpr int kMaxQ = 1 << 24;  // queries of a sequence
 constexpr float kLazy = 8.0f;   // log2 of how far P grows before the reference moves
 constexpr float kTop = 5.0f;    // log2 of the largest p 2^D where it has moved
 
@@ -175,10 +176,13 @@ struct Seq {
     int pos0, held;    // position of query 0; positions that the table can hold
     __device__ __forceinline__ Seq(const AttnP& p, int b) {
         q0 = p.cu_q ? p.cu_q[b] : b;
-        n_q = p.cu_q ? min(max(p.cu_q[b + 1] - q0, 0), p.max_q) : 1;
+        const int64_t n = p.cu_q ? max((int64_t)p.cu_q[b + 1] - q0, (int64_t)0) : 1;
+        n_q = (int)min(n, (int64_t)p.max_q);  // of more than the caller announced, the first ones, where they are
         const int len = max(p.kv_lens[b], 0);
         held = min(len, p.table_slots);
-        pos0 = len - n_q;
+        // no query that is computed lies further than max_q behind this bound, so
+        // those below it see nothing either way
+        pos0 = (int)max(len - n, -(int64_t)kMaxQ);
     }
     // tiles that queries i0 .. i1 see
     __device__ __forceinline__ void tiles(const AttnP& p, int i0, int i1, int& tile0, int& tile1) const {
@@ -1780,7 +1784,7 @@ int check_query(const rq_kv4* c, const rq_kv4_query* a, const char* fn) {
     if (a->n_heads < 1 || a->n_heads > 65536 || a->n_heads % c->n_kv)
         return set_error(RQ_ERR_INVALID, "%s: %lld query heads over %d kv heads", fn, (long long)a->n_heads, c->n_kv);
     if (a->batch < 0 || a->batch > INT32_MAX - 1 || a->n_tokens < 0 || a->n_tokens > INT32_MAX || a->max_q < 1 ||
-        a->max_q > (1 << 24) || a->table_width < 0 || a->table_width > INT32_MAX || a->max_len < 0 || a->window < 0)
+        a->max_q > kMaxQ || a->table_width < 0 || a->table_width > INT32_MAX || a->max_len < 0 || a->window < 0)
         return set_error(RQ_ERR_INVALID,
                          "%s: batch %lld, n_tokens %lld, max_q %lld, table_width %lld, max_len %lld, window %lld", fn,
                          (long long)a->batch, (long long)a->n_tokens, (long long)a->max_q, (long long)a->table_width,
@@ -1884,7 +1888,7 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     p.table = a->block_table;
     p.table_stride = a->table_stride;
     p.table_slots = (int)(a->table_width * c->page_size);
-    // positions stay below 2^31 and a query is never more than max_q below 0,
+    // positions stay below 2^31 and a query is never more than kMaxQ below 0,
     // so a window this long hides nothing and its differences fit 32 bits
     p.window = a->window < (1 << 30) * 2ll - (1 << 25) ? (int)a->window : 0;
     p.scale = a->scale * 1.44269504088896340736f;

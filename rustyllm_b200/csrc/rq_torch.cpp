@@ -7,6 +7,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <optional>
 #include <string>
 
 #include "../../include/rq.h"
@@ -114,7 +116,7 @@ py::tuple read(const Cache& c, const Tensor& slots, at::ScalarType type) {
 }
 
 Tensor attention(const Cache& c, const Tensor& q, const Tensor& block_table, const Tensor& kv_lens, const OptTensor& cu_q,
-                 int64_t max_q, double scale, int64_t window, const OptTensor& out, int64_t max_len) {
+                 const std::optional<int64_t>& max_q, double scale, int64_t window, const OptTensor& out, int64_t max_len) {
     if (q.dim() != 3) refuse("q: [tokens, heads, head_dim] is wanted");
     rows(q, "q", q.size(1), c.dim, c.dev);
     if (table(block_table, -1, "block_table") != c.dev) refuse("block_table: on " + cuda(c.dev) + " is wanted");
@@ -132,7 +134,7 @@ Tensor attention(const Cache& c, const Tensor& q, const Tensor& block_table, con
     a.n_tokens = q.size(0);
     a.n_heads = q.size(1);
     a.batch = batch;
-    a.max_q = max_q;
+    a.max_q = max_q ? *max_q : cu_q ? std::max<int64_t>(q.size(0), 1) : 1;
     a.block_table = block_table.data_ptr<int32_t>();
     a.table_stride = block_table.stride(0);
     a.table_width = block_table.size(1);

@@ -49,12 +49,14 @@ class KV4Cache:
         (zeros for a slot outside the cache)."""
         return _rqtorch.read(self.native, slots, dtype)
 
-    def attention(self, q, block_table, kv_lens, cu_q=None, max_q: int = 1, scale: float | None = None, window: int = 0,
+    def attention(self, q, block_table, kv_lens, cu_q=None, max_q: int | None = None, scale: float | None = None, window: int = 0,
                   out=None, max_len: int = 0):
         """Attention of the newest tokens of each sequence over the cache:
         q [tokens, n_heads, head_dim], block_table [batch, width] and kv_lens
         [batch] int32; without cu_q one query a sequence, with it (int32
-        [batch + 1]) the rows cu_q[b] .. cu_q[b + 1] - 1, at most max_q each.
+        [batch + 1]) the rows cu_q[b] .. cu_q[b + 1] - 1, at most max_q each
+        (rows behind that are not computed; without max_q any number is, by the
+        form for many rows: give it where it is small).
         Causal; window > 0 limits a query to that many newest positions.
         Rows that belong to no sequence are left as they are in ``out`` (and
         undefined where ``out`` is not given).  max_len, an upper bound of

@@ -151,3 +151,36 @@ def test_finite_values_of_every_size_saturate_at_their_own_end(gen, kind):
     for cache in every:
         for got, x in zip(cache.read(slots), (k, v)):
             assert np.array_equal(got.cpu().numpy().astype(np.float64), quantize_ref(x.double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("kind,kv,group", [("f32", 2, 1), ("bf16", 2, 1), ("f32", 1, 16), ("bf16", 1, 16), ("bf16", 1, 40)])
+def test_sequences_of_more_queries_than_announced(gen, kind, kv, group):
+    """The first max_q rows of each sequence at their own positions (two of
+    them before the first one held), the others left as they were; without
+    max_q all of them."""
+    from rustyllm_b200.kv4 import KV4Cache
+    n, lens = 4 + 18 + 7, [60, 100, 5]
+    cache = KV4Cache(24, 16, kv, 64)
+    k, v = make(gen, 24 * 16, kv, 64, kind)
+    every = torch.arange(24 * 16, dtype=torch.int32, device="cuda")
+    cache.append(k, v, every)
+    rk, rv = (x.double().cpu().numpy() for x in cache.read(every))
+    table = torch.randperm(24, generator=gen, device="cuda")[:21].view(3, 7).to(torch.int32)
+    q = torch.randn(n, kv * group, 64, generator=gen, device="cuda").to(TYPES[kind])
+    cu = [0, 4, 22, 29]
+    want = attention_ref(q.double().cpu().numpy(), rk, rv, table.cpu().numpy(), 16, lens, cu, 0.125, 0, 24)
+    for most in (4, 1):
+        out = torch.full_like(q, 9.0)
+        cache.attention(q, table, i32(*lens), cu_q=i32(*cu), max_q=most, out=out)
+        first = [r for b in range(3) for r in range(cu[b], min(cu[b] + most, cu[b + 1]))]
+        close(out[first], want, first, kind)
+        rest = [r for r in range(n) if r not in first]
+        assert (out[rest] == 9).all()
+    close(cache.attention(q, table, i32(*lens), cu_q=i32(*cu)), want, slice(None), kind)
+    # offsets that say anything at all: nothing outside the rows is read or written
+    out = torch.full_like(q, 9.0)
+    cache.attention(q, table, i32(*lens), cu_q=i32(-2 ** 31, 2 ** 31 - 1, 28, 29), max_q=4, out=out, window=2 ** 31 - 1)
+    assert (out[:28] == 9).all() and out[28].isfinite().all()
+    if kind == "f32":
+        last = attention_ref(q.double().cpu().numpy(), rk, rv, table.cpu().numpy()[2:], 16, lens[2:], [28, 29], 0.125, 0, 24)
+        close(out[28:], last, [28], kind)
