@@ -1791,6 +1791,10 @@ int check_query(const rq_kv4* c, const rq_kv4_query* a, const char* fn) {
                          (long long)a->max_len, (long long)a->window);
     if (a->table_width * c->page_size > INT32_MAX)
         return set_error(RQ_ERR_INVALID, "%s: a table of %lld pages passes 2^31 positions", fn, (long long)a->table_width);
+    // (in floating point: the product of the largest passes 64 bits)
+    if ((double)a->batch * (double)a->n_heads * (double)(a->cu_q ? a->max_q : 1) > (double)INT32_MAX)
+        return set_error(RQ_ERR_INVALID, "%s: too many rows for one call: %lld sequences of up to %lld queries of %lld heads", fn,
+                         (long long)a->batch, (long long)(a->cu_q ? a->max_q : 1), (long long)a->n_heads);
     if (!a->cu_q && a->n_tokens < a->batch)
         return set_error(RQ_ERR_INVALID, "%s: %lld tokens for %lld sequences of one query each", fn, (long long)a->n_tokens,
                          (long long)a->batch);

@@ -184,3 +184,16 @@ def test_sequences_of_more_queries_than_announced(gen, kind, kv, group):
     if kind == "f32":
         last = attention_ref(q.double().cpu().numpy(), rk, rv, table.cpu().numpy()[2:], 16, lens[2:], [28, 29], 0.125, 0, 24)
         close(out[28:], last, [28], kind)
+
+
+def test_rows_past_32_bits_are_refused(gen):
+    """2^38 rows of a kv head and some: their number of row tiles, cut to 32
+    bits, would be a small one."""
+    from rustyllm_b200 import RqError
+    from rustyllm_b200.kv4 import KV4Cache
+    cache = KV4Cache(1, 16, 1, 32)
+    q = torch.zeros(1, 65536, 32, device="cuda")
+    for most in (2 ** 22 + 16, 2 ** 24, 2 ** 15):
+        with pytest.raises(RqError, match="too many rows"):
+            cache.attention(q, i32(0)[None], i32(1), cu_q=i32(0, 1), max_q=most)
+    assert not cache.attention(q, i32(0)[None], i32(1), cu_q=i32(0, 1), max_q=2).any()
