@@ -399,7 +399,8 @@ RQ_API int rq_kv4_read(rq_kv4* c, const int32_t* slots, int64_t n, int dtype, vo
  * that sees nothing gets zeros.  Positions behind table_width * page_size or
  * on a page outside the cache are not seen.  Rows of q and out that belong to
  * no sequence (or lie at or behind n_tokens) are left as they were.  out may
- * be q.  max_len (> 0): an upper bound of kv_lens that only guides how the
+ * be q, otherwise the two must not overlap; rows of out that overlap one
+ * another are refused.  max_len (> 0): an upper bound of kv_lens that only guides how the
  * work is split (0: table_width * page_size).  One form serves the whole
  * call, chosen by max_q: single tokens on long caches are faster in a call of
  * their own than among prompts.  `workspace` holds at least
@@ -429,7 +430,8 @@ RQ_API int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream);
  * 2i with 2i + 1).  cos, sin: f32 [max_pos][rot_dim / 2].  Computed in f32,
  * rounded once.  A token whose position lies outside 0..max_pos-1 (-1:
  * padding) leaves its output rows as they were.  q_out may be q and k_out may
- * be k; otherwise outputs and inputs must not overlap.  n_heads or n_kv_heads
+ * be k; otherwise outputs and inputs must not overlap, and rows of an output
+ * that overlap one another are refused.  n_heads or n_kv_heads
  * may be 0.  head_dim even, at most 256. */
 typedef struct rq_qk_rope {
     int dtype;

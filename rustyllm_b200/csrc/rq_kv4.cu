@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 
 #include "rq_kv4.cuh"
 
@@ -22,6 +23,26 @@ int check_device_ptr(const rq_ctx* ctx, const void* p, const char* fn, const cha
     if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != ctx->device))
         return set_error(RQ_ERR_INVALID, "%s: %s must be device memory on device %d", fn, name, ctx->device);
     return RQ_OK;
+}
+
+int check_rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len, const char* fn, const char* name) {
+    using wide = __int128;
+    if (n0 < 1 || n1 < 1) return RQ_OK;
+    // the larger stride's axis is `a`; an axis of one row has none
+    wide sa = n0 > 1 ? (s0 < 0 ? -(wide)s0 : s0) : 0, sb = n1 > 1 ? (s1 < 0 ? -(wide)s1 : s1) : 0;
+    if (sa < sb) {
+        std::swap(sa, sb);
+        std::swap(n0, n1);
+    }
+    bool meet = (n0 > 1 && sa < len) || (n1 > 1 && sb < len);
+    // rows i of a and j of b lie i sa - j sb apart: nothing meets where a steps
+    // over all of b, else the nearest j of each i say
+    const wide span = n1 > 1 ? sb * (n1 - 1) : 0;
+    for (int64_t i = 1; !meet && n1 > 1 && i < n0 && i * sa < span + len; i++) {
+        const wide j = i * sa / sb, off = i * sa - j * sb;
+        meet = (j < n1 && off < len) || (j + 1 < n1 && sb - off < len);
+    }
+    return meet ? set_error(RQ_ERR_INVALID, "%s: %s: its rows lie on one another", fn, name) : RQ_OK;
 }
 
 int launch_pdl(const void* fn, unsigned grid, unsigned block, size_t smem, cudaStream_t st, void** args, const char* what,
@@ -513,8 +534,11 @@ int check_rope(const rq_ctx* ctx, const rq_qk_rope* a, bool append, const char* 
         if (!rc) rc = check_device_ptr(ctx, a->positions, fn, "positions");
         if (!rc && a->n_heads) rc = check_device_ptr(ctx, a->q, fn, "q");
         if (!rc && a->n_heads) rc = check_device_ptr(ctx, a->q_out, fn, "q_out");
+        if (!rc) rc = check_rows_apart(a->n_tokens, a->q_out_stride[0], a->n_heads, a->q_out_stride[1], a->head_dim, fn, "q_out");
         if (!rc && a->n_kv_heads) rc = check_device_ptr(ctx, a->k, fn, "k");
         if (!rc && a->n_kv_heads && !append) rc = check_device_ptr(ctx, a->k_out, fn, "k_out");
+        if (!rc && !append)
+            rc = check_rows_apart(a->n_tokens, a->k_out_stride[0], a->n_kv_heads, a->k_out_stride[1], a->head_dim, fn, "k_out");
         if (!rc && a->rot_dim) rc = check_device_ptr(ctx, a->cos, fn, "cos");
         if (!rc && a->rot_dim) rc = check_device_ptr(ctx, a->sin, fn, "sin");
         if (!rc && a->q_weight) rc = check_device_ptr(ctx, a->q_weight, fn, "q_weight");

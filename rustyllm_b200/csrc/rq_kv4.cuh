@@ -283,6 +283,9 @@ struct DevGuard {  // the context's device for the duration of a call
 };
 // RQ_OK when p is device memory on ctx's device, else an error that names it
 int check_device_ptr(const rq_ctx* ctx, const void* p, const char* fn, const char* name);
+// RQ_OK when no two rows of an output [n0][n1] (strides s0, s1, rows of len
+// contiguous elements) share an element
+int check_rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len, const char* fn, const char* name);
 // a launch that may begin while the previous kernel of the stream drains
 // (the kernel waits with griddepcontrol.wait before it touches memory);
 // cluster > 1: thread-block clusters of that many CTAs along x

@@ -1948,6 +1948,7 @@ int rq_kv4_attention(rq_kv4* c, const rq_kv4_query* a, void* stream) {
     const rq_ctx* ctx = c->ctx;
     rc = check_device_ptr(ctx, a->q, fn_name, "q");
     if (!rc) rc = check_device_ptr(ctx, a->out, fn_name, "out");
+    if (!rc) rc = check_rows_apart(a->n_tokens, a->out_stride[0], a->n_heads, a->out_stride[1], c->head_dim, fn_name, "out");
     if (!rc) rc = check_device_ptr(ctx, a->kv_lens, fn_name, "kv_lens");
     if (!rc && a->cu_q) rc = check_device_ptr(ctx, a->cu_q, fn_name, "cu_q");
     if (!rc && a->table_width) rc = check_device_ptr(ctx, a->block_table, fn_name, "block_table");

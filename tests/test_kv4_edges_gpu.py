@@ -197,3 +197,40 @@ def test_rows_past_32_bits_are_refused(gen):
         with pytest.raises(RqError, match="too many rows"):
             cache.attention(q, i32(0)[None], i32(1), cu_q=i32(0, 1), max_q=most)
     assert not cache.attention(q, i32(0)[None], i32(1), cu_q=i32(0, 1), max_q=2).any()
+
+
+def test_outputs_whose_rows_overlap_in_part_are_refused(gen):
+    """Every layout of [tokens, heads] in which two rows share an element, and
+    none of the others: transposed, inside a packed matrix, interleaved."""
+    from rustyllm_b200 import RqError
+    from rustyllm_b200.kv4 import KV4Cache
+    from rustyllm_b200.rope import qk_norm_rope, qk_norm_rope_append, rope_tables
+    cache = KV4Cache(2, 16, 2, 32)
+    k, v = make(gen, 32, 2, 32, "f32")
+    cache.append(k, v, torch.arange(32, dtype=torch.int32, device="cuda"))
+    tables = rope_tables(8, 32)
+    refused = 0
+    for n, h in ((3, 4), (5, 2), (1, 4)):
+        q = torch.randn(n, h, 32, generator=gen, device="cuda")
+        pos = torch.arange(n, dtype=torch.int32, device="cuda")
+        args = dict(cu_q=i32(0, n), max_q=n)
+        table, lens = i32(0, 1)[None], i32(20)
+        plain = cache.attention(q, table, lens, **args), *qk_norm_rope(q, k[:n], pos, *tables)
+        for st, sh in ((32, 32 * n), (32 * h, 32), (31, 200), (200, 31), (64, 32), (96, 64), (64, 96), (64, 95), (96, 33), (160, 64), (80, 48),
+                       (32 * h - 1, 32), (7 * 32, 40), (0, 32)):
+            cells = torch.zeros(n, h, 32, dtype=torch.int64)
+            at = (torch.arange(n)[:, None, None] * st + torch.arange(h)[:, None] * sh + torch.arange(32) + cells).reshape(-1)
+            apart = at.unique().numel() == at.numel()
+            out = torch.zeros(4096, device="cuda").as_strided((n, h, 32), (st, sh, 1))
+            calls = (lambda: cache.attention(q, table, lens, out=out, **args),
+                     lambda: qk_norm_rope(q, k[:n], pos, *tables, q_out=out)[0],
+                     lambda: qk_norm_rope_append(cache, q, k[:n], v[:n], pos, pos - 40, *tables, q_out=out),
+                     lambda: qk_norm_rope(k[:n], q, pos, *tables, k_out=out)[1])
+            for call, want in zip(calls, (plain[0], plain[1], plain[1], plain[1])):
+                if apart:
+                    assert torch.allclose(call(), want, rtol=1e-5, atol=1e-5)
+                else:
+                    refused += 1
+                    with pytest.raises(RqError, match="lie on one another"):
+                        call()
+    assert refused == 60  # 15 of the 42 layouts
