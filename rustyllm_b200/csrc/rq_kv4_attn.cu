@@ -1287,7 +1287,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             int e2 = 0;
             if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e2);
-            e2 = max(-110, min(110, e2));
+            e2 = max(-120, min(120, e2));
             // the scale's sign is the operand's, so that scores grow with their sums
             const float down = p.scale == 0.0f ? 0.0f : copysignf(__int_as_float((127 - e2) << 23), p.scale);
             if ((lane & 1) == 0) s_qs[row] = p.scale == 0.0f ? 1.0f : __int_as_float((127 + e2) << 23) * fabsf(p.scale);

@@ -234,3 +234,17 @@ def test_outputs_whose_rows_overlap_in_part_are_refused(gen):
                     with pytest.raises(RqError, match="lie on one another"):
                         call()
     assert refused == 60  # 15 of the 42 layouts
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("nq", [1, 3, 20])
+@pytest.mark.parametrize("size", [2.0 ** 127, 2.0 ** 100, 2.0 ** -100, 2.0 ** -125])
+def test_queries_of_every_finite_size(gen, kind, nq, size):
+    """Queries near both ends of the type's range, the softmax scale bringing
+    the scores back."""
+    k, v = make(gen, 90, 2, 64, kind)
+    small = 2.0 ** -6 if size > 1 else 2.0 ** 6
+    q = (torch.randn(nq, 8, 64, generator=gen, device="cuda").clamp(-1.9, 1.9).double() * size).to(TYPES[kind])
+    assert q.isfinite().all() and q.abs().amax() > size
+    s = Setup(gen, kind, 90, nq, 2, 4, 64, (k.float() * small).to(TYPES[kind]), v, q, scale=0.1 / small / size)
+    close(s.call(), s.want(), slice(None), kind)
