@@ -88,7 +88,7 @@ void pair(int64_t (&s)[2], const Tensor& t) {
 // ------------------------------------------------------------------ cache
 
 struct Cache {
-    rq_kv4* handle;
+    rq_kv4* handle;  // NULL once closed: the entries refuse it
     int64_t heads, dim;
     int dev;
 };
@@ -296,7 +296,7 @@ py::tuple spec_verify(uintptr_t ctx, const Tensor& p, const Tensor& drafts, cons
 PYBIND11_MODULE(_rqtorch, m) {
     py::class_<Cache>(m, "Cache").def(py::init([](uintptr_t handle, int64_t heads, int64_t dim, int dev) {
         return Cache{(rq_kv4*)handle, heads, dim, dev};
-    }));
+    })).def("close", [](Cache& c) { c.handle = nullptr; });
     m.def("append", &append);
     m.def("read", [](const Cache& c, const Tensor& slots, py::object dtype) {
         return read(c, slots, torch::python::detail::py_object_to_dtype(std::move(dtype)));

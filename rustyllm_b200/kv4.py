@@ -65,9 +65,10 @@ class KV4Cache:
                                   window, out, max_len)
 
     def close(self) -> None:
-        """Frees the cache; it must not be used afterwards."""
+        """Frees the cache; calls that use it afterwards raise RqError."""
         if self.handle:
-            self.native = None
+            if hasattr(self, "native"):
+                self.native.close()
             _lib.lib().rq_kv4_free(self.handle)
             self.handle = None
 

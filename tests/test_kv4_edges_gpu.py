@@ -248,3 +248,21 @@ def test_queries_of_every_finite_size(gen, kind, nq, size):
     assert q.isfinite().all() and q.abs().amax() > size
     s = Setup(gen, kind, 90, nq, 2, 4, 64, (k.float() * small).to(TYPES[kind]), v, q, scale=0.1 / small / size)
     close(s.call(), s.want(), slice(None), kind)
+
+
+def test_a_closed_cache_refuses_every_call(gen):
+    from rustyllm_b200 import RqError
+    from rustyllm_b200.kv4 import KV4Cache
+    from rustyllm_b200.rope import qk_norm_rope_append, rope_tables
+    cache = KV4Cache(1, 16, 2, 32)
+    k, v = make(gen, 1, 2, 32, "f32")
+    calls = (lambda: cache.append(k, v, i32(0)), lambda: cache.append(k[:0], v[:0], i32()), lambda: cache.read(i32(0)),
+             lambda: cache.attention(k, i32(0)[None], i32(1)), lambda: cache.device_bytes(),
+             lambda: qk_norm_rope_append(cache, k, k, v, i32(0), i32(0), *rope_tables(1, 32)))
+    for call in calls:
+        call()
+    cache.close()
+    cache.close()
+    for call in calls:
+        with pytest.raises(RqError, match="NULL"):
+            call()
