@@ -14,11 +14,13 @@ from __future__ import annotations
 
 from collections import deque
 
-import torch
-
 from .linear import Context
 
-from . import _rqtorch  # isort: skip  (needs torch's libraries loaded)
+try:  # greedy decoding needs neither torch nor its binding
+    import torch
+except Exception:  # pragma: no cover
+    torch = None
+_rqtorch = None  # the binding, from the first verification on
 
 
 def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
@@ -29,6 +31,9 @@ def spec_verify(p, drafts, u, r, q=None, n_drafts=None):
     (float32); rq_spec_verify of include/rq.h.  n_drafts [batch] (int32)
     limits a row's drafts.  A row of tokens is the accepted drafts, one drawn
     token and -1s; with n = 0 the call samples from p."""
+    global _rqtorch
+    if _rqtorch is None:
+        from . import _rqtorch
     return _rqtorch.spec_verify(Context.of(p), p, drafts, u, r, q, n_drafts)
 
 
