@@ -51,6 +51,7 @@ namespace {
 constexpr int kWarps = 4;       // warps of a CTA
 constexpr int kStages = 3;      // pairs of tiles in flight per warp (few rows)
 constexpr int kStagesRows = 2;  // (many rows)
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxQ = 1 << 24;  // queries of a sequence
 constexpr float kLazy = 8.0f;   // log2 of how far P grows before the reference moves
 constexpr float kTop = 5.0f;    // log2 of the largest p 2^D where it has moved
@@ -1798,8 +1799,8 @@ int check_query(const rq_kv4* c, const rq_kv4_query* a, const char* fn) {
     if (!a->cu_q && a->n_tokens < a->batch)
         return set_error(RQ_ERR_INVALID, "%s: %lld tokens for %lld sequences of one query each", fn, (long long)a->n_tokens,
                          (long long)a->batch);
-    if (!(a->scale == a->scale) || a->scale - a->scale != 0.0f)
-        return set_error(RQ_ERR_INVALID, "%s: scale is not finite", fn);
+    const float scale = a->scale * kLog2e;
+    if (scale - scale != 0.0f) return set_error(RQ_ERR_INVALID, "%s: scale is not finite (or passes f32 in base 2)", fn);
     return RQ_OK;
 }
 
@@ -1895,7 +1896,7 @@ int kv4_attention(const rq_kv4* c, const rq_kv4_query* a, int* err, cudaStream_t
     // positions stay below 2^31 and a query is never more than kMaxQ below 0,
     // so a window this long hides nothing and its differences fit 32 bits
     p.window = a->window < (1 << 30) * 2ll - (1 << 25) ? (int)a->window : 0;
-    p.scale = a->scale * 1.44269504088896340736f;
+    p.scale = a->scale * kLog2e;
     p.part = static_cast<float*>(a->workspace);
     if (need) {
         // sums, then the pairs (descriptions first: they want 16 bytes)

@@ -266,3 +266,13 @@ def test_a_closed_cache_refuses_every_call(gen):
     for call in calls:
         with pytest.raises(RqError, match="NULL"):
             call()
+
+
+def test_scales_that_pass_f32_in_base_2_are_refused(gen):
+    from rustyllm_b200 import RqError
+    from rustyllm_b200.kv4 import KV4Cache
+    cache = KV4Cache(1, 16, 1, 32)
+    for scale in (3e38, -2.4e38, 1e39, math.nan):
+        with pytest.raises(RqError, match="scale"):
+            cache.attention(torch.zeros(1, 1, 32, device="cuda"), i32(0)[None], i32(1), scale=scale)
+    assert not cache.attention(torch.zeros(1, 1, 32, device="cuda"), i32(0)[None], i32(1), scale=2.3e38).any()
