@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(const __grid_c
     pdl_wait();
     __shared__ float rows[16][132];
     const int lane = threadIdx.x & 31, sl = lane & 15, gidx = threadIdx.x >> 4;
-    const int H = p.r.heads[0], kv = p.a.n_kv, per = H + 2 * kv, nb = p.a.nb, hd = 32 * nb;
+    const int H = p.r.heads[0], kv = p.a.n_kv, per = H + 2 * kv, nb = p.a.nb;
     const int64_t gi = (int64_t)blockIdx.x * 16 + gidx;
     const int64_t n = gi / per;
     bool live = n < p.a.n;

@@ -216,6 +216,7 @@ __device__ __forceinline__ void unit_tiles(const AttnP& p, const Rows& o, int& t
 // memory (`as`: [MT][NB][2][32 lanes]).
 template <int NB, int MODE, typename T, int MT, bool AS>
 struct Warp {
+    static_assert(MODE == kSplit8 || MT == 1, "16 rows of one part fill an operand tile's both halves");
     static constexpr int R1 = MODE == kOne16 ? 16 : 8, R = R1 * MT;
     static constexpr int HH = MODE == kOne16 ? 2 : 1, H = HH * MT;  // rows a lane: of an operand tile, in all
     uint32_t aq[AS ? 1 : NB][2][4];
@@ -1034,10 +1035,10 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
 // Bound by the issue of products and of what surrounds them (mma.sync, 255
 // registers, two CTAs an SM): three prompts of up to 300 tokens on up to 4500
 // positions, 64 f32 heads on 8, head_dim 128, take 650 us.
-template <int NB, int MODE, typename T>
+template <int NB, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
-    using W = Warp<NB, MODE, T, 2, true>;
+    using W = Warp<NB, kSplit8, T, 2, true>;
     constexpr int R = W::R, H = W::H, HD = 32 * NB, kLists = kWarps / 2;
     constexpr int kOps = SharedSrc<NB>::kOps;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1740,7 +1741,7 @@ Fns fns_of(bool rows, bool pair) {
                 return Fns{(const void*)kv4_attn_tc_kernel<NB, true, T>, (const void*)kv4_join_rows_kernel<NB, 2 * kTcRows, T>};
             return Fns{(const void*)kv4_attn_tc_kernel<NB, false, T>, (const void*)kv4_join_rows_kernel<NB, kTcRows, T>};
         } else {
-            return Fns{(const void*)kv4_attn_rows_kernel<NB, MODE, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
+            return Fns{(const void*)kv4_attn_rows_kernel<NB, T>, (const void*)kv4_join_rows_kernel<NB, 2 * R * kWarps, T>};
         }
     }
     return Fns{(const void*)kv4_attn_kernel<NB, MODE, T>, (const void*)kv4_join_kernel<NB, R, T>};
