@@ -74,9 +74,13 @@ bool wide_ok(const void* p, int64_t s0, int64_t s1, size_t size) {
 
 // ------------------------------------------------------------------ append
 //
-// One thread per 8 elements, the aligned four lanes holding a block of 32; a
-// CTA takes `per_cta` tokens (about two items a thread), so that indexes are
-// 32-bit inside it.  Bound by memory: 16 (or 32) bytes in, 4.5 out, per item.
+// A lane takes 8 elements of a block of 32 (an item) and a CTA whole tokens
+// (`per_cta`, see tokens_per_cta), so that a warp's reads are whole lines and indexes
+// are 32-bit inside it; the largest magnitude crosses four lanes by shuffles, a
+// code is decided without rounding (rq_kv4.cuh).  Bound by the issue of the
+// quantizer's instructions (84 % of the slots; 46 an element): 16001 tokens of 8
+// heads of 128 in bf16 take 50 us (84 MB, 1.7 TB/s), in f32 49; 64 in f32 2.3 us,
+// one launch and one round trip.
 struct AppendP {
     const void* x[2];          // k, v
     int64_t tok[2], head[2];   // strides in elements
@@ -86,13 +90,6 @@ struct AppendP {
     uint8_t* data;
     int page_size, n_kv, nb, per_cta;
 };
-
-// Append: a lane takes 8 elements of a block of 32 and a CTA whole tokens, so that
-// a warp's reads are whole lines; the largest magnitude crosses four lanes by
-// shuffles, a code is decided without rounding (rq_kv4.cuh).  Bound by the loads
-// in flight and the scattered 4-byte code words: 16001 tokens of 8 heads of 128 in
-// bf16 take 81 us with reading them back into bf16 (235 MB, 2.9 TB/s), 64 in f32
-// 4.3 us.
 
 // Item i of a CTA's tokens: row (K's heads, then V's, of a token) and 8 elements
 struct Item {
@@ -126,7 +123,9 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
 }
 
 // k and v rows of the given slots, dequantized; zeros for a slot outside the
-// cache.  The append's thread mapping.
+// cache.  The append's thread mapping.  Bound by memory and the
+// scattered code words: 16001 tokens of 8 heads of 128 take 28 us into bf16 (84 MB,
+// 3.0 TB/s), 35 into f32 (150 MB, 4.3 TB/s).
 struct ReadP {
     const uint8_t* data;
     const int32_t* slots;
@@ -426,7 +425,11 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_rows_kernel(const __grid_
 
 // The same with the append: 16 lanes a row of q, k or v (head_dim <= 128),
 // 8 consecutive elements a lane as the blocks of the cache want them; the
-// rotation's partner comes through shared memory.
+// rotation's partner comes through shared memory.  For decode steps: 5 tokens of 64
+// + 8 + 8 heads of 128 take 3.5 us in f32 (rotation and append one after the other
+// 4.2), 64 4.5 (4.8).  At 8191 tokens the angles and weights fetched by element,
+// the row's way through shared memory and a 64-bit division a row bound it: 189 us
+// in bf16 and 211 in f32, where the two passes take 114 and 134.
 struct RopeAppendP {
     RopeP r;  // y[1] unused
     bool wide_q, wide_qo;
@@ -603,8 +606,8 @@ const void* read_fn(int dtype, int nb) {
     return dtype == RQ_F32 ? read_fn<float>(nb) : dtype == RQ_F16 ? read_fn<__half>(nb) : read_fn<__nv_bfloat16>(nb);
 }
 
-// Tokens of an append or read CTA: about four items a thread where the tokens
-// fill the device anyway, else one.
+// Tokens of an append or read CTA: four items a thread where the tokens fill the
+// device anyway, else one (more where a token alone has more items than threads).
 int tokens_per_cta(const rq_kv4* c, int64_t n) {
     const int64_t items = (int64_t)2 * c->n_kv * (c->head_dim / 8);
     const int64_t want = n * items > (int64_t)c->ctx->sm_count * 2048 * 4 ? 1024 : 256;

@@ -768,10 +768,10 @@ constexpr bool kInShared = NB > 2;
 // begins its range, 2 i + 1 where it starts later) and the CTA that starts it
 // says in desc[i] how many there are.
 //
-// Bound by the issue of the instructions that unpack the codes (some 400 a tile of
+// Bound by the issue of the instructions that unpack the codes (some 430 a tile of
 // 16 positions, head_dim 128, at 2 a cycle and SM): 64 sequences of up to 8192
-// positions, 32 bf16 heads on 8, take 113 us (2.7 TB/s of the cache), 131072
-// positions of one under 64 f32 heads on 8 59 us (2.5 TB/s), 2000 of one 12.9 us
+// positions, 32 bf16 heads on 8, take 109 us (2.8 TB/s of the cache), 131072
+// positions of one under 64 f32 heads on 8 59 us (2.5 TB/s), 2000 of one 12.7 us
 // (two launches and a CTA's latencies).
 constexpr int kHead = 8;
 constexpr int kChunk = 128;  // sequences looked up at a time
@@ -1033,8 +1033,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<NB>) kv4_attn_kernel(const
 // stream.  Two warps share a stream: one unpacks its K, the other its V into
 // f16 operands that all four use.
 // Bound by the issue of products and of what surrounds them (mma.sync, 255
-// registers, two CTAs an SM): three prompts of up to 300 tokens on up to 4500
-// positions, 64 f32 heads on 8, head_dim 128, take 650 us.
+// registers, two CTAs an SM): three prompts of 300, 150 and 225 tokens on 1600,
+// 3100 and 4500 positions, 64 heads on 8, head_dim 128, take 552 us in f32 and
+// 548 in f16 (bf16, on tcgen05: 132).
 template <int NB, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __grid_constant__ AttnP p) {
     using Rec = Kv4Rec<NB>;
@@ -1180,11 +1181,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 //           waited for the products two steps before, 3400 cycles a step where
 //           this takes 2000)
 //
-// 254 us at three prompts of 256 - 512 tokens on up to 4500 positions, 64 query
-// heads on 8, head_dim 128 (297 TFLOP/s): the chains of the softmax (TMEM read,
-// maximum, exponentials, TMEM write) and of the unpacking bound it, at 1.8
-// instructions a cycle and SM, and the last wave's length (288 CTAs on 148 SMs); the
-// tensor pipe is busy for a quarter of the time.
+// Three prompts of 512 tokens on 4500 positions, 64 query heads on 8, head_dim 128:
+// 380 us (562 TFLOP/s); of 256, 384 and 512 tokens on up to 4500 positions each, 220
+// to 254 as the lengths fall out (some 300 TFLOP/s).  The chains of the softmax
+// (TMEM read, maximum, exponentials, TMEM write) and of the unpacking bound these,
+// at 1.8 instructions a cycle and SM, and the last wave's length: in the second case
+// 288 CTAs on 148 SMs, the tensor pipe busy for a quarter of the time.
 constexpr int kTcRows = 128, kTcStep = 64, kTcWarps = 17;
 constexpr int kTcTop = 12, kTcLow = -8;  // see E
 constexpr float kTcUp = 7.0f;  // the largest P lies in [2^7, 2^15], so that f16 has it to 2^-11 down to 2^-21 of that
@@ -1816,11 +1818,12 @@ Plan make_plan(const rq_kv4* c, const rq_kv4_query* a) {
     pl.mode = a->dtype != RQ_BF16 || rows <= 8 ? kSplit8 : kOne16;
     pl.R = pl.mode == kOne16 ? 16 : 8;
     // Where the many-rows forms win, few rows -> many rows (us, 8 heads a kv head of
-    // 8, head_dim 128): bf16 at 16 rows, 16 x 2048 keys 44 -> 42, 64 x 1024
-    // 77 -> 99, 1 x 40000 46 -> 50; at 24 rows 42 -> 42, 117 -> 100, 66 -> 51; at
-    // 128 rows 183 -> 43, 384 -> 105, 206 -> 55.  f32 at 32 rows 64 -> 94,
-    // 118 -> 152, 67 -> 86; at 48 rows 86 -> 101, 166 -> 156, 89 -> 88; at 64 rows
-    // 108 -> 107, 215 -> 161, 126 -> 90.
+    // 8, head_dim 128; other geometries follow the same rule): bf16 at 16 rows,
+    // 16 x 2048 keys 43 -> 41, 64 x 1024 74 -> 98, 1 x 40000 45 -> 49; at 24 rows
+    // 40 -> 41, 112 -> 98, 63 -> 50; at 128 rows 174 -> 42, 364 -> 104, 192 -> 54.
+    // f32 at 32 rows 65 -> 95, 118 -> 151, 68 -> 87; at 48 rows 87 -> 100, 166 -> 153,
+    // 91 -> 88; at 64 rows 109 -> 106, 216 -> 158, 129 -> 89; f16 within 5 % of f32.
+    // The rows are those that the caller announces (max_q), not those that are there.
     pl.rows = rows > (a->dtype == RQ_BF16 ? 16 : 48);
     const int64_t tiles_of_row = (rows + pl.R - 1) / pl.R;
     int64_t len = a->table_width * c->page_size;

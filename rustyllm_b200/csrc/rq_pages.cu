@@ -178,6 +178,8 @@ struct ReleaseP {
 
 // One CTA: the entries to give back are walked in order, a CTA's threads at a
 // time; those that are pages are numbered by a scan and appended to the ring.
+// Bound by the scan's barriers, four a run of 512 entries: 200 sequences that give
+// back 978 pages take 6 us, 16 with 1854 9, and 64 with 60237 200.
 __global__ void __launch_bounds__(kThreads) pages_release_kernel(const __grid_constant__ ReleaseP p) {
     pdl_wait();
     __shared__ int64_t first[kThreads + 1];
