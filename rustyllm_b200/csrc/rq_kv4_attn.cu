@@ -1156,8 +1156,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 // P crossed TMEM head_dim / 32 times, for 1.3 times the softmax's time.)  E is
 // that of 32 positions: their largest scale comes to [2^11, 2^12) -- so that 8 d
 // still is an f16 -- or stays below it with the power at its floor, and only scales
-// 2^26 times smaller than that lose bits.  A row keeps its own largest power of V
-// in sight and weighs the positions by 2^(E - that).  A value that
+// 2^26 times smaller than that lose bits.  A row's reference m follows the largest
+// s_j + E_j that it sees, and P is 2^(s_j + E_j - m): the products that count most
+// keep their bits beside values of any size that count little (with E's largest and
+// the scores' each followed for itself, one value of 5e5 without weight took 12 bits
+// from all weights: 75 % of an output made of weights of 2^-18).  A value that
 // is not a number cannot lie in an operand that rows share which do not see it:
 // it enters as zero, and the rows that do see it are marked and get it at the
 // end.
@@ -1182,8 +1185,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attn_rows_kernel(const __g
 //           this takes 2000)
 //
 // Three prompts of 512 tokens on 4500 positions, 64 query heads on 8, head_dim 128:
-// 380 us (562 TFLOP/s); of 256, 384 and 512 tokens on up to 4500 positions each, 220
-// to 254 as the lengths fall out (some 300 TFLOP/s).  The chains of the softmax
+// 377 us (567 TFLOP/s); of 256, 384 and 512 tokens on up to 4500 positions each, 220
+// to 252 as the lengths fall out (some 300 TFLOP/s).  The chains of the softmax
 // (TMEM read, maximum, exponentials, TMEM write) and of the unpacking bound these,
 // at 1.8 instructions a cycle and SM, and the last wave's length: in the second case
 // 288 CTAs on 148 SMs, the tensor pipe busy for a quarter of the time.
@@ -1218,7 +1221,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4][2], b_ops_full[kTcOps], b_ops_empty[kTcOps], b_s_full[2], b_s_empty[2],
         b_p_full[2], b_pv_done[2];
-    __shared__ float s_qs[kAllRows], s_m[2][kTcRows], s_l[2][kTcRows], s_bound[2][kTcRows];
+    __shared__ float s_qs[kAllRows], s_m[2][kTcRows], s_l[2][kTcRows];
     __shared__ float s_kf[kTcOps][2];  // of a step's half: 2^E of K, E of V, tiles that are there
     __shared__ int s_E[kTcOps][2], s_there[kTcOps][2], s_any_nan[kTcOps][2];
     __shared__ uint32_t s_nan[kTcOps][2][NB], s_bad[2][kTcRows];  // positions that are not numbers: of a step's half, by block
@@ -1499,7 +1502,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         const uint32_t s_at = lanes + 64 * h, p_at = lanes + kPCol + 32 * h, o_at = lanes + kOCol + HD * h;
         float m = -INFINITY, l = 0.0f;
         uint32_t bad = 0;  // blocks of O that a value which is not a number reaches
-        int E = kTcLow;
         const int mine = h >= groups ? 0 : PAIR ? steps : (steps + 1 - h) / 2;
         for (int n = 0; n < mine; n++) {
             const int k = PAIR ? n : 2 * n + h, ph = n & 1, os = k % kTcOps;
@@ -1518,14 +1520,13 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             if (lane == 0) mbar_arrive(smem_u32(&b_s_empty[h]));
             // ---- which of them the row sees
             uint32_t sees[2];
-            float f[2], mx = -INFINITY;
-            int e[2];
+            float f[2], e[2], mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const uint32_t there = (uint32_t)s_there[os][i];
                 const int at = j0 + 32 * i;
                 f[i] = fmaxf(qs * s_kf[os][i], 1.2e-38f);  // (times -inf of a masked place)
-                e[i] = s_E[os][i];
+                e[i] = (float)s_E[os][i];
                 const int hi = min(min(rpos + 1, o.held) - at, 32), lo = p.window > 0 ? max(rpos - p.window + 1 - at, 0) : 0;
                 sees[i] = (hi >= 32 ? 0xFFFFFFFFu : hi > 0 ? (1u << hi) - 1u : 0u) & (lo >= 32 ? 0u : 0xFFFFFFFFu << lo);
                 sees[i] &= (there & 1u ? 0xFFFFu : 0u) | (there & 2u ? 0xFFFF0000u : 0u);
@@ -1537,23 +1538,17 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(a[i][j]));
-                mx = fmaxf(mx, top * f[i]);
+                mx = fmaxf(mx, fmaf(top, f[i], e[i]));
             }
             if (s_any_nan[os][0] | s_any_nan[os][1]) {
                 for (int b = 0; b < NB; b++)
                     if ((s_nan[os][0][b] & sees[0]) | (s_nan[os][1][b] & sees[1])) bad |= 1u << b;
             }
-            const int e_top = max(e[0], e[1]);
-            // ---- move the row's power of V or its reference where they grew
+            // ---- move the row's reference where s + E grew
             float al = 1.0f;
-            if (mx > -INFINITY && e_top > E) {
-                al = __int_as_float((127 + E - e_top) << 23);
-                E = e_top;
-            }
             if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
-                const float d = m == -INFINITY ? 0.0f : ex2(m - mx);
-                al *= d;
-                l *= d;
+                al = m == -INFINITY ? 0.0f : ex2(m - mx);
+                l *= al;
                 m = mx;
             }
             // ---- P and O are free once the group's last products are done
@@ -1573,7 +1568,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float base = (m == -INFINITY ? 0.0f : m) + (float)(E - e[i]) - kTcUp;
+                const float base = (m == -INFINITY ? 0.0f : m) - e[i] - kTcUp;
                 float2 sum = make_float2(0.0f, 0.0f);
                 uint32_t pk[16];
 #pragma unroll
@@ -1585,7 +1580,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
                     pk[j] = pack(y.x, y.y);
                 }
                 tc::tmem_st16u(p_at + 16 * i, pk);
-                l = fmaf(sum.x + sum.y, __int_as_float((127 + E - e[i]) << 23), l);
+                l = fmaf(sum.x + sum.y, __int_as_float((127 - (int)e[i]) << 23), l);
             }
             tc::tmem_wait_st();
             tc::tmem_fence_before();
@@ -1595,11 +1590,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
         if (ok && mine > 0 && !mbar_wait(smem_u32(&b_pv_done[h]), (mine - 1) & 1)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok && lane == 0) atomicExch(p.err, 1);
-        float f0 = __int_as_float((127 + E) << 23), f1 = 0.0f;  // what the groups' O counts
+        float f0 = 1.0f, f1 = 0.0f;  // what the groups' O counts
         if constexpr (!PAIR) {  // the row's even and odd steps together
             s_m[h][row] = m;
             s_l[h][row] = l;
-            s_bound[h][row] = f0;
             s_bad[h][row] = bad;
             tc::tmem_fence_before();
             named_bar_sync(1 + q, 64);
@@ -1607,8 +1601,8 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) kv4_attn_tc_kernel(const __g
             const float w0 = weight(s_m[0][row], m), w1 = weight(s_m[1][row], m);
             l = s_l[0][row] * w0 + s_l[1][row] * w1;
             bad = s_bad[0][row] | s_bad[1][row];
-            f0 = s_bound[0][row] * w0;
-            f1 = s_bound[1][row] * w1;
+            f0 = w0;
+            f1 = w1;
         }
         tc::tmem_fence_after();
         const bool any = l != 0.0f;  // (not a number counts)

@@ -276,3 +276,22 @@ def test_scales_that_pass_f32_in_base_2_are_refused(gen):
         with pytest.raises(RqError, match="scale"):
             cache.attention(torch.zeros(1, 1, 32, device="cuda"), i32(0)[None], i32(1), scale=scale)
     assert not cache.attention(torch.zeros(1, 1, 32, device="cuda"), i32(0)[None], i32(1), scale=2.3e38).any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 21, 40])
+@pytest.mark.parametrize("at", [3, 70])
+def test_small_weights_count_beside_a_value_without_weight(gen, kind, nq, at):
+    """Most of the weight on a position without value, the rest on 240 others
+    at some 2^-18 of it, whose values make the output, and at `at` the largest
+    value that the cache can hold, without weight.  (Short enough that no form
+    splits the positions.)"""
+    n = 240
+    k, v = make(gen, n, 2, 64, kind)
+    k, v = (k.float() * 0.05).to(TYPES[kind]), v.abs()
+    q = torch.randn(nq, 8, 64, generator=gen, device="cuda").abs().to(TYPES[kind])
+    k[100], v[100] = 2, 0
+    k[at] = -20
+    v[at] = 6e4 if kind == "f16" else 5.2e5
+    s = Setup(gen, kind, n, nq, 2, 4, 64, k, v, q)
+    close(s.call(), s.want(), slice(None), kind)
